@@ -28,6 +28,28 @@ NN, TN, NT = 0, 1, 2
 _lib = None
 
 
+# Argument types of the entry points that asca_b200.ops calls with plain Python values (a pointer is an int or None): converted
+# by ctypes itself, at a fraction of the cost of wrapping each value.
+_P, _L, _I, _F, _Z = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_size_t
+_SIGNATURES = {
+    "asca_embed_scaled_fwd": (_I, [_P, _P, _P, _L, _L, _L, _F, _I, _I, _P]),
+    "asca_embed_scaled_bwd_ws": (_L, [_L, _L, _L]),
+    "asca_embed_scaled_bwd": (_I, [_P, _P, _P, _L, _L, _L, _F, _I, _I, _P, _P, _Z]),
+    "asca_gated_residual_rmsnorm_fwd": (_I, [_P, _P, _P, _P, _P, _L, _P, _I, _F, _F, _F, _L, _L, _I, _P, _P]),
+    "asca_gated_residual_rmsnorm_bwd_ws": (_L, [_P, _L, _L]),
+    "asca_gated_residual_rmsnorm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _P, _I, _F, _F, _F, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _Z]),
+    "asca_moe_topk_dispatch_ws": (_L, [_L, _L, _L]),
+    "asca_moe_topk_dispatch": (_I, [_P, _P, _L, _L, _L, _P, _P, _P, _P, _Z]),
+    "asca_moe_sort_rows": (_I, [_P, _P, _P, _L, _L, _L, _I, _I, _P]),
+    "asca_moe_unsort_rows": (_I, [_P, _P, _P, _P, _L, _L, _L, _I, _I, _P]),
+    "asca_moe_unsort_rows_bwd": (_I, [_P, _P, _P, _P, _P, _L, _L, _L, _I, _I, _P, _P]),
+    "asca_grad_norm_ws": (_L, [_P, _I]),
+    "asca_grad_norm": (_I, [_P, _P, _P, _P, _I, _P, _P, _Z]),
+    "asca_clip_grads": (_I, [_P, _P, _P, _P, _I, _P, _F]),
+    "asca_adamw_segmented_clip": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _F, _F, _F, _P, _P, _F]),
+}
+
+
 class AscaError(RuntimeError):
     """A library call returned a negative ASCA_ERR_* status."""
 
@@ -52,6 +74,9 @@ def load() -> C.CDLL:
         _lib.asca_graph_launch_count.restype = C.c_int64
         _lib.asca_delta_ckpt_floats.restype = C.c_int64
         _lib.asca_delta_ckpt_floats.argtypes = [C.c_int64] * 5
+        for name, (result, args) in _SIGNATURES.items():
+            fn = getattr(_lib, name)
+            fn.restype, fn.argtypes = result, args
     return _lib
 
 
@@ -155,12 +180,22 @@ class Gpu:
                                 "there is no CPU fallback")
         self._ctx = ctx
         self.device = device
+        self.bound_stream = 0   # the handle that set_stream was given last; 0 = the context's own stream
 
     # ---- plumbing
     def _call(self, name, *args):
         rc = getattr(self.lib, name)(*args)
         if rc != 0:
             raise AscaError(rc, self.lib.asca_last_error(self._ctx).decode())
+
+    def _fail(self, rc, msg=None):
+        raise AscaError(rc, msg or self.lib.asca_last_error(self._ctx).decode())
+
+    def _run(self, name, *args):
+        """An entry point with a row in _SIGNATURES, on plain Python values."""
+        rc = getattr(self.lib, name)(self._ctx, *args)
+        if rc != 0:
+            self._fail(rc)
 
     def describe(self) -> str:
         return self.lib.asca_describe(self._ctx).decode()
@@ -174,6 +209,7 @@ class Gpu:
 
     def set_stream(self, cuda_stream: int | None):
         self._call("asca_ctx_set_stream", self._ctx, C.c_void_p(cuda_stream or 0))
+        self.bound_stream = int(cuda_stream or 0)
 
     def use_torch_stream(self):
         import torch
@@ -521,6 +557,20 @@ class Model:
 
     def adamw_step(self, lr, beta1=0.9, beta2=0.95, eps=1e-8, wd=0.01):
         self.gpu._call("asca_model_adamw_step", self.gpu._ctx, self._h, _f(lr), _f(beta1), _f(beta2), _f(eps), _f(wd))
+
+    def grad_norm(self) -> float:
+        """The L2 norm of the whole gradient buffer."""
+        norm = C.c_float()
+        self.gpu._call("asca_model_grad_norm", self.gpu._ctx, self._h, C.byref(norm))
+        return norm.value
+
+    def adamw_step_clip(self, lr, max_norm, beta1=0.9, beta2=0.95, eps=1e-8, wd=0.01, want_norm=True):
+        """:meth:`adamw_step` with the gradient clipped to ``max_norm`` (the buffer itself stays as it is). Returns the norm before
+        clipping; without ``want_norm`` None, and the call does not wait for the device."""
+        norm = C.c_float() if want_norm else None
+        self.gpu._call("asca_model_adamw_step_clip", self.gpu._ctx, self._h, _f(lr), _f(beta1), _f(beta2), _f(eps), _f(wd), _f(max_norm),
+                       C.byref(norm) if want_norm else None)
+        return norm.value if want_norm else None
 
     def adamw_slices(self, lr, slices, advance=True, beta1=0.9, beta2=0.95, eps=1e-8, wd=0.01):
         """One optimizer step restricted to the sorted, disjoint (lo, hi) slices of the flat buffer (bf16 mode)."""

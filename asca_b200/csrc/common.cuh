@@ -213,6 +213,12 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
     return red[32];
 }
 
+// min(1, max_norm / (norm + 1e-6)), NaN where the norm is (grad_norm.cu, and the AdamW step that clips)
+__device__ __forceinline__ float asca_clip_coefficient(float norm, float max_norm) {
+    const float c = max_norm / (norm + 1e-6f);
+    return c > 1.0f ? 1.0f : c;
+}
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
 template <>

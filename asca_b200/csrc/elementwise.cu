@@ -5,6 +5,8 @@
 
 #include <cuda_bf16.h>
 
+#include <cmath>
+
 namespace {
 
 // ------------------------------------------------------------------ RMSNorm
@@ -255,12 +257,20 @@ __global__ void __launch_bounds__(256) adamw_kernel(float* __restrict__ p, const
 
 // One launch over a flat buffer of n_seg tensors with per-tensor lr_t / eps_t
 // (the counter advances per tensor, rust/src/tensor.rs:393).
+// CLIP: the gradient enters as clip * g, rounded once, and the update goes on from there as from any gradient: the product is kept
+// from being contracted into the moments, so that the step is bit for bit the plain one on a gradient clipped before.
+__device__ __forceinline__ float clipped(float g, float clip) {
+    float r = __fmul_rn(g, clip);
+    asm("" : "+f"(r));
+    return r;
+}
+template <bool CLIP>
 __device__ __forceinline__ void adamw_seg_body(float* __restrict__ p, const float* __restrict__ g,
                                                float* __restrict__ m, float* __restrict__ v,
                                                const int64_t* __restrict__ seg_off,
                                                const float* __restrict__ lr_t,
                                                const float* __restrict__ eps_t, int n_seg, float b1,
-                                               float b2, float wd, __nv_bfloat16* __restrict__ p16) {
+                                               float b2, float wd, __nv_bfloat16* __restrict__ p16, float clip = 1.0f) {
     const int64_t n = seg_off[n_seg];
     const int64_t stride = (int64_t)gridDim.x * blockDim.x * 4;
     const bool vec_ok = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m) |
@@ -276,7 +286,8 @@ __device__ __forceinline__ void adamw_seg_body(float* __restrict__ p, const floa
         if (i + 4 <= seg_off[s + 1] && vec_ok) {   // the common case: four elements of one tensor, 16-byte accesses
             float4 P = *reinterpret_cast<float4*>(p + i), M = *reinterpret_cast<float4*>(m + i),
                    V = *reinterpret_cast<float4*>(v + i);
-            const float4 G = *reinterpret_cast<const float4*>(g + i);
+            float4 G = *reinterpret_cast<const float4*>(g + i);
+            if (CLIP) G = make_float4(clipped(G.x, clip), clipped(G.y, clip), clipped(G.z, clip), clipped(G.w, clip));
             adamw_one(P.x, G.x, M.x, V.x, lr, b1, b2, ep, wd);
             adamw_one(P.y, G.y, M.y, V.y, lr, b1, b2, ep, wd);
             adamw_one(P.z, G.z, M.z, V.z, lr, b1, b2, ep, wd);
@@ -298,7 +309,7 @@ __device__ __forceinline__ void adamw_seg_body(float* __restrict__ p, const floa
                 lr = lr_t[s];
                 ep = eps_t[s];
             }
-            adamw_one(p[j], g[j], m[j], v[j], lr, b1, b2, ep, wd);
+            adamw_one(p[j], CLIP ? clipped(g[j], clip) : g[j], m[j], v[j], lr, b1, b2, ep, wd);
             if (p16) p16[j] = __float2bfloat16(p[j]);
         }
     }
@@ -309,7 +320,7 @@ __global__ void __launch_bounds__(256) adamw_seg_kernel(float* __restrict__ p, c
                                                         const float* __restrict__ lr_t,
                                                         const float* __restrict__ eps_t, int n_seg, float b1,
                                                         float b2, float wd, __nv_bfloat16* __restrict__ p16) {
-    adamw_seg_body(p, g, m, v, seg_off, lr_t, eps_t, n_seg, b1, b2, wd, p16);
+    adamw_seg_body<false>(p, g, m, v, seg_off, lr_t, eps_t, n_seg, b1, b2, wd, p16);
 }
 // The same with the segment table passed by value (up to 128 tensors): no host-to-device copy in front of the launch. A
 // copy would queue on a copy engine, behind whatever long peer-to-peer transfers the data-parallel exchange has in flight.
@@ -321,7 +332,25 @@ __global__ void __launch_bounds__(256) adamw_seg_tab_kernel(float* __restrict__ 
                                                             float* __restrict__ m, float* __restrict__ v,
                                                             const __grid_constant__ AdamSegTab tab, int n_seg, float b1,
                                                             float b2, float wd, __nv_bfloat16* __restrict__ p16) {
-    adamw_seg_body(p, g, m, v, tab.off, tab.lr, tab.eps, n_seg, b1, b2, wd, p16);
+    adamw_seg_body<false>(p, g, m, v, tab.off, tab.lr, tab.eps, n_seg, b1, b2, wd, p16);
+}
+// Both with the gradient clipped by its norm (grad_norm.cu), which is read on the device: no pass that rewrites the gradient
+// (8 bytes an element of the step's 28), and no wait for the norm on the host.
+__global__ void __launch_bounds__(256) adamw_seg_clip_kernel(float* __restrict__ p, const float* __restrict__ g,
+                                                             float* __restrict__ m, float* __restrict__ v,
+                                                             const int64_t* __restrict__ seg_off,
+                                                             const float* __restrict__ lr_t,
+                                                             const float* __restrict__ eps_t, int n_seg, float b1,
+                                                             float b2, float wd, __nv_bfloat16* __restrict__ p16,
+                                                             const float* __restrict__ norm, float max_norm) {
+    adamw_seg_body<true>(p, g, m, v, seg_off, lr_t, eps_t, n_seg, b1, b2, wd, p16, asca_clip_coefficient(*norm, max_norm));
+}
+__global__ void __launch_bounds__(256) adamw_seg_tab_clip_kernel(float* __restrict__ p, const float* __restrict__ g,
+                                                                 float* __restrict__ m, float* __restrict__ v,
+                                                                 const __grid_constant__ AdamSegTab tab, int n_seg, float b1,
+                                                                 float b2, float wd, __nv_bfloat16* __restrict__ p16,
+                                                                 const float* __restrict__ norm, float max_norm) {
+    adamw_seg_body<true>(p, g, m, v, tab.off, tab.lr, tab.eps, n_seg, b1, b2, wd, p16, asca_clip_coefficient(*norm, max_norm));
 }
 
 inline bool warp_rows_ok(int64_t cols, const void* a, const void* b) {
@@ -449,18 +478,34 @@ int asca_adamw(asca_ctx* ctx, float* p, const float* g, float* m, float* v, int6
     return ASCA_OK;
 }
 
-int asca_adamw_segmented_cast(asca_ctx* ctx, float* p, const float* g, float* m, float* v, const int64_t* seg_off,
-                              const float* lr_t, const float* eps_t, int n_seg, float beta1, float beta2, float wd_eff,
-                              void* p_bf16);
+static int adamw_segmented(asca_ctx* ctx, float* p, const float* g, float* m, float* v, const int64_t* seg_off,
+                           const float* lr_t, const float* eps_t, int n_seg, float beta1, float beta2, float wd_eff,
+                           void* p_bf16, const float* norm, float max_norm);
 
 int asca_adamw_segmented(asca_ctx* ctx, float* p, const float* g, float* m, float* v, const int64_t* seg_off,
                          const float* lr_t, const float* eps_t, int n_seg, float beta1, float beta2, float wd_eff) {
-    return asca_adamw_segmented_cast(ctx, p, g, m, v, seg_off, lr_t, eps_t, n_seg, beta1, beta2, wd_eff, nullptr);
+    return adamw_segmented(ctx, p, g, m, v, seg_off, lr_t, eps_t, n_seg, beta1, beta2, wd_eff, nullptr, nullptr, 0.0f);
 }
 
 int asca_adamw_segmented_cast(asca_ctx* ctx, float* p, const float* g, float* m, float* v, const int64_t* seg_off,
                               const float* lr_t, const float* eps_t, int n_seg, float beta1, float beta2, float wd_eff,
                               void* p_bf16) {
+    return adamw_segmented(ctx, p, g, m, v, seg_off, lr_t, eps_t, n_seg, beta1, beta2, wd_eff, p_bf16, nullptr, 0.0f);
+}
+
+int asca_adamw_segmented_clip(asca_ctx* ctx, float* p, const float* g, float* m, float* v, const int64_t* seg_off,
+                              const float* lr_t, const float* eps_t, int n_seg, float beta1, float beta2, float wd_eff,
+                              void* p_bf16, const float* norm, float max_norm) {
+    if (!ctx) return ASCA_ERR_ARG;
+    ASCA_REQUIRE(ctx, norm && max_norm > 0.0f && std::isfinite(max_norm), "adamw_segmented_clip: needs the norm and a positive, finite largest one");
+    return adamw_segmented(ctx, p, g, m, v, seg_off, lr_t, eps_t, n_seg, beta1, beta2, wd_eff, p_bf16, norm, max_norm);
+}
+
+}  // extern "C"
+
+static int adamw_segmented(asca_ctx* ctx, float* p, const float* g, float* m, float* v, const int64_t* seg_off,
+                           const float* lr_t, const float* eps_t, int n_seg, float beta1, float beta2, float wd_eff,
+                           void* p_bf16, const float* norm, float max_norm) {
     if (!ctx) return ASCA_ERR_ARG;
     ASCA_REQUIRE(ctx, (reinterpret_cast<uintptr_t>(p_bf16) & 7) == 0, "adamw_segmented: bf16 copy must be 8-byte aligned");
     ASCA_REQUIRE(ctx, p && g && m && v && seg_off && lr_t && eps_t && n_seg > 0, "adamw_segmented: bad arguments");
@@ -476,7 +521,11 @@ int asca_adamw_segmented_cast(asca_ctx* ctx, float* p, const float* g, float* m,
         for (int i = 0; i <= n_seg; ++i) tab.off[i] = seg_off[i];
         for (int i = 0; i < n_seg; ++i) tab.lr[i] = lr_t[i], tab.eps[i] = eps_t[i];
         asca_span sp(ctx, "adamw_seg_kernel", (double)n * (p_bf16 ? 30.0 : 28.0));   // bytes read + written
-        adamw_seg_tab_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(p, g, m, v, tab, n_seg, beta1, beta2, wd_eff, (__nv_bfloat16*)p_bf16);
+        if (norm)
+            adamw_seg_tab_clip_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(p, g, m, v, tab, n_seg, beta1, beta2, wd_eff, (__nv_bfloat16*)p_bf16,
+                                                                                 norm, max_norm);
+        else
+            adamw_seg_tab_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(p, g, m, v, tab, n_seg, beta1, beta2, wd_eff, (__nv_bfloat16*)p_bf16);
         ASCA_CHECK_LAUNCH(ctx);
         return ASCA_OK;
     }
@@ -490,11 +539,14 @@ int asca_adamw_segmented_cast(asca_ctx* ctx, float* p, const float* g, float* m,
     ASCA_CUDA(ctx, cudaMemcpyAsync(w + off_b + f_b, eps_t, f_b, cudaMemcpyHostToDevice, ctx->stream));
     // pageable host arrays: the copies above have been staged by the time they return
     asca_span sp(ctx, "adamw_seg_kernel", (double)n * (p_bf16 ? 30.0 : 28.0));   // bytes read + written
-    adamw_seg_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(p, g, m, v, (const int64_t*)w, (const float*)(w + off_b),
-                                                                 (const float*)(w + off_b + f_b), n_seg, beta1, beta2,
-                                                                 wd_eff, (__nv_bfloat16*)p_bf16);
+    if (norm)
+        adamw_seg_clip_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(p, g, m, v, (const int64_t*)w, (const float*)(w + off_b),
+                                                                         (const float*)(w + off_b + f_b), n_seg, beta1, beta2,
+                                                                         wd_eff, (__nv_bfloat16*)p_bf16, norm, max_norm);
+    else
+        adamw_seg_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(p, g, m, v, (const int64_t*)w, (const float*)(w + off_b),
+                                                                     (const float*)(w + off_b + f_b), n_seg, beta1, beta2,
+                                                                     wd_eff, (__nv_bfloat16*)p_bf16);
     ASCA_CHECK_LAUNCH(ctx);
     return ASCA_OK;
 }
-
-}  // extern "C"

@@ -5,6 +5,7 @@
 #include "common.cuh"
 
 #include <algorithm>
+#include <cmath>
 #include <cstddef>
 #include <cstring>
 #include <initializer_list>
@@ -1433,6 +1434,7 @@ int asca_model_destroy(asca_ctx* ctx, asca_model* m) {
     if (m->dec_w) cudaFree(m->dec_w);
     if (m->dec_b) cudaFree(m->dec_b);
     if (m->dec_pk) cudaFree(m->dec_pk);
+    if (m->norm) cudaFree(m->norm);
     delete m;
     return ASCA_OK;
 }
@@ -1542,8 +1544,7 @@ int asca_model_forward_backward_host(asca_ctx* ctx, asca_model* m, const uint32_
     return forward_backward_f32(ctx, m, ids_h, tg_h, B, T, loss_h, logits_h);
 }
 
-int asca_model_adamw_step(asca_ctx* ctx, asca_model* m, float lr, float beta1, float beta2, float eps, float wd) {
-    if (!ctx || !m) return ASCA_ERR_ARG;
+static int adamw_step(asca_ctx* ctx, asca_model* m, float lr, float beta1, float beta2, float eps, float wd, const float* norm, float max_norm) {
     ASCA_TRY(materialize_zero_grads(ctx, m));
     const int n_seg = (int)m->seg_off.size() - 1;
     std::vector<float> lr_t(n_seg), eps_t(n_seg);
@@ -1567,8 +1568,53 @@ int asca_model_adamw_step(asca_ctx* ctx, asca_model* m, float lr, float beta1, f
     m->params16_stale = !fuse;
     m->dec_stale = true;
     m->dec_pk_stale = true;
+    void* p16 = fuse ? (void*)m->params16 : nullptr;
+    if (norm)
+        return asca_adamw_segmented_clip(ctx, m->params, m->grads, m->m, m->v, m->seg_off.data(), lr_t.data(), eps_t.data(), n_seg,
+                                         beta1, beta2, lr * wd, p16, norm, max_norm);
     return asca_adamw_segmented_cast(ctx, m->params, m->grads, m->m, m->v, m->seg_off.data(), lr_t.data(), eps_t.data(), n_seg,
-                                     beta1, beta2, lr * wd, fuse ? (void*)m->params16 : nullptr);
+                                     beta1, beta2, lr * wd, p16);
+}
+
+int asca_model_adamw_step(asca_ctx* ctx, asca_model* m, float lr, float beta1, float beta2, float eps, float wd) {
+    if (!ctx || !m) return ASCA_ERR_ARG;
+    return adamw_step(ctx, m, lr, beta1, beta2, eps, wd, nullptr, 0.0f);
+}
+
+// The norm of the flat gradient buffer, on the device in m->norm (scratch behind it).
+static int model_grad_norm(asca_ctx* ctx, asca_model* m, const char* who) {
+    // (an attached communicator reduces the buffer in parts, some of which then hold this rank's chunk alone)
+    if (m->dp) return asca_fail(ctx, ASCA_ERR_UNSUPPORTED, "%s: not with a communicator attached", who);
+    ASCA_TRY(materialize_zero_grads(ctx, m));
+    const size_t ws = (size_t)asca_grad_norm_ws(ctx, 1);
+    if (!m->norm && cudaMalloc((void**)&m->norm, 256 + ws) != cudaSuccess) {
+        m->norm = nullptr;
+        cudaGetLastError();
+        return asca_fail(ctx, ASCA_ERR_OOM, "%s: cannot allocate %zu bytes", who, 256 + ws);
+    }
+    void* g = m->grads;
+    const int dtype = ASCA_F32;
+    return asca_grad_norm(ctx, &g, &m->n_params, &dtype, 1, m->norm, m->norm + 64, ws);
+}
+
+int asca_model_grad_norm(asca_ctx* ctx, asca_model* m, float* norm) {
+    if (!ctx || !m) return ASCA_ERR_ARG;
+    ASCA_REQUIRE(ctx, norm, "model_grad_norm: null pointer");
+    ASCA_TRY(model_grad_norm(ctx, m, "model_grad_norm"));
+    asca_stage_scope staged(ctx);
+    ASCA_TRY(asca_copy_out(ctx, norm, m->norm, sizeof(float)));
+    return asca_ctx_sync(ctx);
+}
+
+int asca_model_adamw_step_clip(asca_ctx* ctx, asca_model* m, float lr, float beta1, float beta2, float eps, float wd, float max_norm, float* norm) {
+    if (!ctx || !m) return ASCA_ERR_ARG;
+    ASCA_REQUIRE(ctx, max_norm > 0.0f && std::isfinite(max_norm), "model_adamw_step_clip: the largest norm has to be positive and finite");
+    ASCA_TRY(model_grad_norm(ctx, m, "model_adamw_step_clip"));
+    ASCA_TRY(adamw_step(ctx, m, lr, beta1, beta2, eps, wd, m->norm, max_norm));
+    if (!norm) return ASCA_OK;
+    asca_stage_scope staged(ctx);
+    ASCA_TRY(asca_copy_out(ctx, norm, m->norm, sizeof(float)));
+    return asca_ctx_sync(ctx);
 }
 
 // One optimizer step restricted to n sorted, disjoint slices [lo[i], hi[i]) of the flat buffer (a rank's share under a

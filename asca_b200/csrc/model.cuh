@@ -64,6 +64,7 @@ struct asca_model {
     std::vector<int64_t> seg_off;   // tensor offsets in parameter order, + total
     float *params = nullptr, *grads = nullptr, *m = nullptr, *v = nullptr;
     uint32_t adam_counter = 0;
+    float* norm = nullptr;               // device: the last gradient norm, and the scratch of taking it (from the first call that asks)
     int compute = ASCA_F32;              // ASCA_BF16: tensor-core products on a bf16 copy of the weights
     __nv_bfloat16* params16 = nullptr;   // refreshed from the f32 master copy whenever that changed
     bool params16_stale = true;

@@ -218,6 +218,7 @@ class TrainCfg:
     lr: float = 3e-3
     warmup: int = 0
     save_every: int = 0
+    max_norm: float = 0.0   # > 0: the gradient is clipped to this norm (the reference's trainer does not clip)
 
 
 class Trainer:
@@ -234,7 +235,10 @@ class Trainer:
         self.model.zero_grads()
         ids, tgts = self.data.batch_seqs(self.rng, c.seq_len, c.batch, "train")
         loss = self.model.forward_backward(ids, tgts, c.batch)
-        self.model.adamw_step(lr)
+        if c.max_norm > 0:
+            self.grad_norm = self.model.adamw_step_clip(lr, c.max_norm)   # before clipping
+        else:
+            self.model.adamw_step(lr)
         self.step += 1
         return loss
 

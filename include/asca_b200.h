@@ -127,6 +127,28 @@ int asca_rmsnorm_bwd_host(asca_ctx* ctx, const float* x, const float* dy, float*
 int asca_residual_rmsnorm(asca_ctx* ctx, const float* x, const float* y, float* x_mid, float* xn,
                           int64_t rows, int64_t cols, float eps);
 
+/* ------------------------------------------------------------------ norms around a block, gate and residual scale
+ * (no counterpart in the reference, whose norms have no gain and whose residual has no gate)
+ *   n     = post_norm ? rmsnorm(y) * w_post : y                      the norm after the block, y its output
+ *   x_out = skip_scale * x + branch_scale * gate[r / gate_rows] * n  the residual stream
+ *   xn    = rmsnorm(x_out) * w_pre                                   the norm before the next block
+ * y, xn and their gradients are `dtype`; the residual stream, gains, gates and their gradients are f32. gate has
+ * ceil(rows / gate_rows) rows of `cols`: gate_rows = rows is one gate for all tokens, gate_rows = T one a sequence, 1 one a
+ * token. w_post, gate, w_pre nullable (ones); xn nullable (residual only); x_out may be x. cols <= 8192.
+ * Backward, from d_xn (nullable) and d_out (nullable: the gradient that reaches x_out from further on; one of the two is
+ * needed): d_x, d_y, and where their pointers are given d_w_post, d_gate, d_w_pre, which `accumulate` adds to instead of
+ * overwriting. The sums over rows run in a fixed order. d_x may be d_out, d_y may be d_xn. ws: asca_gated_residual_rmsnorm_bwd_ws
+ * bytes of device scratch, 256-byte aligned, the caller's until the call's work has run. */
+int asca_gated_residual_rmsnorm_fwd(asca_ctx* ctx, const void* y, const float* x, const float* w_post, const float* gate,
+                                    int64_t gate_rows, const float* w_pre, int post_norm, float skip_scale, float branch_scale,
+                                    float eps, int64_t rows, int64_t cols, int dtype, float* x_out, void* xn);
+int64_t asca_gated_residual_rmsnorm_bwd_ws(asca_ctx* ctx, int64_t rows, int64_t cols);
+int asca_gated_residual_rmsnorm_bwd(asca_ctx* ctx, const void* y, const float* x_out, const void* d_xn, const float* d_out,
+                                    const float* w_post, const float* gate, int64_t gate_rows, const float* w_pre,
+                                    int post_norm, float skip_scale, float branch_scale, float eps, int64_t rows, int64_t cols,
+                                    int dtype, int accumulate, float* d_x, void* d_y, float* d_w_post, float* d_gate,
+                                    float* d_w_pre, void* ws, size_t ws_bytes);
+
 /* ------------------------------------------------------------------ gather / scatter
  * Gpu::gather_rows (rust/src/cuda/mod.rs:1156-1187): dst[r,:] = src[idx[r],:];
  * Gpu::scatter_rows (:1190-1221): dst[idx[r],:] = src[r,:] (overwrite). idx is int32. */
@@ -156,8 +178,27 @@ int asca_adamw_segmented(asca_ctx* ctx, float* p, const float* g, float* m, floa
 int asca_adamw_segmented_cast(asca_ctx* ctx, float* p, const float* g, float* m, float* v,
                               const int64_t* seg_off, const float* lr_t, const float* eps_t, int n_seg,
                               float beta1, float beta2, float wd_eff, void* p_bf16);
+/* Same update with the gradient entering as min(1, max_norm / (norm + 1e-6)) * g: clipping by the norm that asca_grad_norm has
+ * left in device memory, without a pass that rewrites the gradient. p_bf16 nullable; max_norm > 0 and finite. */
+int asca_adamw_segmented_clip(asca_ctx* ctx, float* p, const float* g, float* m, float* v,
+                              const int64_t* seg_off, const float* lr_t, const float* eps_t, int n_seg,
+                              float beta1, float beta2, float wd_eff, void* p_bf16, const float* norm, float max_norm);
 int asca_adamw_host(asca_ctx* ctx, float* p, const float* g, float* m, float* v, int64_t n,
                     float lr_t, float beta1, float beta2, float eps_t, float wd_eff);
+
+/* ------------------------------------------------------------------ gradient norm and clipping (no counterpart in the reference)
+ * asca_grad_norm: *norm (device float) = sqrt of the sum of squares over all elements of `count` tensors (device addresses,
+ * element counts and dtypes in HOST arrays, read before the call returns; f32 and bf16 may be mixed, tensors may be empty and
+ * begin at any element). Squares are added in 64 bits, in a fixed order. ws: asca_grad_norm_ws bytes of device scratch, 8-byte
+ * aligned, the caller's until the call's work has run; calls with scratch of their own may overlap, captured and replayed
+ * ones included.
+ * asca_clip_grads: g *= min(1, max_norm / (norm + 1e-6)) in place, norm read on the device; nothing is written where the factor
+ * is 1. Tensors must not overlap. max_norm >= 0 and finite. A norm that is not finite follows the formula (factor 0, or NaN). */
+int64_t asca_grad_norm_ws(asca_ctx* ctx, int count);
+int asca_grad_norm(asca_ctx* ctx, void* const* grads, const int64_t* n, const int* dtype, int count, float* norm,
+                   void* ws, size_t ws_bytes);
+int asca_clip_grads(asca_ctx* ctx, void* const* grads, const int64_t* n, const int* dtype, int count, const float* norm,
+                    float max_norm);
 
 /* ------------------------------------------------------------------ delta rule (D1, D2, D4)
  * Forward scan: Gpu::delta_scan (rust/src/cuda/mod.rs:1253-1321), recurrence of
@@ -301,6 +342,35 @@ int asca_moe_step(asca_ctx* ctx, const float* x, const uint32_t* ids, const void
                   const float* b1, const void* w2, const float* b2, int64_t n_streams, int64_t d,
                   int64_t F, int64_t E, int dtype, float* out);
 
+/* Tokens sorted by the experts a router chose for them (no counterpart in the reference, whose routing is the hash above and has one
+ * expert a token). Assignment a = t*K + k gives token t to experts[t, k] (int32, device); an expert at or past E as unsigned, -1
+ * among them, sends the assignment nowhere (padding).
+ *   perm    (N*K) the assignments by expert, ascending inside one; those that go nowhere behind them
+ *   offsets (E+1) the experts' bounds in perm -- what asca_moe_fwd takes; offsets[E] = assignments that go somewhere
+ *   slot    (N, K) the inverse: where assignment a lies in perm, -1 if it goes nowhere
+ * Integer only. At most 2048 experts. ws: asca_moe_topk_dispatch_ws bytes of device scratch, 256-byte aligned, the caller's
+ * until the call's work has run. */
+int64_t asca_moe_topk_dispatch_ws(int64_t N, int64_t K, int64_t E);
+int asca_moe_topk_dispatch(asca_ctx* ctx, const int32_t* experts, int64_t N, int64_t K, int64_t E, int32_t* perm,
+                           int32_t* offsets, int32_t* slot, void* ws, size_t ws_bytes);
+/* The rows moved there and back, and their gradients. Rows of the sorted side (xs, ys, d_xs, d_ys: N*K x d) at and behind
+ * offsets[E] are neither read nor written. Each side has a dtype of its own; sums are f32 in the order of k.
+ *   asca_moe_sort_rows        xs[slot[t,k]] = x[t]
+ *   asca_moe_sort_rows_bwd    d_x[t] = sum_k d_xs[slot[t,k]]
+ *   asca_moe_unsort_rows      out[t] = sum_k weights[t,k] ys[slot[t,k]]      (weights nullable: ones)
+ *   asca_moe_unsort_rows_bwd  d_ys[slot[t,k]] = weights[t,k] d_out[t]; d_w[t,k] = <d_out[t], ys[slot[t,k]]>, 0 where the
+ *                             assignment goes nowhere (d_w nullable, ys then too; d_ys may be ys)
+ * The sorted rows with the identity as permutation are what asca_moe_fwd / asca_moe_bwd take as N*K tokens; d_b2 of the latter is a
+ * sum over all N*K rows, so the rows of dout behind offsets[E] have to be zero there. */
+int asca_moe_sort_rows(asca_ctx* ctx, const void* x, const int32_t* slot, int64_t N, int64_t K, int64_t d, int x_dtype,
+                       int xs_dtype, void* xs);
+int asca_moe_sort_rows_bwd(asca_ctx* ctx, const void* d_xs, const int32_t* slot, int64_t N, int64_t K, int64_t d, int xs_dtype,
+                           int x_dtype, void* d_x);
+int asca_moe_unsort_rows(asca_ctx* ctx, const void* ys, const int32_t* slot, const float* weights, int64_t N, int64_t K,
+                         int64_t d, int ys_dtype, int out_dtype, void* out);
+int asca_moe_unsort_rows_bwd(asca_ctx* ctx, const void* d_out, const void* ys, const int32_t* slot, const float* weights,
+                             int64_t N, int64_t K, int64_t d, int out_dtype, int ys_dtype, void* d_ys, float* d_w);
+
 typedef struct asca_moe_dev asca_moe_dev;
 /* Host forms. `ids` replaces the reference's host-built `buckets` argument (the library
  * builds the same buckets on the device). */
@@ -343,6 +413,16 @@ int asca_embed_fwd(asca_ctx* ctx, const float* table, const uint32_t* ids, int64
                    float* x);
 int asca_embed_bwd(asca_ctx* ctx, const float* dx, const uint32_t* ids, int64_t N, int64_t d,
                    int64_t vocab, float* d_table);
+/* The same with a scale, for tables of any size (the gradient above reads every id for every row of the table) and either dtype
+ * (no counterpart in the reference): x[t] = scale * table[ids[t]]; d_table[v] (f32) = scale * sum over tokens with ids[t] == v of
+ * dx[t] (`dtype`), or += with `accumulate`, which touches the rows of the tokens that occur and no other. An id at or past vocab
+ * (as unsigned) is padding: a row of zeros, no part of any sum. The tokens are sorted by id; the sums run in a fixed order.
+ * ws: asca_embed_scaled_bwd_ws bytes of device scratch, 256-byte aligned, the caller's until the call's work has run. */
+int asca_embed_scaled_fwd(asca_ctx* ctx, const void* table, const uint32_t* ids, int64_t N, int64_t d, int64_t vocab,
+                          float scale, int table_dtype, int out_dtype, void* x);
+int64_t asca_embed_scaled_bwd_ws(int64_t N, int64_t d, int64_t vocab);
+int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, int64_t N, int64_t d, int64_t vocab, float scale,
+                          int dtype, int accumulate, float* d_table, void* ws, size_t ws_bytes);
 
 /* Host forms of the head / loss / optimizer methods of `impl Gpu`:
  *   asca_head_forward_dev_host   Gpu::head_forward_dev (rust/src/cuda/mod.rs:828-846): logits = h_final (T,d) x head
@@ -436,6 +516,13 @@ int asca_model_forward_backward_host(asca_ctx* ctx, asca_model* m, const uint32_
  * rust/src/tensor.rs:396-402. One segmented launch. */
 int asca_model_adamw_step(asca_ctx* ctx, asca_model* m, float lr, float beta1, float beta2, float eps,
                           float wd);
+/* The gradient norm of the whole buffer (asca_grad_norm), and the optimizer step that clips by it: the gradient enters as
+ * min(1, max_norm / (norm + 1e-6)) * grads, the buffer itself is left as it is. norm: host float; nullable in the second, which then
+ * does not wait for the device. ASCA_ERR_UNSUPPORTED while a communicator is attached (asca_model_dp_attach). No counterpart in
+ * the reference, whose trainer does not clip. */
+int asca_model_grad_norm(asca_ctx* ctx, asca_model* m, float* norm);
+int asca_model_adamw_step_clip(asca_ctx* ctx, asca_model* m, float lr, float beta1, float beta2, float eps, float wd,
+                               float max_norm, float* norm);
 /* Sharded optimizer support (bf16 compute mode, unpadded bf16 copy). asca_model_adamw_slices is one optimizer step
  * restricted to n sorted, disjoint slices [lo[i], hi[i]) of the flat buffer -- a rank's parts of the large tensors
  * plus the small tensors every rank updates; every tensor gets the step number asca_model_adamw_step would give
