@@ -5,115 +5,348 @@
 // An id at or past the vocabulary (as unsigned: -1 is one) is padding: a row of zeros forward, no part of any sum backward.
 //
 // Backward. The tokens are sorted by id (stable_sort.cuh), so that the rows of one id lie in one run of the sorted order, in token
-// order. The order is cut into pieces of `piece` rows; a thread owns four columns of a piece and walks down it with the running sum
-// in registers, and a run that lies inside its piece goes straight into the table. A run over several pieces leaves one partial sum
-// a piece (at most two of a piece belong to such runs: the one that comes in from the left and the one that goes on to the right),
-// which a second launch adds in order. Nothing depends on the order in which blocks run. Bound by HBM: dx is read once, the table
-// written once; a scan of all ids for every row of the table, as asca_embed_bwd does it, reads N * V ids.
+// order. The order is cut into pieces; a thread owns a few columns of a piece and walks down it with the running sum in registers,
+// and a run that lies inside its piece goes straight into the table. A run over several pieces leaves one partial sum a piece (at
+// most two of a piece belong to such runs: the one that comes in from the left and the one that goes on to the right), which a last
+// launch adds, eight lanes a column. Where the table is overwritten, blocks among the pieces' write the zeros of the rows that
+// no token has: every row of the table is written once. Nothing depends on the order in which blocks run. Bound by HBM: dx is read
+// once and the table written once; a scan of all ids for every row of the table, as asca_embed_bwd does it, reads N * V ids.
 #include "row_io.cuh"
 #include "stable_sort.cuh"
 
 namespace {
 
-template <int V, typename TT, typename TX>
+// A thread has its columns of TOKENS rows in flight.
+constexpr int TOKENS = 4;
+template <int W, typename TT, typename TX>
 __global__ void __launch_bounds__(256) embed_scaled_fwd_kernel(const TT* __restrict__ table, const uint32_t* __restrict__ ids, int64_t N, int d,
                                                                uint32_t vocab, float scale, TX* __restrict__ x) {
-    const int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    if (r >= N) return;
-    const uint32_t id = ids[r];
-    const bool live = id < vocab;
-    const TT* src = table + (int64_t)(live ? id : 0) * d;
-    TX* dst = x + r * (int64_t)d;
-    for (int c = threadIdx.x * V; c < d; c += blockDim.x * V) {
-        float v[V];
-        if (live) ld_row<V>(src + c, v);
+    using F = frag<W, TT>;
+    const int lanes = blockDim.x;
+    const int64_t r0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * TOKENS;
+    uint32_t id[TOKENS];
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = live ? scale * v[i] : 0.0f;
-        st_row<V>(dst + c, v);
+    for (int i = 0; i < TOKENS; ++i) id[i] = r0 + i < N ? ids[r0 + i] : 0xffffffffu;
+    for (int c = frag_first<W>(threadIdx.x); c < d; c += lanes * F::E) {
+        F r[TOKENS];
+#pragma unroll
+        for (int i = 0; i < TOKENS; ++i)
+            if (id[i] < vocab) r[i].load(table + (int64_t)id[i] * d, c, lanes, d);
+#pragma unroll
+        for (int i = 0; i < TOKENS; ++i) {
+            if (r0 + i >= N) break;
+            float v[F::E] = {};
+            if (id[i] < vocab) {
+                r[i].get(v);
+#pragma unroll
+                for (int j = 0; j < F::E; ++j) v[j] *= scale;
+            }
+            frag<W, TX>::put(x + (r0 + i) * d, c, lanes, d, v);
+        }
     }
 }
 
-template <int V>
-__device__ __forceinline__ void add_row(float* p, const float (&v)[V], float scale, int accumulate) {
-    float o[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = scale * v[i];
+// p[columns] = scale * v, or += with accumulate
+template <int W>
+__device__ __forceinline__ void add_row(float* row, int c, int lanes, int d, const float (&v)[frag<W, float>::E], float scale, int accumulate) {
+    constexpr int E = frag<W, float>::E;
+    float o[E], t[E];
     if (accumulate) {
-        float t[V];
-        ld_row<V>(p, t);
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] += t[i];
+        frag<W, float> r;
+        r.load(row, c, lanes, d);
+        r.get(t);
     }
-    st_row<V>(p, o);
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = accumulate ? t[i] + scale * v[i] : scale * v[i];
+    frag<W, float>::put(row, c, lanes, d, o);
 }
 
-// part[piece][0]: the sum of a run that came in from the left; part[piece][1]: of a run that begins here and goes on to the right
-template <int V, typename T>
-__global__ void __launch_bounds__(128) embed_pieces_kernel(const T* __restrict__ dx, const uint32_t* __restrict__ keys, const int32_t* __restrict__ items,
-                                                           int64_t N, int d, uint32_t vocab, float scale, int accumulate, int piece,
-                                                           float* __restrict__ d_table, float* __restrict__ part) {
-    const int64_t p = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    const int64_t lo = p * piece;
-    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
-    if (lo >= N || c >= d) return;
-    const int64_t hi = lo + piece < N ? lo + piece : N;
-    uint32_t key = keys[lo];
-    bool from_left = lo > 0 && keys[lo - 1] == key;
-    float acc[V] = {};
-    for (int64_t i = lo; i < hi && key < vocab; ) {
-        float v[V];
-        ld_row<V>(dx + (int64_t)items[i] * d + c, v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] += v[j];
-        ++i;
-        const uint32_t next = i < N ? keys[i] : 0xffffffffu;
-        if (next == key && i < hi) continue;
-        const bool to_right = next == key;   // (i == hi then)
-        if (from_left || to_right) st_row<V>(part + (2 * p + (from_left ? 0 : 1)) * d + c, acc);
-        else add_row<V>(d_table + (int64_t)key * d + c, acc, scale, accumulate);
-#pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] = 0.0f;
-        key = next;
-        from_left = false;
+constexpr int MOST_PIECE = 64, AHEAD = 8, ZERO_ROWS = 32;
+
+struct Sum {
+    const void* dx;
+    const uint32_t* keys;   // sorted
+    const int32_t* items;
+    int64_t N;
+    int d, piece, accumulate;
+    uint32_t vocab;
+    float scale;
+    float *d_table, *part;
+    int64_t sums, zeros;    // blocks of the two kinds; they take turns in the grid
+};
+
+// The first place in the sorted keys that is not below v.
+__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t v) {
+    int64_t lo = 0;
+    while (n > 0) {
+        const int64_t half = n >> 1;
+        if (keys[lo + half] < v) {
+            lo += half + 1;
+            n -= half + 1;
+        } else n = half;
+    }
+    return lo;
+}
+
+// ZERO_ROWS rows of the table: those without a token are cleared.
+template <int W>
+__device__ __forceinline__ void zero_rows(const Sum& a, int64_t block) {
+    const int lane = threadIdx.x + threadIdx.y * blockDim.x, threads = blockDim.x * blockDim.y;
+    const int64_t v = block * ZERO_ROWS + (lane & 31);
+    bool none = false;
+    if (v < a.vocab) {
+        const int64_t at = lower_bound(a.keys, a.N, (uint32_t)v);
+        none = at == a.N || a.keys[at] != v;
+    }
+    const unsigned rows = __ballot_sync(0xffffffffu, none);   // (each warp looks for itself)
+    using F = frag<W, float>;
+    const float zero[F::E] = {};
+    for (unsigned left = rows; left; left &= left - 1) {
+        float* p = a.d_table + (block * ZERO_ROWS + __ffs(left) - 1) * a.d;
+        for (int c = frag_first<W>(lane); c < a.d; c += threads * F::E) F::put(p, c, threads, a.d, zero);
     }
 }
 
-// A block owns a piece and some columns; it has work where a run begins in the piece and goes on past it.
-template <int V>
-__global__ void __launch_bounds__(128) embed_join_kernel(const uint32_t* __restrict__ keys, int64_t N, int d, uint32_t vocab, float scale, int accumulate,
-                                                         int piece, const float* __restrict__ part, float* __restrict__ d_table) {
-    const int64_t p = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+// part[piece][0]: the sum of a run that came in from the left; part[piece][1]: of a run that begins here and goes on to the right.
+// A thread owns some columns of a piece; AHEAD rows are asked for before the first of them is added.
+template <int W, typename T>
+__global__ void __launch_bounds__(128) embed_pieces_kernel(const Sum a) {
+    extern __shared__ uint32_t sh[];   // [block's pieces][key before, keys of the piece, key behind; items]
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t all = a.sums + a.zeros, before = (int64_t)blockIdx.x * a.zeros / all;   // zeroing blocks in front of this one
+    if ((int64_t)(blockIdx.x + 1) * a.zeros / all > before) {
+        zero_rows<W>(a, before);
+        return;
+    }
+    using F = frag<W, T>;
+    constexpr int E = F::E;
+    const int d = a.d, piece = a.piece, lanes = blockDim.x, wide = lanes * E, groups = (d + wide - 1) / wide;
+    const int64_t at0 = blockIdx.x - before, p = at0 / groups * blockDim.y + threadIdx.y, lo = p * piece;
+    const int n = lo < a.N ? (int)min((int64_t)piece, a.N - lo) : 0;
+    uint32_t* key = sh + threadIdx.y * (2 * piece + 2) + 1;
+    int32_t* item = reinterpret_cast<int32_t*>(key + piece + 1);
+    for (int i = threadIdx.x; i < n + 2 && n > 0; i += blockDim.x) {
+        const int64_t at = lo + i - 1;
+        key[i - 1] = at >= 0 && at < a.N ? a.keys[at] : 0xffffffffu;   // (no key of a token)
+        if (i > 0 && i <= n) item[i - 1] = a.items[at];
+    }
+    __syncthreads();
+    const int c = (int)(at0 % groups) * wide + frag_first<W>(threadIdx.x);
+    if (c >= d) return;
+    const T* dx = static_cast<const T*>(a.dx);
+    float acc[E] = {};
+    bool from_left = n > 0 && key[-1] == key[0];
+    for (int i0 = 0; i0 < n; i0 += AHEAD) {
+        F r[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (i0 + u < n && key[i0 + u] < a.vocab) r[u].load(dx + (int64_t)item[i0 + u] * d, c, lanes, d);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int i = i0 + u;
+            if (i >= n || key[i] >= a.vocab) return;   // the end of the piece, or padding from here on
+            float v[E];
+            r[u].get(v);
+#pragma unroll
+            for (int j = 0; j < E; ++j) acc[j] += v[j];
+            const bool goes_on = key[i + 1] == key[i];
+            if (goes_on && i + 1 < n) continue;
+            if (from_left || goes_on) frag<W, float>::put(a.part + (2 * p + (from_left ? 0 : 1)) * d, c, lanes, d, acc);
+            else add_row<W>(a.d_table + (int64_t)key[i] * d, c, lanes, d, acc, a.scale, a.accumulate);
+#pragma unroll
+            for (int j = 0; j < E; ++j) acc[j] = 0.0f;
+            from_left = false;
+        }
+    }
+}
+
+// A block owns a piece; it has work where a run begins in the piece and goes on past it. Its lanes beside each other (threadIdx.y) take the
+// run's pieces in turn, eight of them in flight.
+template <int W>
+__global__ void __launch_bounds__(256) embed_join_kernel(const Sum a) {
+    using F = frag<W, float>;
+    constexpr int E = F::E;
+    extern __shared__ uint32_t sh_raw[];
+    float(*sh)[E] = reinterpret_cast<float(*)[E]>(sh_raw);   // [lane beside][column lane]
+    const int64_t p = blockIdx.x;
+    const int piece = a.piece, d = a.d, lanes = blockDim.x, beside = blockDim.y, threads = lanes * beside, me = threadIdx.y * lanes + threadIdx.x;
+    pdl_wait();
     const int64_t end = (p + 1) * piece;
-    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
-    if (end >= N || c >= d) return;
-    const uint32_t key = keys[end - 1];
-    if (key >= vocab || keys[end] != key) return;
-    if (p > 0 && keys[p * piece - 1] == key) return;   // (it began further left)
-    float acc[V];
-    ld_row<V>(part + (2 * p + 1) * d + c, acc);
-    for (int64_t q = p + 1; q * piece < N && keys[q * piece] == key; ++q) {
-        float v[V];
-        ld_row<V>(part + 2 * q * d + c, v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] += v[j];
+    const uint32_t key = a.keys[end - 1], next = a.keys[end], left = p > 0 ? a.keys[p * piece - 1] : 0xffffffffu;   // (the last piece has no block)
+    if (key >= a.vocab || next != key || left == key) return;   // (the last: it began further left)
+    int64_t more = 0;   // pieces that the run comes into from the left
+    for (;; more += threads) {
+        const int64_t q = p + 1 + more + me;
+        const int in = __syncthreads_count(q * piece < a.N && a.keys[q * piece] == key);
+        if (in < threads) {
+            more += in;
+            break;
+        }
     }
-    add_row<V>(d_table + (int64_t)key * d + c, acc, scale, accumulate);
+    for (int c = frag_first<W>(threadIdx.x); c - frag_first<W>(threadIdx.x) < d; c += lanes * E) {   // (the same turns for all)
+        float acc[E] = {};
+        auto add = [&](const F& r) {
+            float v[E];
+            r.get(v);
+#pragma unroll
+            for (int j = 0; j < E; ++j) acc[j] += v[j];
+        };
+        if (c < d) {
+            F r[AHEAD];
+            if (threadIdx.y == 0) {
+                r[0].load(a.part + (2 * p + 1) * d, c, lanes, d);
+                add(r[0]);
+            }
+            for (int64_t q0 = threadIdx.y; q0 < more; q0 += (int64_t)AHEAD * beside) {
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u)
+                    if (q0 + u * beside < more) r[u].load(a.part + 2 * (p + 1 + q0 + u * beside) * d, c, lanes, d);
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u)
+                    if (q0 + u * beside < more) add(r[u]);
+            }
+        }
+        if (beside > 1) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) sh[me][j] = acc[j];
+            __syncthreads();
+            if (threadIdx.y == 0) {
+                for (int i = 1; i < beside; ++i) {
+#pragma unroll
+                    for (int j = 0; j < E; ++j) acc[j] += sh[i * lanes + threadIdx.x][j];
+                }
+            }
+            __syncthreads();
+        }
+        if (threadIdx.y == 0 && c < d) add_row<W>(a.d_table + (int64_t)key * d, c, lanes, d, acc, a.scale, a.accumulate);
+    }
 }
 
-constexpr int PIECE = 64;
+// Few tokens: everything in one launch. Every CTA sorts all of them in its own shared memory (the same few microseconds at the same time)
+// and then owns some rows of the table and some columns. A row of up to SHORT tokens is summed by the lanes that share a row, others of
+// the CTA doing other rows meanwhile; a longer one by the whole CTA, each of the lanes beside each other taking tokens in turn.
+constexpr int SHORT = 16;
+template <int W, typename T>
+__global__ void __launch_bounds__(1024) embed_small_kernel(const Sum a, const stable_sort::Job j, int lanes, int rows) {
+    using F = frag<W, T>;
+    constexpr int E = F::E;
+    extern __shared__ uint32_t sh[];   // keys and tokens, twice; places; counters. Behind the sort: the sums of the lanes beside each other
+    __shared__ int32_t wsum[32];
+    __shared__ int32_t long_rows[stable_sort::SMALL / SHORT], n_long;
+    const int n = (int)j.n, per = (n + 1023) / 1024, room = (n + 7) & ~7;
+    uint32_t* keys[2] = {sh, sh + room};
+    int32_t* items[2] = {reinterpret_cast<int32_t*>(sh) + 2 * room, reinterpret_cast<int32_t*>(sh) + 3 * room};
+    int32_t* first = reinterpret_cast<int32_t*>(sh) + 4 * room;
+    uint16_t *counts = reinterpret_cast<uint16_t*>(first + j.bins), *run = counts + (threadIdx.x >> 5) * j.bins;
+    const uint32_t mask = stable_sort::mask_of(j);
+    if (threadIdx.x == 0) n_long = 0;
+    int now = 0;
+    for (int pass = 0; pass < j.passes; ++pass) {
+        stable_sort::Items t;
+        const int lo = (threadIdx.x >> 5) * per * 32 + (threadIdx.x & 31);
+#pragma unroll
+        for (int i = 0; i < stable_sort::PER; ++i) {
+            const int at = lo + i * 32;
+            t.item[i] = -1;
+            if (i < per && at < n) {
+                t.key[i] = pass == 0 ? min(j.ids[at], j.limit) : keys[now][at];
+                t.item[i] = pass == 0 ? at : items[now][at];
+            }
+        }
+        const int shift = pass * j.digit;
+        stable_sort::rank_cta(j.bins, shift, mask, counts, first, wsum, t);
+        now ^= pass > 0;
+#pragma unroll
+        for (int i = 0; i < stable_sort::PER; ++i) {
+            if (t.item[i] < 0) continue;
+            const int b = (int)((t.key[i] >> shift) & mask), at = first[b] + run[b] + t.rank[i];
+            keys[now][at] = t.key[i];
+            items[now][at] = t.item[i];
+        }
+        __syncthreads();
+    }
+    const uint32_t* key = keys[now];
+    const int32_t* item = items[now];
+    const int d = a.d, beside = 1024 / lanes, x = threadIdx.x % lanes, y = threadIdx.x / lanes;
+    const T* dx = static_cast<const T*>(a.dx);
+    const int wide = lanes * E, c = blockIdx.y * wide + frag_first<W>(x);
+    const bool in = c < d;
+    const int64_t v0 = (int64_t)blockIdx.x * rows;
+    auto sum = [&](int lo, int step, int end, float (&acc)[E]) {
+        for (int i0 = lo; i0 < end; i0 += AHEAD * step) {
+            F r[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+                if (i0 + u * step < end) r[u].load(dx + (int64_t)item[i0 + u * step] * d, c, lanes, d);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                if (i0 + u * step >= end) break;
+                float v[E];
+                r[u].get(v);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += v[e];
+            }
+        }
+    };
+    auto bound = [&](uint32_t v) { return (int)lower_bound(key, n, v); };
+    for (int64_t v = v0 + y; v < v0 + rows && v < a.vocab && in; v += beside) {
+        const int lo = bound((uint32_t)v);
+        const bool some = lo < n && key[lo] == v;
+        if (!some && a.accumulate) continue;   // left as it was
+        const int end = some ? bound((uint32_t)v + 1) : lo;
+        if (end - lo > SHORT) {
+            if (x == 0) long_rows[atomicAdd(&n_long, 1)] = (int32_t)v;   // (rows are summed one by one: their order does not matter)
+            continue;
+        }
+        float acc[E] = {};
+        sum(lo, 1, end, acc);
+        add_row<W>(a.d_table + v * d, c, lanes, d, acc, a.scale, a.accumulate);
+    }
+    __syncthreads();
+    float* part = reinterpret_cast<float*>(first);   // [lane beside][column lane][E]: the places and counters are no longer needed
+    for (int l = 0; l < n_long; ++l) {
+        const uint32_t v = (uint32_t)long_rows[l];
+        const int lo = bound(v), end = bound(v + 1);
+        float acc[E] = {};
+        if (in) sum(lo + y, beside, end, acc);
+#pragma unroll
+        for (int e = 0; e < E; ++e) part[threadIdx.x * E + e] = acc[e];
+        __syncthreads();
+        if (y == 0 && in) {
+            for (int i = 1; i < beside; ++i) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += part[(i * lanes + x) * E + e];
+            }
+            add_row<W>(a.d_table + (int64_t)v * d, c, lanes, d, acc, a.scale, a.accumulate);
+        }
+        __syncthreads();
+    }
+}
 
 // Scratch: sorted keys and items, the pass before's where there are two, the counts, and the partial sums.
 struct Plan {
-    int bits, passes, digit;
+    int passes, digit, bins, piece;
+    bool small;   // everything in one launch
     size_t list, counts, part;
     Plan(int64_t N, int64_t d, int64_t vocab) {
-        bits = 1;
+        int bits = 1;
         while (((int64_t)1 << bits) <= vocab) ++bits;   // keys 0 .. vocab
         passes = (int)ceil_div64(bits, 11);
         digit = (int)ceil_div64(bits, passes);
+        bins = passes == 1 ? (int)vocab + 1 : 1 << digit;
+        // short pieces where the tokens are few: the walk down a piece is what such a call waits for
+        piece = MOST_PIECE;
+        while (piece > AHEAD && N * d < (int64_t)piece * 148 * 4096) piece /= 2;
+        // (a CTA of the one launch may have to add all of dx's rows by itself)
+        small = N <= stable_sort::SMALL && N * d <= (1 << 20);
+        if (small) {
+            list = counts = part = 0;
+            return;
+        }
         list = ((size_t)N * 4 + 255) & ~(size_t)255;
-        counts = stable_sort::counts_bytes(N, 1 << digit);
-        part = (size_t)ceil_div64(N, PIECE) * 2 * d * 4;
+        counts = stable_sort::scratch_bytes(N, bins);
+        part = (size_t)ceil_div64(N, piece) * 2 * d * 4;
     }
     size_t bytes() const { return 4 * list + counts + part + 256; }
 };
@@ -131,17 +364,17 @@ int asca_embed_scaled_fwd(asca_ctx* ctx, const void* table, const uint32_t* ids,
     ASCA_REQUIRE(ctx, table && ids && x, "embed_scaled_fwd: null pointer");
     ASCA_REQUIRE(ctx, N < ((int64_t)1 << 31), "embed_scaled_fwd: at most 2^31 - 1 tokens");
     asca_device_scope on(ctx);
-    const bool four = asca_rows_by_four(table, d, table_dtype) && asca_rows_by_four(x, d, out_dtype);
-    const int64_t per_row = four ? d / 4 : d;
-    const int tx = per_row >= 256 ? 256 : (int)ceil_div64(per_row, 32) * 32, ty = 256 / tx;
-    const dim3 grid((unsigned)ceil_div64(N, ty)), block(tx, ty);
-    auto go = [&](auto tab, auto out) {
-        using TT = std::remove_const_t<std::remove_pointer_t<decltype(tab)>>;
-        using TX = std::remove_const_t<std::remove_pointer_t<decltype(out)>>;
-        if (four) embed_scaled_fwd_kernel<4, TT, TX><<<grid, block, 0, ctx->stream>>>(tab, ids, N, (int)d, (uint32_t)vocab, scale, out);
-        else embed_scaled_fwd_kernel<1, TT, TX><<<grid, block, 0, ctx->stream>>>(tab, ids, N, (int)d, (uint32_t)vocab, scale, out);
-    };
-    asca_with_dtype(table, table_dtype, [&](auto tab) { asca_with_dtype(x, out_dtype, [&](auto out) { go(tab, out); }); });
+    const int v = asca_row_width(d, table, table_dtype, x, out_dtype);
+    const dim3 block = asca_row_block(asca_row_frags(d, v), 256), grid((unsigned)ceil_div64(N, (int64_t)block.y * TOKENS));
+    asca_with_dtype(table, table_dtype, [&](auto tab) {
+        asca_with_dtype(x, out_dtype, [&](auto out) {
+            using TT = std::remove_const_t<std::remove_pointer_t<decltype(tab)>>;
+            using TX = std::remove_pointer_t<decltype(out)>;
+            asca_with_width<TT, TX>(v, [&](auto w) {
+                embed_scaled_fwd_kernel<w(), TT, TX><<<grid, block, 0, ctx->stream>>>(tab, ids, N, (int)d, (uint32_t)vocab, scale, out);
+            });
+        });
+    });
     ASCA_CHECK_LAUNCH(ctx);
     return ASCA_OK;
 }
@@ -159,48 +392,71 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
     ASCA_REQUIRE(ctx, N < ((int64_t)1 << 31), "embed_scaled_bwd: at most 2^31 - 1 tokens");
     ASCA_REQUIRE(ctx, d_table, "embed_scaled_bwd: null pointer");
     asca_device_scope on(ctx);
-    if (!accumulate) ASCA_CUDA(ctx, cudaMemsetAsync(d_table, 0, (size_t)vocab * d * 4, ctx->stream));
-    if (N == 0) return ASCA_OK;
+    if (N == 0) {
+        if (!accumulate) ASCA_CUDA(ctx, cudaMemsetAsync(d_table, 0, (size_t)vocab * d * 4, ctx->stream));
+        return ASCA_OK;
+    }
     ASCA_REQUIRE(ctx, dx && ids && ws, "embed_scaled_bwd: null pointer");
     const Plan plan(N, d, vocab);
     ASCA_REQUIRE(ctx, asca_aligned(ws, 256) && ws_bytes >= plan.bytes(), "embed_scaled_bwd: the workspace has to have asca_embed_scaled_bwd_ws bytes, 256-byte aligned");
+    const int v = asca_row_width(d, dx, dtype, d_table, ASCA_F32);
+    const int64_t frags = asca_row_frags(d, v);
+    dim3 block = asca_row_block(frags, 128);
+    const unsigned place = (2 * plan.piece + 2) * 4;   // a piece's keys and items in shared memory
+    block.y = std::min(block.y, 4096u / plan.piece);   // 36 KiB at most
+    const int64_t pieces = ceil_div64(N, plan.piece), groups = ceil_div64(frags, block.x);
     char* w = (char*)ws;
-    uint32_t* keys[2] = {(uint32_t*)w, (uint32_t*)(w + plan.list)};
-    int32_t* items[2] = {(int32_t*)(w + 2 * plan.list), (int32_t*)(w + 3 * plan.list)};
-    int32_t* counts = (int32_t*)(w + 4 * plan.list);
-    float* part = (float*)(w + 4 * plan.list + plan.counts);
-    int at = 0;
-    for (int i = 0; i < plan.passes; ++i) {
-        stable_sort::Pass p;
-        p.n = N;
-        p.limit = (uint32_t)vocab;
-        if (i == 0) p.ids = ids;
-        else p.keys = keys[at], p.items = items[at];
-        p.shift = i * plan.digit;
-        p.bins = 1 << plan.digit;
-        p.mask = (uint32_t)p.bins - 1;
-        at = i == 0 ? 0 : 1 - at;
-        p.out_keys = keys[at];
-        p.out_items = items[at];
-        ASCA_TRY(stable_sort::run(ctx, p, counts, nullptr, 0));
+    stable_sort::Job j{};
+    j.ids = ids;
+    j.limit = (uint32_t)vocab;
+    j.n = N;
+    j.passes = plan.passes;
+    j.digit = plan.digit;
+    j.bins = plan.bins;
+    for (int i = 0; i < 2; ++i) j.keys[i] = (uint32_t*)(w + i * plan.list), j.items[i] = (int32_t*)(w + (2 + i) * plan.list);
+    Sum a{};
+    a.dx = dx; a.N = N; a.d = (int)d; a.piece = plan.piece; a.accumulate = accumulate; a.vocab = (uint32_t)vocab; a.scale = scale; a.d_table = d_table;
+    a.keys = j.keys[(plan.passes - 1) & 1];
+    a.items = j.items[(plan.passes - 1) & 1];
+    a.part = (float*)(w + 4 * plan.list + plan.counts);
+    a.sums = ceil_div64(pieces, block.y) * groups;
+    a.zeros = accumulate ? 0 : ceil_div64(vocab, ZERO_ROWS);
+    if (plan.small) {
+        int lanes = 1;
+        while (lanes < frags && lanes < 256) lanes *= 2;
+        const int64_t across = ceil_div64(frags, lanes), rows = ceil_div64(vocab, std::max<int64_t>(1, ctx->sm_count / across));   // one CTA an SM
+        const dim3 grid((unsigned)ceil_div64(vocab, rows), (unsigned)across);
+        const size_t sums = 1024 * 4 * (size_t)(v == 1 ? 4 : v), sorts = (size_t)j.bins * 4 + 32 * (size_t)j.bins * 2;
+        const size_t smem = 4 * (((size_t)N + 7) & ~(size_t)7) * 4 + std::max(sums, sorts);
+        cudaError_t e = cudaSuccess;
+        asca_with_dtype(dx, dtype, [&](auto src) {
+            using T = std::remove_const_t<std::remove_pointer_t<decltype(src)>>;
+            asca_with_width<T, T>(v, [&](auto wd) {
+                auto kern = embed_small_kernel<wd(), T>;
+                if (smem > 32 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+                if (e == cudaSuccess) kern<<<grid, 1024, smem, ctx->stream>>>(a, j, lanes, (int)rows);
+            });
+        });
+        ASCA_CUDA(ctx, e);
+        ASCA_CHECK_LAUNCH(ctx);
+        return ASCA_OK;
     }
-    const bool four = asca_rows_by_four(dx, d, dtype) && asca_aligned(d_table, 16);
-    const int64_t per_row = four ? d / 4 : d;
-    const int tx = per_row >= 128 ? 128 : (int)ceil_div64(per_row, 32) * 32, ty = 128 / tx;
-    const int64_t pieces = ceil_div64(N, PIECE);
-    const dim3 block(tx, ty), grid((unsigned)ceil_div64(pieces, ty), (unsigned)ceil_div64(per_row, tx));
-    ASCA_REQUIRE(ctx, grid.y <= 65535, "embed_scaled_bwd: rows too wide");
+    ASCA_REQUIRE(ctx, a.sums + a.zeros < ((int64_t)1 << 31) && ceil_div64(frags, 32) <= 65535, "embed_scaled_bwd: too large");
+    ASCA_TRY(stable_sort::sort(ctx, j, (int32_t*)(w + 4 * plan.list)));
+    cudaError_t e = cudaSuccess;
     asca_with_dtype(dx, dtype, [&](auto src) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(src)>>;
-        if (four) embed_pieces_kernel<4, T><<<grid, block, 0, ctx->stream>>>(src, keys[at], items[at], N, (int)d, (uint32_t)vocab, scale, accumulate, PIECE, d_table, part);
-        else embed_pieces_kernel<1, T><<<grid, block, 0, ctx->stream>>>(src, keys[at], items[at], N, (int)d, (uint32_t)vocab, scale, accumulate, PIECE, d_table, part);
+        asca_with_width<T, T>(v, [&](auto wd) {
+            // (whole warps: a zeroing block votes)
+            e = asca_launch_after(ctx, embed_pieces_kernel<wd(), T>, dim3((unsigned)(a.sums + a.zeros)), block, (size_t)block.y * place, a);
+            const dim3 wide = asca_row_block(frags, 256);
+            if (e == cudaSuccess && pieces > 1)
+                e = asca_launch_after(ctx, embed_join_kernel<wd()>, dim3((unsigned)(pieces - 1)), wide,
+                                      wide.y > 1 ? (size_t)wide.x * wide.y * 4 * frag<wd(), float>::E : 0, a);
+        });
     });
-    ASCA_CHECK_LAUNCH(ctx);
-    if (pieces > 1) {
-        if (four) embed_join_kernel<4><<<grid, block, 0, ctx->stream>>>(keys[at], N, (int)d, (uint32_t)vocab, scale, accumulate, PIECE, part, d_table);
-        else embed_join_kernel<1><<<grid, block, 0, ctx->stream>>>(keys[at], N, (int)d, (uint32_t)vocab, scale, accumulate, PIECE, part, d_table);
-        ASCA_CHECK_LAUNCH(ctx);
-    }
+    ASCA_CUDA(ctx, e);
+    ctx->launches += pieces > 1 ? 2 : 1;
     return ASCA_OK;
 }
 

@@ -2,10 +2,11 @@
 //
 //   norm = sqrt(sum over all elements of all tensors of g^2)          c = min(1, max_norm / (norm + 1e-6))
 //
-// The tensors are cut into pieces of 16,384 elements; a CTA takes every gridDim-th piece and adds the squares in 64 bits, in which
-// neither the square of a large f32 overflows nor that of a small one vanishes, and a long sum loses nothing. A second launch adds
-// the CTAs' sums in a fixed order. Bound by reading the gradients. The tensors' addresses travel with the launch (no copy in
-// front of it, and a captured graph keeps them), 160 a launch.
+// A CTA owns an equal, contiguous share of all tensors laid end to end, eight 16-byte loads in flight a thread, and adds the squares in
+// 64 bits, in which neither the square of a large f32 overflows nor that of a small one vanishes, and a long sum loses nothing. A
+// second launch adds the CTAs' sums in a fixed order; up to 2 MiB of gradients one cluster does both in one launch through
+// distributed shared memory. Bound by reading the gradients. The tensors' addresses travel with the launch (no copy in front of
+// it, and a captured graph keeps them), 128 a launch.
 //
 // A norm that is not finite follows the formula: c is 0 for an infinite norm (an infinite gradient then gives NaN), NaN for NaN.
 #include "row_io.cuh"
@@ -15,50 +16,49 @@
 
 namespace {
 
-constexpr int MAX_TENSORS = 160, PIECE = 16384;
+constexpr int MAX_TENSORS = 128, CLUSTER = 8, CTAS_PER_SM = 32, LOADS = 8, GRAIN = 256;
+constexpr int64_t CLUSTER_BYTES = 2 << 20, SHARE = 128 << 10;   // bytes of a CTA at least
 struct Tensors {
     void* p[MAX_TENSORS];
     int64_t n[MAX_TENSORS];
-    int32_t first[MAX_TENSORS + 1];   // the first piece of each tensor
+    int64_t off[MAX_TENSORS + 1];   // bytes in front of each tensor, all rounded up to GRAIN
     uint8_t bf16[MAX_TENSORS];
     int count;
 };
 
-// f(pointer to the tensor's type, first element, past the last) for every piece of this CTA
+// f(pointer to the tensor's type, elements) for every tensor's part in this CTA's share
 template <typename F>
-__device__ __forceinline__ void each_piece(const Tensors& t, F f) {
-    const int total = t.first[t.count];
-    for (int i = blockIdx.x; i < total; i += gridDim.x) {
-        int lo = 0, hi = t.count - 1;   // last tensor whose first piece is at most i
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (t.first[mid] <= i) lo = mid; else hi = mid - 1;
-        }
-        const int64_t a = (int64_t)(i - t.first[lo]) * PIECE, b = min(a + PIECE, t.n[lo]);
-        if (t.bf16[lo]) f(static_cast<__nv_bfloat16*>(t.p[lo]) + a, (int)(b - a));
-        else f(static_cast<float*>(t.p[lo]) + a, (int)(b - a));
+__device__ __forceinline__ void each_part(const Tensors& t, F f) {
+    const int64_t grains = t.off[t.count] / GRAIN, start = grains * blockIdx.x / gridDim.x * GRAIN, end = grains * (blockIdx.x + 1) / gridDim.x * GRAIN;
+    int lo = 0, hi = t.count - 1;   // last tensor that begins at or in front of the share
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.off[mid] <= start) lo = mid; else hi = mid - 1;
+    }
+    for (; lo < t.count && t.off[lo] < end; ++lo) {
+        const int size = t.bf16[lo] ? 2 : 4;
+        const int64_t a = (start > t.off[lo] ? start - t.off[lo] : 0) / size, b = min((end - t.off[lo]) / size, t.n[lo]);
+        if (a >= b) continue;   // (in the padding behind a tensor)
+        if (t.bf16[lo]) f(static_cast<__nv_bfloat16*>(t.p[lo]) + a, b - a);
+        else f(static_cast<float*>(t.p[lo]) + a, b - a);
     }
 }
 
-// A piece of a tensor that may begin anywhere: single elements up to the 16-byte grid, then groups of G (16 bytes), then the rest.
+// A part of a tensor that may begin anywhere: single elements up to the 16-byte grid, then groups of G (16 bytes), then the rest.
 template <typename T>
-__device__ __forceinline__ int lead(const T* p, int n) {
+__device__ __forceinline__ int lead(const T* p, int64_t n) {
     const int off = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
-    return min(n, off ? (int)(16 / sizeof(T)) - off : 0);
+    return (int)min(n, (int64_t)(off ? (int)(16 / sizeof(T)) - off : 0));
 }
 __device__ __forceinline__ void square_add(double& s, float v) { s = fma((double)v, (double)v, s); }
-__device__ __forceinline__ void group_add(double& s, const float* p) {
-    const float4 v = __ldg(reinterpret_cast<const float4*>(p));
-    square_add(s, v.x); square_add(s, v.y); square_add(s, v.z); square_add(s, v.w);
+__device__ __forceinline__ void group_add(double (&s)[4], const raw_row<4, float>& r) {
+    square_add(s[0], r.v.x); square_add(s[1], r.v.y); square_add(s[2], r.v.z); square_add(s[3], r.v.w);
 }
-__device__ __forceinline__ void group_add(double& s, const __nv_bfloat16* p) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void group_add(double (&s)[4], const raw_row<8, __nv_bfloat16>& r) {
+    float v[8];
+    unpack(r, v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 v = bf16x2_f32(w[i]);
-        square_add(s, v.x); square_add(s, v.y);
-    }
+    for (int i = 0; i < 8; ++i) square_add(s[i & 3], v[i]);
 }
 
 __device__ double block_sum_f64(double v, double* red) {
@@ -73,22 +73,60 @@ __device__ double block_sum_f64(double v, double* red) {
     return v;
 }
 
+// The CTA's sum, in every thread.
+__device__ __forceinline__ double squares(const Tensors& t, double* red) {
+    double s[4] = {};
+    each_part(t, [&](auto* p, int64_t n) {
+        using T = std::remove_pointer_t<decltype(p)>;
+        constexpr int G = 16 / sizeof(T);
+        const int head = lead(p, n), threads = blockDim.x;
+        const int64_t groups = (n - head) / G;
+        int64_t i = threadIdx.x;
+        for (; i + (LOADS - 1) * threads < groups; i += LOADS * threads) {
+            raw_row<G, T> r[LOADS];
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) r[u] = ld_raw<G>(p + head + (i + u * threads) * G);
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) group_add(s, r[u]);
+        }
+        for (; i < groups; i += threads) group_add(s, ld_raw<G>(p + head + i * G));
+        const int rest = (int)(n - groups * G);   // in front of the groups and behind them
+        for (i = threadIdx.x; i < rest; i += threads) square_add(s[0], to_f32(p[i < head ? i : i + groups * G]));
+    });
+    return block_sum_f64((s[0] + s[1]) + (s[2] + s[3]), red);
+}
+
 __global__ void __launch_bounds__(256) norm_parts_kernel(const __grid_constant__ Tensors t, double* __restrict__ part) {
     __shared__ double red[32];
-    double s = 0.0;
-    each_piece(t, [&](auto* p, int n) {
-        constexpr int G = 16 / sizeof(*p);
-        const int head = lead(p, n), groups = (n - head) / G;
-        for (int i = threadIdx.x; i < groups; i += 256) group_add(s, p + head + i * G);
-        const int rest = n - groups * G;   // in front of the groups and behind them
-        for (int i = threadIdx.x; i < rest; i += 256) square_add(s, to_f32(p[i < head ? i : i + groups * G]));
-    });
-    s = block_sum_f64(s, red);
+    pdl_launch_dependents();
+    const double s = squares(t, red);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+// All of it in one cluster.
+__global__ void __launch_bounds__(1024) norm_cluster_kernel(const __grid_constant__ Tensors t, float* __restrict__ norm) {
+    __shared__ double red[32];
+    __shared__ double mine;
+    const double s = squares(t, red);
+    if (threadIdx.x == 0) mine = s;
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        double sum = 0.0;
+        for (uint32_t c = 0; c < CLUSTER; ++c) {
+            uint32_t at;
+            double x;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&mine)), "r"(c));
+            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(x) : "r"(at) : "memory");
+            sum += x;
+        }
+        *norm = (float)sqrt(sum);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // nobody leaves before its sum is read
 }
 
 __global__ void __launch_bounds__(256) norm_join_kernel(const double* __restrict__ part, int n, float* __restrict__ norm) {
     __shared__ double red[32];
+    pdl_wait();
     double s = 0.0;
     for (int i = threadIdx.x; i < n; i += 256) s += part[i];
     s = block_sum_f64(s, red);
@@ -98,18 +136,30 @@ __global__ void __launch_bounds__(256) norm_join_kernel(const double* __restrict
 __global__ void __launch_bounds__(256) clip_kernel(const __grid_constant__ Tensors t, const float* __restrict__ norm, float max_norm) {
     const float c = asca_clip_coefficient(*norm, max_norm);
     if (c == 1.0f) return;   // nothing changes
-    each_piece(t, [&](auto* p, int n) {
+    each_part(t, [&](auto* p, int64_t n) {
         using T = std::remove_pointer_t<decltype(p)>;
-        const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T))), groups = (n - head) / 4;
-        for (int i = threadIdx.x; i < groups; i += 256) {
-            T* q = p + head + i * 4;
-            float4 v = ld4(q);
-            v.x *= c; v.y *= c; v.z *= c; v.w *= c;
-            st4(q, v);
+        constexpr int G = 16 / sizeof(T);
+        const int head = lead(p, n);
+        const int64_t groups = (n - head) / G;
+        auto scale = [&](T* q, const raw_row<G, T>& r) {
+            float v[G];
+            unpack(r, v);
+#pragma unroll
+            for (int e = 0; e < G; ++e) v[e] *= c;
+            st_row<G>(q, v);
+        };
+        int64_t i = threadIdx.x;
+        for (; i + 3 * 256 < groups; i += 4 * 256) {
+            raw_row<G, T> r[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) r[u] = ld_raw<G>(p + head + (i + u * 256) * G);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) scale(p + head + (i + u * 256) * G, r[u]);
         }
-        const int rest = n - groups * 4;
-        for (int i = threadIdx.x; i < rest; i += 256) {
-            T* q = p + (i < head ? i : i + groups * 4);
+        for (; i < groups; i += 256) scale(p + head + i * G, ld_raw<G>(p + head + i * G));
+        const int rest = (int)(n - groups * G);
+        for (i = threadIdx.x; i < rest; i += 256) {
+            T* q = p + (i < head ? i : i + groups * G);
             *q = from_f32<T>(c * to_f32<T>(*q));
         }
     });
@@ -118,7 +168,7 @@ __global__ void __launch_bounds__(256) clip_kernel(const __grid_constant__ Tenso
 int check_tensors(asca_ctx* ctx, const char* who, void* const* p, const int64_t* n, const int* dtype, int count) {
     ASCA_REQUIRE(ctx, count >= 0 && (count == 0 || (p && n && dtype)), "%s: bad arguments", who);
     for (int i = 0; i < count; ++i) {
-        ASCA_REQUIRE(ctx, n[i] >= 0 && n[i] < ((int64_t)1 << 37) && (n[i] == 0 || p[i]), "%s: tensor %d: bad pointer or size", who, i);
+        ASCA_REQUIRE(ctx, n[i] >= 0 && n[i] < ((int64_t)1 << 35) && (n[i] == 0 || p[i]), "%s: tensor %d: bad pointer or size", who, i);
         ASCA_REQUIRE(ctx, asca_known_dtype(dtype[i]), "%s: tensor %d: unknown dtype", who, i);
         ASCA_REQUIRE(ctx, asca_aligned(p[i], asca_dtype_size(dtype[i])), "%s: tensor %d is not aligned to its elements", who, i);
     }
@@ -129,22 +179,19 @@ int check_tensors(asca_ctx* ctx, const char* who, void* const* p, const int64_t*
 Tensors take(void* const* p, const int64_t* n, const int* dtype, int count, int& at) {
     Tensors t;
     int k = 0;
-    int64_t pieces = 0;
+    t.off[0] = 0;
     for (; at < count && k < MAX_TENSORS; ++at) {
         if (n[at] == 0) continue;
         t.p[k] = p[at];
         t.n[k] = n[at];
         t.bf16[k] = dtype[at] == ASCA_BF16;
-        t.first[k] = (int32_t)pieces;
-        pieces += ceil_div64(n[at], PIECE);
+        t.off[k + 1] = t.off[k] + ceil_div64(n[at] * (int64_t)asca_dtype_size(dtype[at]), GRAIN) * GRAIN;
         ++k;
     }
-    t.first[k] = (int32_t)pieces;
     t.count = k;
     return t;
 }
-
-constexpr int CTAS_PER_SM = 8;
+int ctas_of(const asca_ctx* ctx, const Tensors& t) { return (int)std::min<int64_t>(ceil_div64(t.off[t.count], SHARE), ctx->sm_count * CTAS_PER_SM); }
 
 }  // namespace
 
@@ -165,14 +212,23 @@ int asca_grad_norm(asca_ctx* ctx, void* const* grads, const int64_t* n, const in
     int parts = 0;
     for (int at = 0; at < count; ) {
         const Tensors t = take(grads, n, dtype, count, at);
-        const int grid = std::min(t.first[t.count], ctx->sm_count * CTAS_PER_SM);
+        const int grid = ctas_of(ctx, t);
+        if (parts == 0 && at == count && t.off[t.count] <= CLUSTER_BYTES) {
+            ASCA_CUDA(ctx, asca_launch_cluster(ctx, norm_cluster_kernel, dim3(CLUSTER), dim3(1024), 0, CLUSTER, t, norm));
+            ctx->launches++;
+            return ASCA_OK;
+        }
         if (grid == 0) continue;
         norm_parts_kernel<<<(unsigned)grid, 256, 0, ctx->stream>>>(t, part + parts);
         ASCA_CHECK_LAUNCH(ctx);
         parts += grid;
     }
-    norm_join_kernel<<<1, 256, 0, ctx->stream>>>(part, parts, norm);
-    ASCA_CHECK_LAUNCH(ctx);
+    if (parts == 0) {   // (no tensors)
+        ASCA_CUDA(ctx, cudaMemsetAsync(norm, 0, sizeof(float), ctx->stream));
+        return ASCA_OK;
+    }
+    ASCA_CUDA(ctx, asca_launch_after(ctx, norm_join_kernel, dim3(1), dim3(256), 0, (const double*)part, parts, norm));
+    ctx->launches++;
     return ASCA_OK;
 }
 
@@ -189,7 +245,7 @@ int asca_clip_grads(asca_ctx* ctx, void* const* grads, const int64_t* n, const i
     asca_device_scope on(ctx);
     for (int at = 0; at < count; ) {
         const Tensors t = take(grads, n, dtype, count, at);
-        const int grid = std::min(t.first[t.count], ctx->sm_count * CTAS_PER_SM);
+        const int grid = ctas_of(ctx, t);
         if (grid == 0) continue;
         clip_kernel<<<(unsigned)grid, 256, 0, ctx->stream>>>(t, norm, max_norm);
         ASCA_CHECK_LAUNCH(ctx);

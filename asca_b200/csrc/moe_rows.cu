@@ -15,92 +15,160 @@
 
 namespace {
 
-// a thread owns V columns of a token
-template <int V, typename TX, typename TS>
+// sort: a thread has its columns of TOKENS tokens in flight (the rows are asked for before the first is used); a block has as many lanes
+// a token as a row has groups of columns, 256 at most.
+constexpr int TOKENS = 4;
+
+template <int W, typename TX, typename TS>
 __global__ void __launch_bounds__(256) sort_rows_kernel(const TX* __restrict__ x, const int32_t* __restrict__ slot, int64_t N, int K, int d,
                                                         TS* __restrict__ xs) {
-    const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    if (t >= N) return;
-    for (int c = threadIdx.x * V; c < d; c += blockDim.x * V) {
-        float v[V];
-        ld_row<V>(x + t * d + c, v);
-        for (int k = 0; k < K; ++k) {
-            const int32_t s = slot[t * K + k];
-            if (s >= 0) st_row<V>(xs + (int64_t)s * d + c, v);
+    using F = frag<W, TX>;
+    const int lanes = blockDim.x;
+    const int64_t t0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * TOKENS;
+    for (int c = frag_first<W>(threadIdx.x); c < d; c += lanes * F::E) {
+        F r[TOKENS];
+#pragma unroll
+        for (int i = 0; i < TOKENS; ++i)
+            if (t0 + i < N) r[i].load(x + (t0 + i) * d, c, lanes, d);
+#pragma unroll
+        for (int i = 0; i < TOKENS; ++i) {
+            if (t0 + i >= N) break;
+            for (int k = 0; k < K; ++k) {
+                const int32_t s = slot[(t0 + i) * K + k];
+                if (s < 0) continue;
+                TS* p = xs + (int64_t)s * d;
+                if constexpr (std::is_same_v<TX, TS>) r[i].store(p, c, lanes, d);   // bit for bit
+                else {
+                    float v[F::E];
+                    r[i].get(v);
+                    frag<W, TS>::put(p, c, lanes, d, v);
+                }
+            }
         }
     }
 }
+
+// unsort and its gradient: LANES lanes own PAIRS / KS tokens, KS assignments of each at a time: PAIRS rows of the sorted side in flight.
+constexpr int PAIRS = 4;
 
 // weights null: every weight is one
-template <int V, typename TS, typename TX>
+template <int W, int LANES, int KS, typename TS, typename TX>
 __global__ void __launch_bounds__(256) unsort_rows_kernel(const TS* __restrict__ ys, const int32_t* __restrict__ slot, const float* __restrict__ weights,
                                                           int64_t N, int K, int d, TX* __restrict__ out) {
-    const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    if (t >= N) return;
-    for (int c = threadIdx.x * V; c < d; c += blockDim.x * V) {
-        float acc[V] = {};
-        for (int k = 0; k < K; ++k) {
-            const int32_t s = slot[t * K + k];
-            if (s < 0) continue;
-            const float w = weights ? weights[t * K + k] : 1.0f;
-            float v[V];
-            ld_row<V>(ys + (int64_t)s * d + c, v);
+    using F = frag<W, TS>;
+    constexpr int T = PAIRS / KS;
+    const int64_t t0 = ((int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES) * T;
+    for (int c = frag_first<W>(threadIdx.x % LANES); c < d; c += LANES * F::E) {
+        float acc[T][F::E] = {};
+        for (int k0 = 0; k0 < K; k0 += KS) {
+            F r[T][KS];
+            float w[T][KS];
+            int32_t s[T][KS];
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+            for (int i = 0; i < T; ++i) {
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    s[i][j] = t0 + i < N && k0 + j < K ? slot[(t0 + i) * K + k0 + j] : -1;
+                    w[i][j] = s[i][j] >= 0 && weights ? weights[(t0 + i) * K + k0 + j] : 1.0f;
+                    if (s[i][j] >= 0) r[i][j].load(ys + (int64_t)s[i][j] * d, c, LANES, d);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    if (s[i][j] < 0) continue;   // (adds nothing, whatever its weight)
+                    float v[F::E];
+                    r[i][j].get(v);
+#pragma unroll
+                    for (int e = 0; e < F::E; ++e) acc[i][e] = fmaf(w[i][j], v[e], acc[i][e]);
+                }
+            }
         }
-        st_row<V>(out + t * d + c, acc);
+#pragma unroll
+        for (int i = 0; i < T; ++i)
+            if (t0 + i < N) frag<W, TX>::put(out + (t0 + i) * d, c, LANES, d, acc[i]);
     }
 }
 
-// A warp owns a token. d_w (nullable); d_ys may be ys; four assignments at a time share one reading of d_out's row.
-template <int V, typename TX, typename TS>
+// The KS assignments of a token share one reading of d_out's row; d_w (nullable) is a sum over it. d_ys may be ys.
+template <int W, int LANES, int KS, typename TX, typename TS>
 __global__ void __launch_bounds__(256) unsort_rows_bwd_kernel(const TX* __restrict__ d_out, const TS* ys, const int32_t* __restrict__ slot,
                                                               const float* __restrict__ weights, int64_t N, int K, int d, TS* d_ys,
                                                               float* __restrict__ d_w) {
-    const int lane = threadIdx.x & 31;
-    const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (t >= N) return;
-    for (int k0 = 0; k0 < K; k0 += 4) {
-        int32_t s[4];
-        float w[4], dot[4] = {};
+    constexpr int T = PAIRS / KS, E = frag<W, TX>::E;
+    const int lane = threadIdx.x % LANES;
+    const int64_t t0 = ((int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES) * T;
+    for (int k0 = 0; k0 < K; k0 += KS) {
+        int32_t s[T][KS];
+        float w[T][KS], dot[T][KS] = {};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            s[j] = k0 + j < K ? slot[t * K + k0 + j] : -1;
-            w[j] = s[j] >= 0 && weights ? weights[t * K + k0 + j] : 1.0f;
+        for (int i = 0; i < T; ++i) {
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                s[i][j] = t0 + i < N && k0 + j < K ? slot[(t0 + i) * K + k0 + j] : -1;
+                w[i][j] = s[i][j] >= 0 && weights ? weights[(t0 + i) * K + k0 + j] : 1.0f;
+            }
         }
-        for (int c = lane * V; c < d; c += 32 * V) {
-            float g[V];
-            ld_row<V>(d_out + t * d + c, g);
+        for (int c = frag_first<W>(lane); c < d; c += LANES * E) {
+            frag<W, TX> rg[T];
+            frag<W, TS> ry[T][KS];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (s[j] < 0) continue;
-                float y[V], o[V];
-                if (d_w) ld_row<V>(ys + (int64_t)s[j] * d + c, y);
+            for (int i = 0; i < T; ++i) {
+                if (t0 + i < N) rg[i].load(d_out + (t0 + i) * d, c, LANES, d);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    if (d_w) dot[j] = fmaf(g[i], y[i], dot[j]);
-                    o[i] = w[j] * g[i];
+                for (int j = 0; j < KS; ++j)
+                    if (d_w && s[i][j] >= 0) ry[i][j].load(ys + (int64_t)s[i][j] * d, c, LANES, d);
+            }
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                float g[E];
+                if (t0 + i < N) rg[i].get(g);
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    if (s[i][j] < 0) continue;
+                    float y[E], o[E];
+                    if (d_w) ry[i][j].get(y);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        if (d_w && (W > 1 || c + e * LANES < d)) dot[i][j] = fmaf(g[e], y[e], dot[i][j]);
+                        o[e] = w[i][j] * g[e];
+                    }
+                    frag<W, TS>::put(d_ys + (int64_t)s[i][j] * d, c, LANES, d, o);
                 }
-                st_row<V>(d_ys + (int64_t)s[j] * d + c, o);
             }
         }
         if (d_w) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float sum = warp_sum(dot[j]);
-                if (lane == 0 && k0 + j < K) d_w[t * K + k0 + j] = s[j] >= 0 ? sum : 0.0f;
+            for (int i = 0; i < T; ++i) {
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+#pragma unroll
+                    for (int o = LANES / 2; o > 0; o >>= 1) dot[i][j] += __shfl_xor_sync(0xffffffffu, dot[i][j], o);
+                    if (t0 + i < N && lane == 0 && k0 + j < K) d_w[(t0 + i) * K + k0 + j] = s[i][j] >= 0 ? dot[i][j] : 0.0f;
+                }
             }
         }
     }
 }
 
-struct Shape {
-    dim3 grid, block;
+// The lanes that own a token and the assignments they take at a time, as constants; the blocks of N tokens.
+struct Team {
+    int lanes, ks;
+    Team(int64_t frags, int64_t K) : lanes(frags <= 8 ? 8 : frags <= 16 ? 16 : 32), ks(K == 1 ? 1 : K <= 3 ? 2 : 4) {}
+    unsigned blocks(int64_t N) const { return (unsigned)ceil_div64(N, (256 / lanes) * (PAIRS / ks)); }
+    template <typename F>
+    void with(F f) const {
+        auto k = [&](auto l) {
+            if (ks == 1) f(l, std::integral_constant<int, 1>());
+            else if (ks == 2) f(l, std::integral_constant<int, 2>());
+            else f(l, std::integral_constant<int, 4>());
+        };
+        if (lanes == 8) k(std::integral_constant<int, 8>());
+        else if (lanes == 16) k(std::integral_constant<int, 16>());
+        else k(std::integral_constant<int, 32>());
+    }
 };
-inline Shape by_token(int64_t N, int64_t per_row) {
-    const int tx = per_row >= 256 ? 256 : (int)ceil_div64(per_row, 32) * 32, ty = 256 / tx;
-    return {dim3((unsigned)ceil_div64(N, ty)), dim3(tx, ty)};
-}
 
 int check_rows(asca_ctx* ctx, const char* who, int64_t N, int64_t K, int64_t d, int tok_dtype, int row_dtype) {
     ASCA_REQUIRE(ctx, N >= 0 && K > 0 && d > 0 && d < (1 << 30) && K < (1 << 16) && N < ((int64_t)1 << 31) / K, "%s: bad shape (N * K must fit int32)", who);
@@ -114,7 +182,7 @@ extern "C" {
 
 int64_t asca_moe_topk_dispatch_ws(int64_t N, int64_t K, int64_t E) {
     if (N < 0 || K <= 0 || E <= 0 || E + 1 > stable_sort::MAX_BINS) return ASCA_ERR_ARG;
-    return (int64_t)stable_sort::counts_bytes(N * K, (int)E + 1) + 256;
+    return (int64_t)stable_sort::scratch_bytes(N * K, (int)E + 1) + 256;
 }
 
 int asca_moe_topk_dispatch(asca_ctx* ctx, const int32_t* experts, int64_t N, int64_t K, int64_t E, int32_t* perm, int32_t* offsets, int32_t* slot,
@@ -131,14 +199,16 @@ int asca_moe_topk_dispatch(asca_ctx* ctx, const int32_t* experts, int64_t N, int
     ASCA_REQUIRE(ctx, experts && perm && slot && ws, "moe_topk_dispatch: null pointer");
     ASCA_REQUIRE(ctx, asca_aligned(ws, 256) && ws_bytes >= (size_t)asca_moe_topk_dispatch_ws(N, K, E),
                  "moe_topk_dispatch: the workspace has to have asca_moe_topk_dispatch_ws bytes, 256-byte aligned");
-    stable_sort::Pass p;
-    p.ids = (const uint32_t*)experts;
-    p.limit = (uint32_t)E;
-    p.n = N * K;
-    p.bins = (int)E + 1;
-    p.out_items = perm;
-    p.place = slot;
-    return stable_sort::run(ctx, p, (int32_t*)ws, offsets, (int)E + 1);
+    stable_sort::Job j{};
+    j.ids = (const uint32_t*)experts;
+    j.limit = (uint32_t)E;
+    j.n = N * K;
+    j.passes = 1;
+    j.bins = (int)E + 1;
+    j.items[0] = perm;
+    j.place = slot;
+    j.offsets = offsets;
+    return stable_sort::sort(ctx, j, (int32_t*)ws);
 }
 
 int asca_moe_sort_rows(asca_ctx* ctx, const void* x, const int32_t* slot, int64_t N, int64_t K, int64_t d, int x_dtype, int xs_dtype, void* xs) {
@@ -147,14 +217,13 @@ int asca_moe_sort_rows(asca_ctx* ctx, const void* x, const int32_t* slot, int64_
     if (N == 0) return ASCA_OK;
     ASCA_REQUIRE(ctx, x && slot && xs, "moe_sort_rows: null pointer");
     asca_device_scope on(ctx);
-    const bool four = asca_rows_by_four(x, d, x_dtype) && asca_rows_by_four(xs, d, xs_dtype);
-    const Shape s = by_token(N, four ? d / 4 : d);
+    const int v = asca_row_width(d, x, x_dtype, xs, xs_dtype);
+    const dim3 block = asca_row_block(asca_row_frags(d, v), 256), grid((unsigned)ceil_div64(N, (int64_t)block.y * TOKENS));
     asca_with_dtype(x, x_dtype, [&](auto a) {
         asca_with_dtype(xs, xs_dtype, [&](auto b) {
             using TX = std::remove_const_t<std::remove_pointer_t<decltype(a)>>;
             using TS = std::remove_pointer_t<decltype(b)>;
-            if (four) sort_rows_kernel<4, TX, TS><<<s.grid, s.block, 0, ctx->stream>>>(a, slot, N, (int)K, (int)d, b);
-            else sort_rows_kernel<1, TX, TS><<<s.grid, s.block, 0, ctx->stream>>>(a, slot, N, (int)K, (int)d, b);
+            asca_with_width<TX, TS>(v, [&](auto w) { sort_rows_kernel<w(), TX, TS><<<grid, block, 0, ctx->stream>>>(a, slot, N, (int)K, (int)d, b); });
         });
     });
     ASCA_CHECK_LAUNCH(ctx);
@@ -168,14 +237,17 @@ int asca_moe_unsort_rows(asca_ctx* ctx, const void* ys, const int32_t* slot, con
     if (N == 0) return ASCA_OK;
     ASCA_REQUIRE(ctx, ys && slot && out, "moe_unsort_rows: null pointer");
     asca_device_scope on(ctx);
-    const bool four = asca_rows_by_four(ys, d, ys_dtype) && asca_rows_by_four(out, d, out_dtype);
-    const Shape s = by_token(N, four ? d / 4 : d);
+    const int v = asca_row_width(d, ys, ys_dtype, out, out_dtype);
+    const Team team(asca_row_frags(d, v), K);
     asca_with_dtype(ys, ys_dtype, [&](auto a) {
         asca_with_dtype(out, out_dtype, [&](auto b) {
             using TS = std::remove_const_t<std::remove_pointer_t<decltype(a)>>;
             using TX = std::remove_pointer_t<decltype(b)>;
-            if (four) unsort_rows_kernel<4, TS, TX><<<s.grid, s.block, 0, ctx->stream>>>(a, slot, weights, N, (int)K, (int)d, b);
-            else unsort_rows_kernel<1, TS, TX><<<s.grid, s.block, 0, ctx->stream>>>(a, slot, weights, N, (int)K, (int)d, b);
+            asca_with_width<TX, TS>(v, [&](auto w) {
+                team.with([&](auto l, auto ks) {
+                    unsort_rows_kernel<w(), l(), ks(), TS, TX><<<team.blocks(N), 256, 0, ctx->stream>>>(a, slot, weights, N, (int)K, (int)d, b);
+                });
+            });
         });
     });
     ASCA_CHECK_LAUNCH(ctx);
@@ -194,15 +266,18 @@ int asca_moe_unsort_rows_bwd(asca_ctx* ctx, const void* d_out, const void* ys, c
     ASCA_REQUIRE(ctx, d_out && slot && d_ys, "moe_unsort_rows_bwd: null pointer");
     ASCA_REQUIRE(ctx, !d_w || ys, "moe_unsort_rows_bwd: the weights' gradient needs ys");
     asca_device_scope on(ctx);
-    const bool four = asca_rows_by_four(d_out, d, out_dtype) && asca_rows_by_four(ys, d, ys_dtype) && asca_rows_by_four(d_ys, d, ys_dtype);
-    const unsigned grid = (unsigned)ceil_div64(N, 8);
+    const int v = std::min(asca_row_width(d, d_out, out_dtype, ys, ys_dtype), asca_row_width(d, d_out, out_dtype, d_ys, ys_dtype));
+    const Team team(asca_row_frags(d, v), K);
     asca_with_dtype(d_out, out_dtype, [&](auto a) {
         asca_with_dtype(d_ys, ys_dtype, [&](auto b) {
             using TX = std::remove_const_t<std::remove_pointer_t<decltype(a)>>;
             using TS = std::remove_pointer_t<decltype(b)>;
-            const TS* y = static_cast<const TS*>(ys);
-            if (four) unsort_rows_bwd_kernel<4, TX, TS><<<grid, 256, 0, ctx->stream>>>(a, y, slot, weights, N, (int)K, (int)d, b, d_w);
-            else unsort_rows_bwd_kernel<1, TX, TS><<<grid, 256, 0, ctx->stream>>>(a, y, slot, weights, N, (int)K, (int)d, b, d_w);
+            asca_with_width<TX, TS>(v, [&](auto w) {
+                team.with([&](auto l, auto ks) {
+                    unsort_rows_bwd_kernel<w(), l(), ks(), TX, TS><<<team.blocks(N), 256, 0, ctx->stream>>>(a, static_cast<const TS*>(ys), slot, weights, N,
+                                                                                                           (int)K, (int)d, b, d_w);
+                });
+            });
         });
     });
     ASCA_CHECK_LAUNCH(ctx);

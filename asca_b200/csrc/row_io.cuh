@@ -2,6 +2,7 @@
 #pragma once
 #include "common.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 // Makes the context's device current while an entry point launches, for callers that have another one current.
@@ -19,8 +20,10 @@ struct asca_device_scope {
 inline bool asca_known_dtype(int dtype) { return dtype == ASCA_F32 || dtype == ASCA_BF16; }
 inline size_t asca_dtype_size(int dtype) { return dtype == ASCA_BF16 ? 2 : 4; }
 inline bool asca_aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-// four elements of a row of `cols` can be moved at once at every multiple of four columns (a null pointer has no rows)
-inline bool asca_rows_by_four(const void* p, int64_t cols, int dtype) { return (cols & 3) == 0 && asca_aligned(p, 4 * asca_dtype_size(dtype)); }
+// v (4 or 8) elements of a row of `cols` can be moved at once at every multiple of v columns (a null pointer has no rows)
+inline bool asca_rows_by(int v, const void* p, int64_t cols, int dtype) {
+    return cols % v == 0 && asca_aligned(p, std::min<size_t>(16, v * asca_dtype_size(dtype)));
+}
 
 // f(pointer of the type that `dtype` names); a const pointer stays const
 template <typename F>
@@ -34,7 +37,48 @@ inline void asca_with_dtype(void* p, int dtype, F f) {
     else f(static_cast<float*>(p));
 }
 
+// How a thread moves its columns between rows of two types (frag below): 8 together where a bf16 side then moves 16 bytes, else 4, else
+// (1) single columns; and f(std::integral_constant of that), eight only for pairs of types that have it.
+inline int asca_row_width(int64_t cols, const void* a, int a_dtype, const void* b, int b_dtype) {
+    if ((a_dtype == ASCA_BF16 || b_dtype == ASCA_BF16) && asca_rows_by(8, a, cols, a_dtype) && asca_rows_by(8, b, cols, b_dtype)) return 8;
+    return asca_rows_by(4, a, cols, a_dtype) && asca_rows_by(4, b, cols, b_dtype) ? 4 : 1;
+}
+inline int64_t asca_row_frags(int64_t cols, int width) { return ceil_div64(cols, width == 1 ? 4 : width); }
 #ifdef __CUDACC__
+// A block of at most `threads` (a power of two) with a power of two or whole warps of lanes a row of `frags` groups of columns, as few
+// rounds as that allows, the lanes spread evenly over them; and the rows beside each other.
+inline dim3 asca_row_block(int64_t frags, int threads) {
+    int tx = 1;
+    while (tx < frags && tx < 32) tx *= 2;
+    if (frags > 32) tx = (int)ceil_div64(ceil_div64(frags, ceil_div64(frags, threads)), 32) * 32;
+    return dim3(tx, threads / tx);
+}
+#endif
+template <typename A, typename B, typename F>
+inline void asca_with_width(int v, F f) {
+    if constexpr (sizeof(A) == 2 || sizeof(B) == 2)
+        if (v == 8) return f(std::integral_constant<int, 8>());
+    if (v == 4) f(std::integral_constant<int, 4>());
+    else f(std::integral_constant<int, 1>());
+}
+
+#ifdef __CUDACC__
+// Launches a kernel that begins with pdl_wait() behind the one before it on the stream without waiting for that one's end to be
+// scheduled: a second or third launch of one call then costs about a microsecond less.
+template <typename... KArgs, typename... Args>
+inline cudaError_t asca_launch_after(asca_ctx* ctx, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
+}
 __device__ __forceinline__ float2 bf16x2_f32(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
 __device__ __forceinline__ uint32_t f32_bf16x2(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -49,20 +93,102 @@ __device__ __forceinline__ float4 ld4(const __nv_bfloat16* p) {
 __device__ __forceinline__ void st4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
 __device__ __forceinline__ void st4(__nv_bfloat16* p, float4 v) { *reinterpret_cast<uint2*>(p) = make_uint2(f32_bf16x2(v.x, v.y), f32_bf16x2(v.z, v.w)); }
 
-// V consecutive elements: V = 4 through the vector forms, V = 1 for rows off their grid or of a width that four does not divide
+// V consecutive elements as they lie in memory, for loads that wait their turn in half the registers or move on unchanged
 template <int V, typename T>
-__device__ __forceinline__ void ld_row(const T* p, float (&v)[V]) {
-    if constexpr (V == 4) {
-        const float4 x = ld4(p);
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-    } else {
-        static_assert(V == 1, "four or one");
-        v[0] = to_f32<T>(*p);
-    }
+struct raw_row {
+    T v;
+};
+template <>
+struct raw_row<4, float> {
+    float4 v;
+};
+template <>
+struct raw_row<8, float> {
+    float4 v, w;
+};
+template <>
+struct raw_row<4, __nv_bfloat16> {
+    uint2 v;
+};
+template <>
+struct raw_row<8, __nv_bfloat16> {
+    uint4 v;
+};
+// V consecutive elements of a row: 8 or 4 through 16-byte accesses (8 for bf16 alone), 1 for rows off their grid or of another width
+template <int V, typename T>
+__device__ __forceinline__ raw_row<V, T> ld_raw(const T* p) {
+    raw_row<V, T> r;
+    if constexpr (V == 8 && sizeof(T) == 4) {
+        r.v = *reinterpret_cast<const float4*>(p);
+        r.w = *reinterpret_cast<const float4*>(p + 4);
+    } else r.v = *reinterpret_cast<const decltype(r.v)*>(p);
+    return r;
 }
+template <int V, typename T>
+__device__ __forceinline__ void st_raw(T* p, const raw_row<V, T>& r) {
+    *reinterpret_cast<std::remove_const_t<decltype(r.v)>*>(p) = r.v;
+    if constexpr (V == 8 && sizeof(T) == 4) *reinterpret_cast<float4*>(p + 4) = r.w;
+}
+__device__ __forceinline__ void unpack(const raw_row<1, float>& r, float (&v)[1]) { v[0] = r.v; }
+__device__ __forceinline__ void unpack(const raw_row<1, __nv_bfloat16>& r, float (&v)[1]) { v[0] = __bfloat162float(r.v); }
+__device__ __forceinline__ void unpack4(const float4& x, float* v) { v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
+__device__ __forceinline__ void unpack(const raw_row<4, float>& r, float (&v)[4]) { unpack4(r.v, v); }
+__device__ __forceinline__ void unpack(const raw_row<8, float>& r, float (&v)[8]) { unpack4(r.v, v); unpack4(r.w, v + 4); }
+__device__ __forceinline__ void unpack2(uint32_t u, float* v) {
+    const float2 x = bf16x2_f32(u);
+    v[0] = x.x; v[1] = x.y;
+}
+__device__ __forceinline__ void unpack(const raw_row<4, __nv_bfloat16>& r, float (&v)[4]) { unpack2(r.v.x, v); unpack2(r.v.y, v + 2); }
+__device__ __forceinline__ void unpack(const raw_row<8, __nv_bfloat16>& r, float (&v)[8]) {
+    unpack2(r.v.x, v); unpack2(r.v.y, v + 2); unpack2(r.v.z, v + 4); unpack2(r.v.w, v + 6);
+}
+template <int V, typename T>
+__device__ __forceinline__ void ld_row(const T* p, float (&v)[V]) { unpack(ld_raw<V>(p), v); }
 template <int V, typename T>
 __device__ __forceinline__ void st_row(T* p, const float (&v)[V]) {
-    if constexpr (V == 4) st4(p, make_float4(v[0], v[1], v[2], v[3]));
-    else *p = from_f32<T>(v[0]);
+    if constexpr (V == 8 && sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(f32_bf16x2(v[0], v[1]), f32_bf16x2(v[2], v[3]), f32_bf16x2(v[4], v[5]), f32_bf16x2(v[6], v[7]));
+    } else if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) st4(p + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+    } else *p = from_f32<T>(v[0]);
 }
+
+// A thread's columns of a row that `lanes` threads share: W = 8 or 4 together, or W = 1: four single ones, `lanes` apart. Thread x begins at
+// frag_first(x) and goes on by lanes * frag<W, T>::E.
+template <int W, typename T>
+struct frag {
+    static constexpr int E = W;
+    raw_row<W, T> r;
+    __device__ __forceinline__ void load(const T* row, int c, int, int) { r = ld_raw<W>(row + c); }
+    __device__ __forceinline__ void store(T* row, int c, int, int) const { st_raw<W>(row + c, r); }
+    __device__ __forceinline__ void get(float (&v)[E]) const { unpack(r, v); }
+    static __device__ __forceinline__ void put(T* row, int c, int, int, const float (&v)[E]) { st_row<W>(row + c, v); }
+};
+template <typename T>
+struct frag<1, T> {
+    static constexpr int E = 4;
+    T r[4];
+    __device__ __forceinline__ void load(const T* row, int c, int lanes, int cols) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i * lanes < cols) r[i] = row[c + i * lanes];
+    }
+    __device__ __forceinline__ void store(T* row, int c, int lanes, int cols) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i * lanes < cols) row[c + i * lanes] = r[i];
+    }
+    __device__ __forceinline__ void get(float (&v)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = to_f32<T>(r[i]);
+    }
+    static __device__ __forceinline__ void put(T* row, int c, int lanes, int cols, const float (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i * lanes < cols) row[c + i * lanes] = from_f32<T>(v[i]);
+    }
+};
+template <int W>
+__device__ __forceinline__ int frag_first(int x) { return W == 1 ? x : x * W; }
 #endif
