@@ -28,8 +28,8 @@ NN, TN, NT = 0, 1, 2
 _lib = None
 
 
-# Argument types of the entry points that asca_b200.ops calls with plain Python values (a pointer is an int or None): converted
-# by ctypes itself, at a fraction of the cost of wrapping each value.
+# Argument types of entry points that take plain Python values through Gpu._run (a pointer is an int or None), for callers with
+# memory of their own; asca_b200.ops reaches the same ones through asca_b200._torch_ops.
 _P, _L, _I, _F, _Z = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_size_t
 _SIGNATURES = {
     "asca_embed_scaled_fwd": (_I, [_P, _P, _P, _L, _L, _L, _F, _I, _I, _P]),
@@ -179,6 +179,7 @@ class Gpu:
             raise AscaError(rc, f"cannot create a context on CUDA device {device} (no GPU, or driver missing); "
                                 "there is no CPU fallback")
         self._ctx = ctx
+        self.handle = ctx.value   # the context's address, 0 once it is closed
         self.device = device
         self.bound_stream = 0   # the handle that set_stream was given last; 0 = the context's own stream
 
@@ -188,14 +189,11 @@ class Gpu:
         if rc != 0:
             raise AscaError(rc, self.lib.asca_last_error(self._ctx).decode())
 
-    def _fail(self, rc, msg=None):
-        raise AscaError(rc, msg or self.lib.asca_last_error(self._ctx).decode())
-
     def _run(self, name, *args):
         """An entry point with a row in _SIGNATURES, on plain Python values."""
         rc = getattr(self.lib, name)(self._ctx, *args)
         if rc != 0:
-            self._fail(rc)
+            raise AscaError(rc, self.lib.asca_last_error(self._ctx).decode())
 
     def describe(self) -> str:
         return self.lib.asca_describe(self._ctx).decode()
@@ -243,6 +241,7 @@ class Gpu:
         if self._ctx:
             self.lib.asca_ctx_destroy(self._ctx)
             self._ctx = None
+            self.handle = 0
 
     # ---- Gpu::matmul / matmul_ta (rust/src/cuda/mod.rs:286-344)
     def matmul(self, a, b):

@@ -2,6 +2,9 @@
 
     python -m asca_b200.build [--force] [--verbose]
 
+asca_b200/_torch_ops.so, the binding of asca_b200.ops to torch tensors (csrc/torch_ops.cpp), is built beside it with g++
+against the torch of this interpreter.
+
 Each .cu under csrc/ is compiled to an object in csrc/build/ (skipped when newer than the
 source and the headers), then linked into asca_b200/libasca_b200.so with the static CUDA
 runtime, so loading the library needs no CUDA installation beyond the driver.
@@ -19,6 +22,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OBJ = CSRC / "build"
 SO = PKG / "libasca_b200.so"
+TORCH_OPS = PKG / "_torch_ops.so"
 INCLUDE = PKG.parent / "include"
 
 NVCC_FLAGS = [
@@ -80,6 +84,29 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return SO
 
 
+def build_torch_ops(force: bool = False) -> Path:
+    """The binding of asca_b200.ops (the library itself has been built). Torch's own libraries are in the process when it is
+    loaded; libasca_b200.so is found beside it."""
+    import importlib.util
+    import sysconfig
+
+    src = CSRC / "torch_ops.cpp"
+    torch = Path(importlib.util.find_spec("torch").origin).parent
+    if not force and not _stale(TORCH_OPS, [src, *sorted(INCLUDE.glob("*.h")), torch / "version.py"]):
+        return TORCH_OPS
+    cuda = Path(nvcc()).resolve().parent.parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
+           "-I", sysconfig.get_paths()["include"], "-I", str(torch / "include"), "-I", str(torch / "include/torch/csrc/api/include"),
+           "-I", str(cuda / "include"), str(src), "-o", str(TORCH_OPS), "-L", str(PKG), f"-l:{SO.name}", "-L", str(torch / "lib"),
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
+        raise RuntimeError("g++ failed on torch_ops.cpp")
+    return TORCH_OPS
+
+
 if __name__ == "__main__":
     out = build(force="--force" in sys.argv, verbose="--verbose" in sys.argv)
+    build_torch_ops(force="--force" in sys.argv)
     print(out)

@@ -13,6 +13,11 @@ import torch
 
 from . import BF16, F32, NN, NT, TN, Gpu, _f, _i64, _p  # noqa: F401
 
+try:
+    from . import _torch_ops as _t
+except ImportError as e:   # no slower way in its place
+    raise ImportError("asca_b200/_torch_ops.so is missing or was built for another torch: build it with `python -m asca_b200.build`") from e
+
 
 def _dt(t: torch.Tensor) -> int:
     if t.dtype == torch.float32:
@@ -99,10 +104,7 @@ def adamw_segmented(gpu, p, g, m, v, seg_off, lr_t, eps_t, beta1, beta2, wd_eff,
     lr_t = np.ascontiguousarray(lr_t, dtype=np.float32)
     eps_t = np.ascontiguousarray(eps_t, dtype=np.float32)
     if norm is not None:
-        _on_stream(gpu)
-        ptrs = [_need(gpu, name, t, (p.numel(),), torch.float32) for name, t in (("p", p), ("g", g), ("m", m), ("v", v))]
-        gpu._run("asca_adamw_segmented_clip", *ptrs, seg_off.ctypes.data, lr_t.ctypes.data, eps_t.ctypes.data, lr_t.size, float(beta1), float(beta2), float(wd_eff), None,
-                 _need(gpu, "norm", norm, (1,), torch.float32), float(max_norm))
+        _t.adamw_clip(gpu.handle, gpu.device, gpu.bound_stream, p, g, m, v, seg_off, lr_t, eps_t, beta1, beta2, wd_eff, norm, max_norm)
         return
     gpu._call("asca_adamw_segmented", gpu._ctx, _p(p), _p(g), _p(m), _p(v), _p(seg_off), _p(lr_t), _p(eps_t),
               C.c_int(lr_t.size), _f(beta1), _f(beta2), _f(wd_eff))
@@ -111,79 +113,18 @@ def adamw_segmented(gpu, p, g, m, v, seg_off, lr_t, eps_t, beta1, beta2, wd_eff,
 # ------------------------------------------------------------------ a training step around the blocks
 # These check their tensors (device, dtype, shape, contiguity) and that the context is on torch's current stream, because
 # scratch and outputs come from torch's allocator in that stream's order: call gpu.use_torch_stream() after changing streams.
-# A call that is captured into a CUDA graph has its scratch in the graph's own memory.
-_FLOATS = {torch.float32: F32, torch.bfloat16: BF16}
-
-
-def _need(gpu, name, t, shape=None, dtype=None):
-    """t is a contiguous tensor on the context's device with this shape (None: any extent) and dtype (None: f32 or bf16)."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device.index != gpu.device:
-        raise ValueError(f"{name}: expected a tensor on cuda:{gpu.device}")
-    if (t.dtype not in _FLOATS) if dtype is None else (t.dtype != dtype):
-        raise TypeError(f"{name}: expected {dtype or 'float32 or bfloat16'}, got {t.dtype}")
-    if shape is not None and (t.dim() != len(shape) or any(want is not None and want != got for want, got in zip(shape, t.shape))):
-        raise ValueError(f"{name}: expected the shape {tuple('any' if x is None else x for x in shape)}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous tensor")
-    return t.data_ptr()
-
-
-def _on_stream(gpu):
-    if gpu.bound_stream != (torch._C._cuda_getCurrentRawStream(gpu.device) or 1):
-        raise RuntimeError("the context is not on torch's current stream: call gpu.use_torch_stream()")
-
-
-def _new(like, shape, dtype):
-    return torch.empty(shape, dtype=dtype, device=like.device)
-
-
-def _scratch(like, nbytes):
-    """Scratch of an entry point (negative: sizes that it will refuse): (the tensor, its address, its size)."""
-    ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=like.device)
-    return ws, ws.data_ptr(), max(nbytes, 0)
-
-
+# A call that is captured into a CUDA graph has its scratch in the graph's own memory. The work of the wrappers is done in
+# csrc/torch_ops.cpp.
 def embed_fwd(gpu, table, ids, scale=1.0, out_dtype=None, out=None):
     """x[t] = scale * table[ids[t]]: table (V, d) f32 or bf16, ids int32 or uint32 of any shape; an id outside the table (-1, say) is
     padding and gives zeros. Returns ids.shape + (d,) in ``out_dtype`` (default: the table's)."""
-    _on_stream(gpu)
-    p_table, p_ids = _need(gpu, "table", table, (None, None)), _need(gpu, "ids", ids, dtype=torch.uint32 if ids.dtype == torch.uint32 else torch.int32)
-    v, d = table.shape
-    shape = (*ids.shape, d)
-    if out is None:
-        out = _new(table, shape, out_dtype or table.dtype)
-    p_out = _need(gpu, "out", out, shape, out_dtype)
-    gpu._run("asca_embed_scaled_fwd", p_table, p_ids, ids.numel(), d, v, float(scale), _FLOATS[table.dtype], _FLOATS[out.dtype], p_out)
-    return out
+    return _t.embed_fwd(gpu.handle, gpu.device, gpu.bound_stream, table, ids, scale, out_dtype, out)
 
 
 def embed_bwd(gpu, dx, ids, vocab, scale=1.0, d_table=None, accumulate=False):
     """The gradient of :func:`embed_fwd` for a table of ``vocab`` rows: d_table[v] = scale * (sum of dx[t] over ids[t] == v), f32;
     with ``accumulate`` added to the given ``d_table``, of which only the rows of the tokens that occur are touched."""
-    _on_stream(gpu)
-    p_ids = _need(gpu, "ids", ids, dtype=torch.uint32 if ids.dtype == torch.uint32 else torch.int32)
-    d = dx.shape[-1]
-    p_dx = _need(gpu, "dx", dx, (*ids.shape, None))
-    if d_table is None:
-        if accumulate:
-            raise ValueError("embed_bwd: accumulate needs the d_table to add to")
-        d_table = _new(dx, (vocab, d), torch.float32)
-    p_dt = _need(gpu, "d_table", d_table, (vocab, d), torch.float32)
-    _ws, p_ws, nbytes = _scratch(dx, gpu.lib.asca_embed_scaled_bwd_ws(ids.numel(), d, vocab))
-    gpu._run("asca_embed_scaled_bwd", p_dx, p_ids, ids.numel(), d, vocab, float(scale), _FLOATS[dx.dtype], 1 if accumulate else 0, p_dt, p_ws, nbytes)
-    return d_table
-
-
-def _join_args(gpu, y, gate, gate_rows, w_post, w_pre, post_norm):
-    """The checks that both directions of the join share: (rows, cols, gate_rows, pointers of w_post, gate and w_pre)."""
-    _need(gpu, "y", y, (None, None))
-    rows, cols = y.shape
-    gate_rows = gate_rows or max(rows, 1)
-    p_gate = None if gate is None else _need(gpu, "gate", gate, (-(-rows // gate_rows), cols), torch.float32)
-    if w_post is not None and not post_norm:
-        raise ValueError("w_post belongs to the norm after the block: post_norm is False")
-    p_post, p_pre = (None if w is None else _need(gpu, n, w, (cols,), torch.float32) for n, w in (("w_post", w_post), ("w_pre", w_pre)))
-    return rows, cols, gate_rows, p_post, p_gate, p_pre
+    return _t.embed_bwd(gpu.handle, gpu.device, gpu.bound_stream, dx, ids, vocab, scale, d_table, accumulate)
 
 
 def gated_residual_rmsnorm_fwd(gpu, y, x, gate=None, gate_rows=None, w_post=None, w_pre=None, post_norm=True, skip_scale=1.0, branch_scale=1.0,
@@ -193,125 +134,52 @@ def gated_residual_rmsnorm_fwd(gpu, y, x, gate=None, gate_rows=None, w_post=None
     n = rmsnorm(y) * w_post (y itself without ``post_norm``), x_out = skip_scale * x + branch_scale * gate[r // gate_rows] * n,
     xn = rmsnorm(x_out) * w_pre in y's dtype. gate (ceil(rows / gate_rows), cols) f32, gate_rows None: one gate for all rows.
     Returns (x_out, xn); xn is None without ``want_norm``. ``x_out`` may be x."""
-    _on_stream(gpu)
-    rows, cols, gate_rows, p_post, p_gate, p_pre = _join_args(gpu, y, gate, gate_rows, w_post, w_pre, post_norm)
-    p_x = _need(gpu, "x", x, (rows, cols), torch.float32)
-    if x_out is None:
-        x_out = torch.empty_like(x)
-    p_xo = _need(gpu, "x_out", x_out, (rows, cols), torch.float32)
-    xn = torch.empty_like(y) if want_norm else None
-    gpu._run("asca_gated_residual_rmsnorm_fwd", y.data_ptr(), p_x, p_post, p_gate, gate_rows, p_pre, 1 if post_norm else 0, float(skip_scale), float(branch_scale), float(eps),
-             rows, cols, _FLOATS[y.dtype], p_xo, xn.data_ptr() if want_norm else None)
-    return x_out, xn
+    return _t.join_fwd(gpu.handle, gpu.device, gpu.bound_stream, y, x, gate, gate_rows, w_post, w_pre, post_norm, skip_scale, branch_scale, eps,
+                       want_norm, x_out)
 
 
 def gated_residual_rmsnorm_bwd(gpu, y, x_out, d_xn, d_out, gate=None, gate_rows=None, w_post=None, w_pre=None, post_norm=True, skip_scale=1.0,
                                branch_scale=1.0, eps=1e-6, grads=None):
     """Gradients of :func:`gated_residual_rmsnorm_fwd`, from d_xn (y's dtype) and d_out (f32, what reaches x_out from further on);
     one of the two may be None. Returns a dict: d_x, d_y, and d_gate, d_w_post, d_w_pre for those of the three that are given.
-    ``grads``: a dict with some of these three tensors to add to instead of making new ones."""
-    _on_stream(gpu)
-    rows, cols, gate_rows, p_post, p_gate, p_pre = _join_args(gpu, y, gate, gate_rows, w_post, w_pre, post_norm)
-    p_xo = _need(gpu, "x_out", x_out, (rows, cols), torch.float32)
-    p_dn = None if d_xn is None else _need(gpu, "d_xn", d_xn, (rows, cols), y.dtype)
-    p_do = None if d_out is None else _need(gpu, "d_out", d_out, (rows, cols), torch.float32)
-    if d_xn is None and d_out is None:
-        raise ValueError("gated_residual_rmsnorm_bwd: needs d_xn or d_out")
-    out = {"d_x": torch.empty_like(x_out), "d_y": torch.empty_like(y)}
-    sums = [None, None, None]
-    for i, (name, w) in enumerate((("d_w_post", w_post), ("d_gate", gate), ("d_w_pre", w_pre))):
-        if w is not None:
-            out[name] = grads[name] if grads is not None else torch.empty_like(w)
-            sums[i] = _need(gpu, name, out[name], tuple(w.shape), torch.float32)
-    _ws, p_ws, nbytes = _scratch(y, gpu.lib.asca_gated_residual_rmsnorm_bwd_ws(gpu._ctx, rows, cols))
-    gpu._run("asca_gated_residual_rmsnorm_bwd", y.data_ptr(), p_xo, p_dn, p_do, p_post, p_gate, gate_rows, p_pre, 1 if post_norm else 0, float(skip_scale),
-             float(branch_scale), float(eps), rows, cols, _FLOATS[y.dtype], 0 if grads is None else 1, out["d_x"].data_ptr(), out["d_y"].data_ptr(), *sums,
-             p_ws, nbytes)
-    return out
+    ``grads``: a dict with these tensors to add to instead of making new ones."""
+    return _t.join_bwd(gpu.handle, gpu.device, gpu.bound_stream, y, x_out, d_xn, d_out, gate, gate_rows, w_post, w_pre, post_norm, skip_scale,
+                       branch_scale, eps, grads)
 
 
 def moe_topk_dispatch(gpu, experts, E):
     """experts (N, K) int32, a router's choice; one outside [0, E) (-1, say) sends the assignment nowhere. Returns perm (N*K: the
     assignments t*K + k by expert, ascending inside one, those that go nowhere last), offsets (E+1: the experts' bounds in perm) and
     slot (N, K: where each assignment lies in perm, -1 if it goes nowhere), all int32."""
-    _on_stream(gpu)
-    p_e = _need(gpu, "experts", experts, (None, None), torch.int32)
-    n, k = experts.shape
-    i32 = torch.int32
-    perm, offsets, slot = _new(experts, (n * k,), i32), _new(experts, (E + 1,), i32), _new(experts, (n, k), i32)
-    _ws, p_ws, nbytes = _scratch(experts, gpu.lib.asca_moe_topk_dispatch_ws(n, k, E))
-    gpu._run("asca_moe_topk_dispatch", p_e, n, k, E, perm.data_ptr(), offsets.data_ptr(), slot.data_ptr(), p_ws, nbytes)
-    return perm, offsets, slot
+    return _t.moe_dispatch(gpu.handle, gpu.device, gpu.bound_stream, experts, E)
 
 
 def moe_sort_rows(gpu, x, slot, out_dtype=None, out=None):
     """xs[slot[t, k]] = x[t]: (N, d) -> (N*K, d) in expert order. Rows behind the last expert's are left as they were (in a new
     tensor: undefined)."""
-    _on_stream(gpu)
-    p_x, p_s = _need(gpu, "x", x, (None, None)), _need(gpu, "slot", slot, (x.shape[0], None), torch.int32)
-    (n, d), k = x.shape, slot.shape[1]
-    if out is None:
-        out = _new(x, (n * k, d), out_dtype or x.dtype)
-    p_o = _need(gpu, "out", out, (n * k, d), out_dtype)
-    gpu._run("asca_moe_sort_rows", p_x, p_s, n, k, d, _FLOATS[x.dtype], _FLOATS[out.dtype], p_o)
-    return out
+    return _t.moe_sort(gpu.handle, gpu.device, gpu.bound_stream, x, slot, out_dtype, out)
 
 
 def moe_sort_rows_bwd(gpu, d_xs, slot, out_dtype=torch.float32):
     """d_x[t] = sum over k of d_xs[slot[t, k]]."""
-    return moe_unsort_rows(gpu, d_xs, slot, None, out_dtype)
+    return _t.moe_unsort(gpu.handle, gpu.device, gpu.bound_stream, d_xs, slot, None, out_dtype, None)
 
 
 def moe_unsort_rows(gpu, ys, slot, weights=None, out_dtype=torch.float32, out=None):
-    """out[t] = sum over k of weights[t, k] * ys[slot[t, k]]: (N*K, d) in expert order -> (N, d). weights (N, K) f32, None: ones."""
-    _on_stream(gpu)
-    n, k = slot.shape
-    p_s, p_y = _need(gpu, "slot", slot, (None, None), torch.int32), _need(gpu, "ys", ys, (n * k, None))
-    p_w = None if weights is None else _need(gpu, "weights", weights, (n, k), torch.float32)
-    d = ys.shape[1]
-    if out is None:
-        out = _new(ys, (n, d), out_dtype)
-    p_o = _need(gpu, "out", out, (n, d))
-    gpu._run("asca_moe_unsort_rows", p_y, p_s, p_w, n, k, d, _FLOATS[ys.dtype], _FLOATS[out.dtype], p_o)
-    return out
+    """out[t] = sum over k of weights[t, k] * ys[slot[t, k]]: (N*K, d) in expert order -> (N, d). weights (N, K) f32, None: ones.
+    A given ``out`` has its own dtype."""
+    return _t.moe_unsort(gpu.handle, gpu.device, gpu.bound_stream, ys, slot, weights, out_dtype, out)
 
 
 def moe_unsort_rows_bwd(gpu, d_out, ys, slot, weights=None, d_ys=None):
     """Gradients of :func:`moe_unsort_rows`: (d_ys in ys' dtype, rows behind the last expert's left as they were; d_w (N, K) f32, or
-    None without weights)."""
-    _on_stream(gpu)
-    n, k = slot.shape
-    p_s, p_y = _need(gpu, "slot", slot, (None, None), torch.int32), _need(gpu, "ys", ys, (n * k, None))
-    d = ys.shape[1]
-    p_g = _need(gpu, "d_out", d_out, (n, d))
-    p_w = None if weights is None else _need(gpu, "weights", weights, (n, k), torch.float32)
-    if d_ys is None:
-        d_ys = torch.empty_like(ys)
-    p_dy = _need(gpu, "d_ys", d_ys, (n * k, d), ys.dtype)
-    d_w = None if weights is None else _new(ys, (n, k), torch.float32)
-    gpu._run("asca_moe_unsort_rows_bwd", p_g, p_y if weights is not None else None, p_s, p_w, n, k, d, _FLOATS[d_out.dtype], _FLOATS[ys.dtype], p_dy,
-             None if d_w is None else d_w.data_ptr())
-    return d_ys, d_w
-
-
-def _tensor_table(gpu, grads):
-    """Host arrays of the tensors' addresses, lengths and dtypes."""
-    n = len(grads)
-    for i, g in enumerate(grads):
-        _need(gpu, f"grads[{i}]", g)
-    return (C.c_void_p * n)(*[g.data_ptr() for g in grads]), (C.c_int64 * n)(*[g.numel() for g in grads]), (C.c_int * n)(*[_FLOATS[g.dtype] for g in grads]), n
+    None without weights). ``d_ys`` may be ys."""
+    return _t.moe_unsort_bwd(gpu.handle, gpu.device, gpu.bound_stream, d_out, ys, slot, weights, d_ys)
 
 
 def grad_norm(gpu, grads, out=None):
     """The L2 norm over all elements of all tensors (f32 and bf16 may be mixed), as a device tensor (1,) f32; no wait."""
-    _on_stream(gpu)
-    p, n, dt, count = _tensor_table(gpu, grads)
-    if out is None:
-        out = torch.empty(1, dtype=torch.float32, device=torch.device("cuda", gpu.device))
-    p_out = _need(gpu, "out", out, (1,), torch.float32)
-    _ws, p_ws, nbytes = _scratch(out, gpu.lib.asca_grad_norm_ws(gpu._ctx, count))
-    gpu._run("asca_grad_norm", p, n, dt, count, p_out, p_ws, nbytes)
-    return out
+    return _t.grad_norm(gpu.handle, gpu.device, gpu.bound_stream, grads, out)
 
 
 def clip_grads(gpu, grads, max_norm, norm=None):
@@ -319,10 +187,7 @@ def clip_grads(gpu, grads, max_norm, norm=None):
     Tensors must not overlap. An optimizer step that follows in :func:`adamw_segmented` can clip by itself, without this pass."""
     if norm is None:
         norm = grad_norm(gpu, grads)
-    _on_stream(gpu)
-    p_norm = _need(gpu, "norm", norm, (1,), torch.float32)
-    p, n, dt, count = _tensor_table(gpu, grads)
-    gpu._run("asca_clip_grads", p, n, dt, count, p_norm, float(max_norm))
+    _t.clip_grads(gpu.handle, gpu.device, gpu.bound_stream, grads, max_norm, norm)
     return norm
 
 

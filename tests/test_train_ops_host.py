@@ -6,12 +6,9 @@ import asca_b200
 from asca_b200 import ops
 
 
-class Nothing:
-    """Stands for a context on cuda:0 that must not be reached."""
-    device = 0
-
-    def _run(self, *args):
-        raise AssertionError("the library was called")
+class Closed:
+    """Stands for a context that has been closed."""
+    handle, device, bound_stream = 0, 0, 1
 
 
 def test_scratch_sizes():
@@ -32,9 +29,16 @@ def test_entry_points_refuse_a_null_context():
             assert getattr(lib, name)(*[None if a in (asca_b200._P,) else 0 for a in args]) == -1, name
 
 
-def test_tensors_that_are_not_on_the_device_are_refused():
-    t = torch.zeros(4, 8)
-    with pytest.raises(ValueError, match="cuda:0"):
-        ops._need(Nothing(), "x", t)
-    with pytest.raises(ValueError, match="x: expected"):
-        ops._need(Nothing(), "x", None)
+def test_a_closed_context_is_refused():
+    t, ids = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int32)
+    for call in (lambda: ops.embed_fwd(Closed(), t, ids), lambda: ops.grad_norm(Closed(), [t]), lambda: ops.moe_topk_dispatch(Closed(), ids.view(2, 2), 4),
+                 lambda: ops.gated_residual_rmsnorm_fwd(Closed(), t, t)):
+        with pytest.raises(ValueError, match="closed"):
+            call()
+
+
+def test_norm_and_largest_norm_belong_together():
+    t = torch.zeros(8)
+    for kw in (dict(norm=t), dict(max_norm=1.0)):
+        with pytest.raises((ValueError, AssertionError)):
+            ops.adamw_segmented(Closed(), t, t, t, t, [0, 8], [1e-3], [1e-8], 0.9, 0.95, 0.0, **kw)
