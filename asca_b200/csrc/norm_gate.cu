@@ -74,32 +74,89 @@ __device__ __forceinline__ void st_cols(T* p, int team, int tid, int cols, const
     }
 }
 
-// Sums of N values over a team, the same in all its threads. LANES: the team's part of a warp (8, 16, 32), or 0 for a whole CTA, which
-// alternates between two halves of `red` (`turn`), so that one barrier is enough: who writes a half again has passed the barrier of
-// the other, behind everybody's reading of this one.
-template <int LANES, int N>
-__device__ __forceinline__ void team_sum(float (&v)[N], float (*red)[32][8], int& turn) {
-    static_assert(N <= 8, "a warp's place holds eight");
+// Two columns at a time: half the instructions of the element-wise work, which is what the backward pass waits for next after HBM.
+using pair_t = unsigned long long;
+__device__ __forceinline__ pair_t pair(float a, float b) {
+    pair_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ pair_t pair(float a) { return pair(a, a); }
+__device__ __forceinline__ float2 two(pair_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+    pair_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) {
+    pair_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// Sums over a team, the same in all its threads. LANES: the team's part of a warp (8, 16, 32), or 0 for a whole CTA, which alternates
+// between two halves of `red` (`turn`), so that one barrier is enough: who writes a half again has passed the barrier of the other,
+// behind everybody's reading of this one.
+template <int LANES>
+__device__ __forceinline__ float team_sum(float v, float (*red)[32], int& turn) {
 #pragma unroll
-    for (int o = (LANES ? LANES : 32) / 2; o > 0; o >>= 1) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    }
+    for (int o = (LANES ? LANES : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if constexpr (LANES == 0) {
+        float* r = red[turn];
+        turn ^= 1;
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) r[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = lane < (int)(blockDim.x >> 5) ? r[lane] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    return v;
+}
+// Six sums. The first three steps halve what a lane has (it keeps the sums that three bits of its number name), so that six sums take
+// 7 shuffles and more where one takes 5; the way back to all lanes is one shuffle a sum.
+template <int LANES>
+__device__ __forceinline__ void team_sums(float (&v)[6], float (*red)[32][8], int& turn) {
+    constexpr int L = LANES ? LANES : 32;
+    const int lane = threadIdx.x & 31;
+    float a[4], b[2], c;
+    const bool hi = lane & (L / 2), mid = lane & (L / 4), low = lane & (L / 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float high = i + 4 < 6 ? v[(i + 4) % 6] : 0.0f;   // (v[6], v[7] are not there)
+        const float got = __shfl_xor_sync(0xffffffffu, hi ? v[i] : high, L / 2);
+        a[i] = (hi ? high : v[i]) + got;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) b[i] = (mid ? a[i + 2] : a[i]) + __shfl_xor_sync(0xffffffffu, mid ? a[i] : a[i + 2], L / 4);
+    c = (low ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, low ? b[0] : b[1], L / 8);
+#pragma unroll
+    for (int o = L / 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+    if constexpr (LANES == 0) {
+        // every warp adds the warps' sums: lane l those of its pair l % 4 and of every eighth warp from l / 4 on
         float(*r)[8] = red[turn];
         turn ^= 1;
-        const int nw = blockDim.x >> 5;
-        if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) r[threadIdx.x >> 5][i] = v[i];
-        }
+        if ((lane & 3) == 0) r[threadIdx.x >> 5][lane >> 2] = c;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = 0.0f;
-        for (int w = 0; w < nw; ++w) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] += r[w][i];
+        float2 s = make_float2(0.0f, 0.0f);
+        for (int w = lane >> 2; w < (int)(blockDim.x >> 5); w += 8) {
+            const float2 x = *reinterpret_cast<const float2*>(&r[w][(lane & 3) * 2]);
+            s.x += x.x; s.y += x.y;
         }
+#pragma unroll
+        for (int o = 16; o >= 4; o >>= 1) {
+            s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+            s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+        }
+#pragma unroll
+        for (int i = 0; i < 6; ++i) v[i] = __shfl_sync(0xffffffffu, i & 1 ? s.y : s.x, i >> 1);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) v[i] = __shfl_sync(0xffffffffu, c, (i >> 2 & 1) * (L / 2) + (i >> 1 & 1) * (L / 4) + (i & 1) * (L / 8), L);
     }
 }
 
@@ -120,7 +177,7 @@ struct Join {
 
 template <typename T, bool FOUR, int LANES, int MOST>
 __global__ void __launch_bounds__(MOST, 2048 / MOST) join_fwd_kernel(const Join a) {
-    __shared__ __align__(16) float red[2][32][8];
+    __shared__ float red[2][32];
     constexpr int TEAMS = LANES ? 256 / (LANES ? LANES : 1) : 1;   // a CTA's
     const int team = LANES ? LANES : blockDim.x, tid = LANES ? threadIdx.x % (LANES ? LANES : 1) : threadIdx.x;
     const int64_t r0 = LANES ? (int64_t)blockIdx.x * TEAMS + threadIdx.x / (LANES ? LANES : 1) : blockIdx.x;
@@ -131,12 +188,12 @@ __global__ void __launch_bounds__(MOST, 2048 / MOST) join_fwd_kernel(const Join 
     float y[EPT], x[EPT], w[EPT];
     ld_cols<FOUR>(static_cast<const T*>(a.y) + r * cols, team, tid, cols, y);
     ld_cols<FOUR>(a.x + r * cols, team, tid, cols, x);
-    float s[1] = {0.0f};
+    const float over = 1.0f / (float)cols;
+    float s = 0.0f;
     if (a.post) {
 #pragma unroll
-        for (int j = 0; j < EPT; ++j) s[0] += y[j] * y[j];
-        team_sum<LANES>(s, red, turn);
-        const float r1 = 1.0f / sqrtf(s[0] / (float)cols + a.eps);
+        for (int j = 0; j < EPT; ++j) s += y[j] * y[j];
+        const float r1 = rsqrtf(team_sum<LANES>(s, red, turn) * over + a.eps);
         ld_gain<FOUR>(a.w_post, team, tid, cols, w);
 #pragma unroll
         for (int j = 0; j < EPT; ++j) y[j] = y[j] * r1 * w[j];
@@ -146,16 +203,15 @@ __global__ void __launch_bounds__(MOST, 2048 / MOST) join_fwd_kernel(const Join 
 #pragma unroll
         for (int j = 0; j < EPT; ++j) y[j] *= w[j];
     }
-    s[0] = 0.0f;
+    s = 0.0f;
 #pragma unroll
     for (int j = 0; j < EPT; ++j) {
         x[j] = a.skip * x[j] + a.branch * y[j];
-        s[0] += x[j] * x[j];
+        s += x[j] * x[j];
     }
     if (live) st_cols<FOUR>(a.x_out + r * cols, team, tid, cols, x);
     if (!a.xn) return;
-    team_sum<LANES>(s, red, turn);
-    const float r2 = 1.0f / sqrtf(s[0] / (float)cols + a.eps);
+    const float r2 = rsqrtf(team_sum<LANES>(s, red, turn) * over + a.eps);
     ld_gain<FOUR>(a.w_pre, team, tid, cols, w);
 #pragma unroll
     for (int j = 0; j < EPT; ++j) x[j] = x[j] * r2 * w[j];
@@ -180,147 +236,196 @@ __device__ __forceinline__ void put_sum(float* p, int team, int tid, int cols, f
 template <bool FOUR, int STAGES, typename T>
 constexpr bool ahead() { return STAGES > 0 && (FOUR || sizeof(T) == 4); }
 template <int BYTES>
-__device__ __forceinline__ void copy_ahead(void* dst, const void* src) {
-    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
+__device__ __forceinline__ void copy_ahead(uint32_t dst, const void* src) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
+// place: of this thread's first columns; row: its first columns'
 template <bool FOUR, int STAGES, typename T>
-__device__ __forceinline__ void ask_row(T* place, const T* row, int team, int tid, int cols) {
+__device__ __forceinline__ void ask_row(uint32_t place, const T* row, int team, int left) {
     if constexpr (ahead<FOUR, STAGES, T>()) {
         constexpr int V = FOUR ? 4 : 1;
 #pragma unroll
-        for (int q = 0; q < EPT / V; ++q) {
-            const int c = (q * team + tid) * V;
-            if (c < cols) copy_ahead<V * sizeof(T)>(place + ((size_t)q * blockDim.x + threadIdx.x) * V, row + c);
-        }
+        for (int q = 0; q < EPT / V; ++q)
+            if (q * team * V < left) copy_ahead<V * sizeof(T)>(place + q * blockDim.x * (uint32_t)(V * sizeof(T)), row + q * team * V);
     }
 }
 template <bool FOUR, int STAGES, typename T>
-__device__ __forceinline__ void take_row(const T* place, const T* row, int team, int tid, int cols, float (&v)[EPT]) {
-    if constexpr (ahead<FOUR, STAGES, T>()) {
-        constexpr int V = FOUR ? 4 : 1;
+__device__ __forceinline__ void take_row(const T* place, const T* row, int team, int left, float (&v)[EPT]) {
+    constexpr int V = FOUR ? 4 : 1;
 #pragma unroll
-        for (int q = 0; q < EPT / V; ++q) {
-            float t[V];
-            ld_row<V>(place + ((size_t)q * blockDim.x + threadIdx.x) * V, t);
-            const bool in = (q * team + tid) * V < cols;
+    for (int q = 0; q < EPT / V; ++q) {
+        float t[V] = {};
+        if (q * team * V < left) ld_row<V>(ahead<FOUR, STAGES, T>() ? place + q * blockDim.x * V : row + q * team * V, t);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[q * V + i] = in ? t[i] : 0.0f;
-        }
-    } else ld_cols<FOUR>(row, team, tid, cols, v);
+        for (int i = 0; i < V; ++i) v[q * V + i] = t[i];
+    }
 }
 
 template <typename T>
 constexpr size_t stage_bytes(int threads) { return (size_t)threads * EPT * (8 + 2 * sizeof(T)); }
 
-template <typename T, bool FOUR, int LANES, int MOST, int STAGES>
+// EACH: every row has a gate of its own, which is asked for a row ahead. (In the other form that costs a shared gate 9 % of the pass;
+// without it a gate a row waits for its gate in every row: 351 us for 32,768 x 2048 where this form takes 297.)
+template <typename T, bool FOUR, int LANES, int MOST, int STAGES, bool EACH>
 __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(const Join a) {
     extern __shared__ __align__(16) char smem[];
     pdl_launch_dependents();
     __shared__ __align__(16) float red[2][32][8];
-    constexpr int L = LANES ? LANES : 1, TEAMS = LANES ? 256 / L : 1;
+    constexpr int L = LANES ? LANES : 1, TEAMS = LANES ? 256 / L : 1, V = FOUR ? 4 : 1;
     const int team = LANES ? LANES : blockDim.x, tid = LANES ? threadIdx.x % L : threadIdx.x, cols = a.cols;
     const int64_t s = (int64_t)blockIdx.x * TEAMS + (LANES ? threadIdx.x / L : 0);   // the strip
     const int64_t r0 = min(s * a.strip, a.rows), r1 = min(r0 + a.strip, a.rows);
-    const int n = (int)(r1 - r0);
+    const int n = (int)(r1 - r0), left = cols - tid * V;   // columns from this thread's first one on
     int turn = 0;
     const float over = 1.0f / (float)cols;
-    const int per = blockDim.x * EPT;   // elements of one matrix in a stage
-    auto place = [&](int i) { return smem + (size_t)(STAGES > 0 ? i % (STAGES > 0 ? STAGES : 1) : 0) * stage_bytes<T>(blockDim.x); };
-    auto ask = [&](int i) {
-        if (i < n) {
-            char* p = place(i);
-            const int64_t at = (r0 + i) * cols;
-            ask_row<FOUR, STAGES>(reinterpret_cast<float*>(p), a.x_out + at, team, tid, cols);
-            if (a.d_out) ask_row<FOUR, STAGES>(reinterpret_cast<float*>(p) + per, a.d_out + at, team, tid, cols);
-            T* t = reinterpret_cast<T*>(p + (size_t)per * 8);
-            ask_row<FOUR, STAGES>(t, static_cast<const T*>(a.y) + at, team, tid, cols);
-            if (a.d_xn) ask_row<FOUR, STAGES>(t + per, static_cast<const T*>(a.d_xn) + at, team, tid, cols);
+    // rows ahead: the next row to ask for, and this thread's places, [x_out, d_out in f32; y, d_xn][columns][thread] a stage
+    const int per = blockDim.x * EPT;
+    const uint32_t stage = (uint32_t)stage_bytes<T>(blockDim.x);
+    int asked = 0, to = 0, from = 0;   // rows asked for; the stages that the next one goes to and the current one comes from
+    int64_t ask_at = r0 * cols + tid * V;
+    char* mine = smem + threadIdx.x * V * 4;
+    const uint32_t mine32 = (uint32_t)__cvta_generic_to_shared(mine);
+    auto half = [&](auto p) { return p - threadIdx.x * V * (4 - sizeof(T)) + (size_t)per * 8; };   // the place of a T column in front of an f32 one's
+    auto ask = [&]() {
+        if (asked < n) {
+            const uint32_t p = mine32 + to * stage;
+            ask_row<FOUR, STAGES>(p, a.x_out + ask_at, team, left);
+            if (a.d_out) ask_row<FOUR, STAGES>(p + per * 4, a.d_out + ask_at, team, left);
+            const uint32_t t = half(p);
+            ask_row<FOUR, STAGES>(t, static_cast<const T*>(a.y) + ask_at, team, left);
+            if (a.d_xn) ask_row<FOUR, STAGES>(t + per * (uint32_t)sizeof(T), static_cast<const T*>(a.d_xn) + ask_at, team, left);
+            ask_at += cols;
         }
+        ++asked;
+        to = to + 1 == STAGES ? 0 : to + 1;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) ask(i);
-    float w_pre[EPT], u[EPT], sw_pre[EPT] = {}, sw_post[EPT] = {}, sum_g[EPT] = {};
-    ld_gain<FOUR>(a.w_pre, team, tid, cols, w_pre);
+    for (int i = 0; i < STAGES - 1; ++i) ask();
+    pair_t w_pre[EPT / 2], u[EPT / 2], sw_pre[EPT / 2] = {}, sum_g[EPT / 2] = {};   // (all-zero bits are two zeros)
+    float sw_post[EPT] = {};
+    {
+        float t[EPT];
+        ld_gain<FOUR>(a.w_pre, team, tid, cols, t);
+#pragma unroll
+        for (int j = 0; j < EPT / 2; ++j) w_pre[j] = pair(t[2 * j], t[2 * j + 1]);
+    }
     int64_t group = r0 / a.gate_rows, first = group * a.gate_rows, end = first + min(a.gate_rows, a.rows - first);
-    auto load_u = [&]() {   // branch gate w_post
+    auto set_u = [&](const float (&gate)[EPT], const float (&w)[EPT]) {   // branch gate w_post
+#pragma unroll
+        for (int j = 0; j < EPT / 2; ++j)
+            u[j] = pair(a.branch * gate[2 * j] * w[2 * j], a.branch * gate[2 * j + 1] * w[2 * j + 1]);
+    };
+    float g[EPT];
+    {
         float w[EPT];
         ld_gain<FOUR>(a.w_post, team, tid, cols, w);
-        ld_gain<FOUR>(a.gate && n > 0 ? a.gate + group * cols : nullptr, team, tid, cols, u);
-#pragma unroll
-        for (int j = 0; j < EPT; ++j) u[j] = a.branch * u[j] * w[j];
-    };
-    load_u();
+        ld_gain<FOUR>(a.gate && n > 0 ? a.gate + group * cols : nullptr, team, tid, cols, g);
+        set_u(g, w);
+    }
     // (teams that share a warp take the same number of turns)
     for (int i = 0; i < (LANES ? (int)a.strip : n); ++i) {
         const bool live = LANES == 0 || i < n;
-        const int64_t r = r0 + i, at = (live ? r : 0) * cols;
+        const int64_t r = r0 + i, at = (live ? r : 0) * cols, mine_at = at + tid * V;
+        float next_g[EPT];
+        if (EACH) ld_gain<FOUR>(a.gate && r + 1 < r1 ? a.gate + (r + 1) * cols : nullptr, team, tid, cols, next_g);
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES > 2 ? STAGES - 2 : 0) : "memory");
-        float y[EPT], xo[EPT], dn[EPT], d[EPT];
+        pair_t y[EPT / 2], xo[EPT / 2], dn[EPT / 2], d[EPT / 2];
         {
-            const char* p = place(i);
-            take_row<FOUR, STAGES>(reinterpret_cast<const float*>(p), a.x_out + at, team, tid, cols, xo);
-            const T* t = reinterpret_cast<const T*>(p + (size_t)per * 8);
-            take_row<FOUR, STAGES>(t, static_cast<const T*>(a.y) + at, team, tid, cols, y);
-            if (a.d_out) take_row<FOUR, STAGES>(reinterpret_cast<const float*>(p) + per, a.d_out + at, team, tid, cols, d);
-            if (a.d_xn) take_row<FOUR, STAGES>(t + per, static_cast<const T*>(a.d_xn) + at, team, tid, cols, dn);
-        }
-        if (STAGES > 0) ask(i + STAGES - 1);   // into the places of the row before
-        float sum[6] = {};
+            const char* p = mine + from * stage;
+            const T* t = reinterpret_cast<const T*>(half(p));
+            auto take = [&](auto place, auto row, pair_t (&v)[EPT / 2]) {
+                float f[EPT];
+                take_row<FOUR, STAGES>(place, row, team, left, f);
 #pragma unroll
-        for (int j = 0; j < EPT; ++j) {
-            if (!a.d_out) d[j] = 0.0f;
-            if (!a.d_xn) dn[j] = 0.0f;
-            const float t = dn[j] * w_pre[j], v = u[j] * y[j];
-            sum[0] = fmaf(y[j], y[j], sum[0]);
-            sum[1] = fmaf(xo[j], xo[j], sum[1]);
-            sum[2] = fmaf(t, xo[j], sum[2]);
-            sum[3] = fmaf(v, d[j], sum[3]);
-            sum[4] = fmaf(v, t, sum[4]);
-            sum[5] = fmaf(v, xo[j], sum[5]);
+                for (int j = 0; j < EPT / 2; ++j) v[j] = pair(f[2 * j], f[2 * j + 1]);
+            };
+            take(reinterpret_cast<const float*>(p), a.x_out + mine_at, xo);
+            take(t, static_cast<const T*>(a.y) + mine_at, y);
+            if (a.d_out) take(reinterpret_cast<const float*>(p) + per, a.d_out + mine_at, d);
+            if (a.d_xn) take(t + per, static_cast<const T*>(a.d_xn) + mine_at, dn);
+            from = from + 1 == STAGES ? 0 : from + 1;
         }
-        team_sum<LANES>(sum, red, turn);
+        if (STAGES > 0) ask();   // into the places of the row before
+        pair_t sum2[6] = {};
+#pragma unroll
+        for (int j = 0; j < EPT / 2; ++j) {
+            if (!a.d_out) d[j] = 0;
+            if (!a.d_xn) dn[j] = 0;
+            const pair_t t = mul2(dn[j], w_pre[j]), v = mul2(u[j], y[j]);
+            sum2[0] = fma2(y[j], y[j], sum2[0]);
+            sum2[1] = fma2(xo[j], xo[j], sum2[1]);
+            sum2[2] = fma2(t, xo[j], sum2[2]);
+            sum2[3] = fma2(v, d[j], sum2[3]);
+            sum2[4] = fma2(v, t, sum2[4]);
+            sum2[5] = fma2(v, xo[j], sum2[5]);
+        }
+        float sum[6];
+#pragma unroll
+        for (int j = 0; j < 6; ++j) {
+            const float2 t = two(sum2[j]);
+            sum[j] = t.x + t.y;
+        }
+        team_sums<LANES>(sum, red, turn);
         // d = d_out + i2 t + c2 x_out; d_y = i1 u d + c1 y
-        const float i2 = 1.0f / sqrtf(sum[1] * over + a.eps), c2 = -i2 * (i2 * (sum[2] * i2 * over));
-        const float i1 = a.post ? 1.0f / sqrtf(sum[0] * over + a.eps) : 1.0f;
+        const float i2 = rsqrtf(sum[1] * over + a.eps), c2 = -i2 * (i2 * (sum[2] * i2 * over));
+        const float i1 = a.post ? rsqrtf(sum[0] * over + a.eps) : 1.0f;
         const float c1 = a.post ? -i1 * (i1 * (i1 * over * (sum[3] + i2 * sum[4] + c2 * sum[5]))) : 0.0f;
-        float dx[EPT];
+        const pair_t I1 = pair(i1), I2 = pair(i2), C1 = pair(c1), C2 = pair(c2);
+        float dx[EPT], dy[EPT];
 #pragma unroll
-        for (int j = 0; j < EPT; ++j) {
-            if (live) sw_pre[j] = fmaf(dn[j] * xo[j], i2, sw_pre[j]);
-            d[j] = fmaf(i2, dn[j] * w_pre[j], fmaf(c2, xo[j], d[j]));
-            dx[j] = a.skip * d[j];
-            if (live) sum_g[j] = fmaf(d[j] * y[j], i1, sum_g[j]);
-            y[j] = fmaf(c1, y[j], i1 * (u[j] * d[j]));
+        for (int j = 0; j < EPT / 2; ++j) {
+            if (live) sw_pre[j] = fma2(mul2(dn[j], xo[j]), I2, sw_pre[j]);
+            d[j] = fma2(I2, mul2(dn[j], w_pre[j]), fma2(C2, xo[j], d[j]));
+            if (live) sum_g[j] = fma2(mul2(d[j], y[j]), I1, sum_g[j]);
+            const float2 x2 = two(mul2(pair(a.skip), d[j])), y2 = two(fma2(C1, y[j], mul2(I1, mul2(u[j], d[j]))));
+            dx[2 * j] = x2.x; dx[2 * j + 1] = x2.y;
+            dy[2 * j] = y2.x; dy[2 * j + 1] = y2.y;
         }
         if (!live) continue;
         st_cols<FOUR>(a.d_x + at, team, tid, cols, dx);
-        st_cols<FOUR>(static_cast<T*>(a.d_y) + at, team, tid, cols, y);
-        if (r + 1 == end || r + 1 == r1) {   // the last row of the gate's group, or of the strip
-            float w[EPT];
-            if (a.d_w_post) {
-                ld_gain<FOUR>(a.gate ? a.gate + group * cols : nullptr, team, tid, cols, w);
+        st_cols<FOUR>(static_cast<T*>(a.d_y) + at, team, tid, cols, dy);
+        if (EACH || r + 1 == end || r + 1 == r1) {   // the last row of the gate's group, or of the strip
+            float w[EPT], sg[EPT];
+            if (!EACH) ld_gain<FOUR>(a.gate ? a.gate + group * cols : nullptr, team, tid, cols, g);
+            ld_gain<FOUR>(a.w_post, team, tid, cols, w);
 #pragma unroll
-                for (int j = 0; j < EPT; ++j) sw_post[j] = fmaf(a.branch * w[j], sum_g[j], sw_post[j]);
+            for (int j = 0; j < EPT / 2; ++j) {
+                const float2 t = two(sum_g[j]);
+                sg[2 * j] = a.branch * t.x; sg[2 * j + 1] = a.branch * t.y;
+                sum_g[j] = 0;
+            }
+#pragma unroll
+            for (int j = 0; j < EPT; ++j) {
+                sw_post[j] = fmaf(g[j], sg[j], sw_post[j]);
+                sg[j] *= w[j];
             }
             if (a.d_gate) {
-                ld_gain<FOUR>(a.w_post, team, tid, cols, w);
-#pragma unroll
-                for (int j = 0; j < EPT; ++j) w[j] *= a.branch * sum_g[j];
-                if (first >= r0 && end <= r1) put_sum<FOUR>(a.d_gate + group * cols, team, tid, cols, w, a.accumulate);
-                else st_cols<FOUR>(a.part_g + (2 * s + (first < r0 ? 0 : 1)) * cols, team, tid, cols, w);
+                if (EACH) put_sum<FOUR>(a.d_gate + at, team, tid, cols, sg, a.accumulate);
+                else if (first >= r0 && end <= r1) put_sum<FOUR>(a.d_gate + group * cols, team, tid, cols, sg, a.accumulate);
+                else st_cols<FOUR>(a.part_g + (2 * s + (first < r0 ? 0 : 1)) * cols, team, tid, cols, sg);
             }
+            if (EACH) {
+                set_u(next_g, w);
 #pragma unroll
-            for (int j = 0; j < EPT; ++j) sum_g[j] = 0.0f;
-            if (r + 1 < r1) {
+                for (int j = 0; j < EPT; ++j) g[j] = next_g[j];
+            } else if (r + 1 < r1) {
                 ++group;
                 first = end;
                 end = first + min(a.gate_rows, a.rows - first);
-                if (a.gate) load_u();
+                if (a.gate) {
+                    ld_cols<FOUR>(a.gate + group * cols, team, tid, cols, g, 1.0f);
+                    set_u(g, w);
+                }
             }
         }
+    }
+    float sums_pre[EPT];
+#pragma unroll
+    for (int j = 0; j < EPT / 2; ++j) {
+        const float2 t = two(sw_pre[j]);
+        sums_pre[2 * j] = t.x; sums_pre[2 * j + 1] = t.y;
     }
     // the CTA's sums of the gains
 #pragma unroll
@@ -332,7 +437,7 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
             constexpr int WIDE = L * EPT;
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < EPT; ++j) part[threadIdx.x / L * WIDE + col_of<FOUR>(j, team, tid)] = which == 0 ? sw_pre[j] : sw_post[j];
+            for (int j = 0; j < EPT; ++j) part[threadIdx.x / L * WIDE + col_of<FOUR>(j, team, tid)] = which == 0 ? sums_pre[j] : sw_post[j];
             __syncthreads();
             for (int c = threadIdx.x; c < cols; c += 256) {
                 float v = 0.0f;
@@ -340,17 +445,19 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
                 for (int i = 0; i < TEAMS; ++i) v += part[i * WIDE + c];
                 out[c] = v;
             }
-        } else if (which == 0) st_cols<FOUR>(out, team, tid, cols, sw_pre);
+        } else if (which == 0) st_cols<FOUR>(out, team, tid, cols, sums_pre);
         else st_cols<FOUR>(out, team, tid, cols, sw_post);
     }
 }
 
 // Adds what the strips left: blockIdx.y = 0, 1 the gains over all CTAs; behind them a gate's groups that reach over several strips.
-// 32 columns a block, blockDim.y lanes a column, each every blockDim.y-th part.
+// A block owns eight columns (a 32-byte sector of every part), 128 lanes a column, each every 128th part.
+constexpr int SUM_COLS = 8;
 __global__ void __launch_bounds__(1024) join_sums_kernel(const Join a, int ctas) {
-    __shared__ float sh[32][33];
+    __shared__ float sh[32][SUM_COLS];
     pdl_wait();
-    const int c = blockIdx.x * 32 + threadIdx.x, y = threadIdx.y, cols = a.cols;
+    const int c = blockIdx.x * SUM_COLS + threadIdx.x % SUM_COLS, y = threadIdx.x / SUM_COLS, w = threadIdx.x >> 5, lane = threadIdx.x & 31, cols = a.cols;
+    constexpr int LANES = 1024 / SUM_COLS;
     float* out;
     float v = 0.0f;
     if (blockIdx.y < 2) {
@@ -358,7 +465,7 @@ __global__ void __launch_bounds__(1024) join_sums_kernel(const Join a, int ctas)
         if (!out) return;
         if (c < cols) {
 #pragma unroll 8
-            for (int i = y; i < ctas; i += blockDim.y) v += a.part_w[(2 * (int64_t)i + blockIdx.y) * cols + c];
+            for (int i = y; i < ctas; i += LANES) v += a.part_w[(2 * (int64_t)i + blockIdx.y) * cols + c];
         }
     } else {
         const int64_t group = blockIdx.y - 2, first = group * a.gate_rows, end = min(first + a.gate_rows, a.rows);
@@ -366,18 +473,23 @@ __global__ void __launch_bounds__(1024) join_sums_kernel(const Join a, int ctas)
         if (s0 == s1) return;   // (written by the strip)
         out = a.d_gate + group * cols;
         if (c < cols) {
-            // a group that begins where its first strip does is that strip's sum to the right as well
+            // the group begins in its first strip, whose sum goes to the right, and comes into the others from the left
+            if (y == 0) v = a.part_g[(2 * s0 + 1) * cols + c];
 #pragma unroll 8
-            for (int64_t i = s0 + y; i <= s1; i += blockDim.y) v += a.part_g[(2 * i + (i == s0 ? 1 : 0)) * cols + c];
+            for (int64_t i = s0 + 1 + y; i <= s1; i += LANES) v += a.part_g[2 * i * cols + c];
         }
     }
-    sh[y][threadIdx.x] = v;
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    v += __shfl_xor_sync(0xffffffffu, v, 16);
+    if (lane < SUM_COLS) sh[w][lane] = v;
     __syncthreads();
-    if (y == 0 && c < cols) {
-        float t = 0.0f;
-        for (int i = 0; i < (int)blockDim.y; ++i) t += sh[i][threadIdx.x];
-        out[c] = a.accumulate ? out[c] + t : t;
-    }
+    if (w > 0) return;
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += sh[lane / SUM_COLS * 8 + i][lane % SUM_COLS];
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    v += __shfl_xor_sync(0xffffffffu, v, 16);
+    if (lane < SUM_COLS && c < cols) out[c] = a.accumulate ? out[c] + v : v;
 }
 
 // Lanes of a warp that make a team (0: a team is a CTA), and the team's threads.
@@ -447,7 +559,8 @@ struct Bwd {
     static cudaError_t go(dim3 grid, int threads, cudaStream_t s, const Join& a) {
         // three rows' places fit twice into an SM up to 256 threads and once up to 512; above that two of bf16, none of f32
         constexpr int STAGES = MOST <= 512 ? 3 : sizeof(T) == 2 ? 2 : 0;
-        auto kern = join_bwd_kernel<T, FOUR, LANES, MOST, STAGES>;
+        constexpr bool EACH = MOST <= 512;   // (a team of more has no registers for a second gate)
+        auto kern = EACH && a.gate && a.gate_rows == 1 ? join_bwd_kernel<T, FOUR, LANES, MOST, STAGES, EACH> : join_bwd_kernel<T, FOUR, LANES, MOST, STAGES, false>;
         const size_t smem = STAGES * stage_bytes<T>(threads);
         const cudaError_t e = smem > 40 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
         if (e == cudaSuccess) kern<<<grid, threads, smem, s>>>(a);
@@ -515,9 +628,8 @@ int asca_gated_residual_rmsnorm_bwd(asca_ctx* ctx, const void* y, const float* x
     ASCA_TRY(launch<Bwd>(ctx, a, dtype, four, s.strips));
     const bool gates = d_gate && a.gate_rows > s.strip;   // (else every group lies in one strip)
     if (d_w_post || d_w_pre || gates) {
-        const int64_t groups = gates ? ceil_div64(rows, a.gate_rows) : 0, most = std::max(s.ctas, gates ? a.gate_rows / s.strip : 0);
-        const dim3 block(32, most >= 64 ? 32 : 8);
-        ASCA_CUDA(ctx, asca_launch_after(ctx, join_sums_kernel, dim3((unsigned)ceil_div64(cols, 32), (unsigned)(2 + groups)), block, 0, a, (int)s.ctas));
+        const int64_t groups = gates ? ceil_div64(rows, a.gate_rows) : 0;
+        ASCA_CUDA(ctx, asca_launch_after(ctx, join_sums_kernel, dim3((unsigned)ceil_div64(cols, SUM_COLS), (unsigned)(2 + groups)), dim3(1024), 0, a, (int)s.ctas));
         ctx->launches++;
     }
     return ASCA_OK;
