@@ -16,22 +16,22 @@
 
 namespace {
 
-// A thread has its columns of TOKENS rows in flight.
+// LANES lanes own TOKENS tokens, all of whose rows they have in flight; where that leaves SMs without work, blocks beside each other
+// (blockIdx.y) share the columns.
 constexpr int TOKENS = 4;
-template <int W, typename TT, typename TX>
+template <int W, int LANES, typename TT, typename TX>
 __global__ void __launch_bounds__(256) embed_scaled_fwd_kernel(const TT* __restrict__ table, const uint32_t* __restrict__ ids, int64_t N, int d,
                                                                uint32_t vocab, float scale, TX* __restrict__ x) {
     using F = frag<W, TT>;
-    const int lanes = blockDim.x;
-    const int64_t r0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * TOKENS;
+    const int64_t r0 = ((int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES) * TOKENS;
     uint32_t id[TOKENS];
 #pragma unroll
     for (int i = 0; i < TOKENS; ++i) id[i] = r0 + i < N ? ids[r0 + i] : 0xffffffffu;
-    for (int c = frag_first<W>(threadIdx.x); c < d; c += lanes * F::E) {
+    for (int c = blockIdx.y * LANES * F::E + frag_first<W>(threadIdx.x % LANES); c < d; c += gridDim.y * LANES * F::E) {
         F r[TOKENS];
 #pragma unroll
         for (int i = 0; i < TOKENS; ++i)
-            if (id[i] < vocab) r[i].load(table + (int64_t)id[i] * d, c, lanes, d);
+            if (id[i] < vocab) r[i].load(table + (int64_t)id[i] * d, c, LANES, d);
 #pragma unroll
         for (int i = 0; i < TOKENS; ++i) {
             if (r0 + i >= N) break;
@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(256) embed_scaled_fwd_kernel(const TT* __restr
 #pragma unroll
                 for (int j = 0; j < F::E; ++j) v[j] *= scale;
             }
-            frag<W, TX>::put(x + (r0 + i) * d, c, lanes, d, v);
+            frag<W, TX>::put(x + (r0 + i) * d, c, LANES, d, v);
         }
     }
 }
@@ -249,6 +249,7 @@ __global__ void __launch_bounds__(1024) embed_small_kernel(const Sum a, const st
         for (int i = 0; i < stable_sort::PER; ++i) {
             const int at = lo + i * 32;
             t.item[i] = -1;
+            t.key[i] = 0;
             if (i < per && at < n) {
                 t.key[i] = pass == 0 ? min(j.ids[at], j.limit) : keys[now][at];
                 t.item[i] = pass == 0 ? at : items[now][at];
@@ -313,11 +314,16 @@ __global__ void __launch_bounds__(1024) embed_small_kernel(const Sum a, const st
 #pragma unroll
         for (int e = 0; e < E; ++e) part[threadIdx.x * E + e] = acc[e];
         __syncthreads();
-        if (y == 0 && in) {
-            for (int i = 1; i < beside; ++i) {
+        for (int s = beside / 2; s > 0; s /= 2) {
+            if (y < s) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] += part[(i * lanes + x) * E + e];
+                for (int e = 0; e < E; ++e) part[threadIdx.x * E + e] += part[(threadIdx.x + s * lanes) * E + e];
             }
+            __syncthreads();
+        }
+        if (y == 0 && in) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = part[x * E + e];
             add_row<W>(a.d_table + (int64_t)v * d, c, lanes, d, acc, a.scale, a.accumulate);
         }
         __syncthreads();
@@ -348,7 +354,7 @@ struct Plan {
         counts = stable_sort::scratch_bytes(N, bins);
         part = (size_t)ceil_div64(N, piece) * 2 * d * 4;
     }
-    size_t bytes() const { return 4 * list + counts + part + 256; }
+    size_t bytes() const { return 4 * list + counts + part; }
 };
 
 }  // namespace
@@ -365,13 +371,17 @@ int asca_embed_scaled_fwd(asca_ctx* ctx, const void* table, const uint32_t* ids,
     ASCA_REQUIRE(ctx, N < ((int64_t)1 << 31), "embed_scaled_fwd: at most 2^31 - 1 tokens");
     asca_device_scope on(ctx);
     const int v = asca_row_width(d, table, table_dtype, x, out_dtype);
-    const dim3 block = asca_row_block(asca_row_frags(d, v), 256), grid((unsigned)ceil_div64(N, (int64_t)block.y * TOKENS));
+    const int64_t frags = asca_row_frags(d, v);
     asca_with_dtype(table, table_dtype, [&](auto tab) {
         asca_with_dtype(x, out_dtype, [&](auto out) {
             using TT = std::remove_const_t<std::remove_pointer_t<decltype(tab)>>;
             using TX = std::remove_pointer_t<decltype(out)>;
             asca_with_width<TT, TX>(v, [&](auto w) {
-                embed_scaled_fwd_kernel<w(), TT, TX><<<grid, block, 0, ctx->stream>>>(tab, ids, N, (int)d, (uint32_t)vocab, scale, out);
+                asca_with_lanes(frags, [&](auto l) {
+                    const int64_t blocks = ceil_div64(N, 256 / l() * TOKENS);
+                    const dim3 grid((unsigned)blocks, asca_column_blocks(ctx, blocks, frags, l()));
+                    embed_scaled_fwd_kernel<w(), l(), TT, TX><<<grid, 256, 0, ctx->stream>>>(tab, ids, N, (int)d, (uint32_t)vocab, scale, out);
+                });
             });
         });
     });
@@ -396,9 +406,9 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
         if (!accumulate) ASCA_CUDA(ctx, cudaMemsetAsync(d_table, 0, (size_t)vocab * d * 4, ctx->stream));
         return ASCA_OK;
     }
-    ASCA_REQUIRE(ctx, dx && ids && ws, "embed_scaled_bwd: null pointer");
+    ASCA_REQUIRE(ctx, dx && ids, "embed_scaled_bwd: null pointer");
     const Plan plan(N, d, vocab);
-    ASCA_REQUIRE(ctx, asca_aligned(ws, 256) && ws_bytes >= plan.bytes(), "embed_scaled_bwd: the workspace has to have asca_embed_scaled_bwd_ws bytes, 256-byte aligned");
+    ASCA_REQUIRE(ctx, asca_aligned(ws, 256) && ws_bytes >= plan.bytes() && (ws || ws_bytes == 0), "embed_scaled_bwd: the workspace has to have asca_embed_scaled_bwd_ws bytes, 256-byte aligned");
     const int v = asca_row_width(d, dx, dtype, d_table, ASCA_F32);
     const int64_t frags = asca_row_frags(d, v);
     dim3 block = asca_row_block(frags, 128);

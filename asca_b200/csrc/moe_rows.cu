@@ -51,14 +51,14 @@ __global__ void __launch_bounds__(256) sort_rows_kernel(const TX* __restrict__ x
 // unsort and its gradient: LANES lanes own PAIRS / KS tokens, KS assignments of each at a time: PAIRS rows of the sorted side in flight.
 constexpr int PAIRS = 4;
 
-// weights null: every weight is one
+// weights null: every weight is one. Few tokens: blocks beside each other (blockIdx.y) share the columns.
 template <int W, int LANES, int KS, typename TS, typename TX>
 __global__ void __launch_bounds__(256) unsort_rows_kernel(const TS* __restrict__ ys, const int32_t* __restrict__ slot, const float* __restrict__ weights,
                                                           int64_t N, int K, int d, TX* __restrict__ out) {
     using F = frag<W, TS>;
     constexpr int T = PAIRS / KS;
     const int64_t t0 = ((int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES) * T;
-    for (int c = frag_first<W>(threadIdx.x % LANES); c < d; c += LANES * F::E) {
+    for (int c = blockIdx.y * LANES * F::E + frag_first<W>(threadIdx.x % LANES); c < d; c += gridDim.y * LANES * F::E) {
         float acc[T][F::E] = {};
         for (int k0 = 0; k0 < K; k0 += KS) {
             F r[T][KS];
@@ -152,23 +152,16 @@ __global__ void __launch_bounds__(256) unsort_rows_bwd_kernel(const TX* __restri
     }
 }
 
-// The lanes that own a token and the assignments they take at a time, as constants; the blocks of N tokens.
-struct Team {
-    int lanes, ks;
-    Team(int64_t frags, int64_t K) : lanes(frags <= 8 ? 8 : frags <= 16 ? 16 : 32), ks(K == 1 ? 1 : K <= 3 ? 2 : 4) {}
-    unsigned blocks(int64_t N) const { return (unsigned)ceil_div64(N, (256 / lanes) * (PAIRS / ks)); }
-    template <typename F>
-    void with(F f) const {
-        auto k = [&](auto l) {
-            if (ks == 1) f(l, std::integral_constant<int, 1>());
-            else if (ks == 2) f(l, std::integral_constant<int, 2>());
-            else f(l, std::integral_constant<int, 4>());
-        };
-        if (lanes == 8) k(std::integral_constant<int, 8>());
-        else if (lanes == 16) k(std::integral_constant<int, 16>());
-        else k(std::integral_constant<int, 32>());
-    }
-};
+// f(lanes that own a token, assignments they take at a time, blocks of N tokens)
+template <typename F>
+inline void with_team(int64_t frags, int64_t N, int64_t K, F f) {
+    asca_with_lanes(frags, [&](auto l) {
+        auto go = [&](auto ks) { f(l, ks, ceil_div64(N, 256 / l() * (PAIRS / ks()))); };
+        if (K == 1) go(std::integral_constant<int, 1>());
+        else if (K <= 3) go(std::integral_constant<int, 2>());
+        else go(std::integral_constant<int, 4>());
+    });
+}
 
 int check_rows(asca_ctx* ctx, const char* who, int64_t N, int64_t K, int64_t d, int tok_dtype, int row_dtype) {
     ASCA_REQUIRE(ctx, N >= 0 && K > 0 && d > 0 && d < (1 << 30) && K < (1 << 16) && N < ((int64_t)1 << 31) / K, "%s: bad shape (N * K must fit int32)", who);
@@ -182,7 +175,7 @@ extern "C" {
 
 int64_t asca_moe_topk_dispatch_ws(int64_t N, int64_t K, int64_t E) {
     if (N < 0 || K <= 0 || E <= 0 || E + 1 > stable_sort::MAX_BINS) return ASCA_ERR_ARG;
-    return (int64_t)stable_sort::scratch_bytes(N * K, (int)E + 1) + 256;
+    return (int64_t)stable_sort::scratch_bytes(N * K, (int)E + 1);   // (few assignments: none)
 }
 
 int asca_moe_topk_dispatch(asca_ctx* ctx, const int32_t* experts, int64_t N, int64_t K, int64_t E, int32_t* perm, int32_t* offsets, int32_t* slot,
@@ -196,8 +189,8 @@ int asca_moe_topk_dispatch(asca_ctx* ctx, const int32_t* experts, int64_t N, int
         ASCA_CUDA(ctx, cudaMemsetAsync(offsets, 0, (size_t)(E + 1) * 4, ctx->stream));
         return ASCA_OK;
     }
-    ASCA_REQUIRE(ctx, experts && perm && slot && ws, "moe_topk_dispatch: null pointer");
-    ASCA_REQUIRE(ctx, asca_aligned(ws, 256) && ws_bytes >= (size_t)asca_moe_topk_dispatch_ws(N, K, E),
+    ASCA_REQUIRE(ctx, experts && perm && slot, "moe_topk_dispatch: null pointer");
+    ASCA_REQUIRE(ctx, asca_aligned(ws, 256) && ws_bytes >= (size_t)asca_moe_topk_dispatch_ws(N, K, E) && (ws || ws_bytes == 0),
                  "moe_topk_dispatch: the workspace has to have asca_moe_topk_dispatch_ws bytes, 256-byte aligned");
     stable_sort::Job j{};
     j.ids = (const uint32_t*)experts;
@@ -238,14 +231,15 @@ int asca_moe_unsort_rows(asca_ctx* ctx, const void* ys, const int32_t* slot, con
     ASCA_REQUIRE(ctx, ys && slot && out, "moe_unsort_rows: null pointer");
     asca_device_scope on(ctx);
     const int v = asca_row_width(d, ys, ys_dtype, out, out_dtype);
-    const Team team(asca_row_frags(d, v), K);
+    const int64_t frags = asca_row_frags(d, v);
     asca_with_dtype(ys, ys_dtype, [&](auto a) {
         asca_with_dtype(out, out_dtype, [&](auto b) {
             using TS = std::remove_const_t<std::remove_pointer_t<decltype(a)>>;
             using TX = std::remove_pointer_t<decltype(b)>;
             asca_with_width<TX, TS>(v, [&](auto w) {
-                team.with([&](auto l, auto ks) {
-                    unsort_rows_kernel<w(), l(), ks(), TS, TX><<<team.blocks(N), 256, 0, ctx->stream>>>(a, slot, weights, N, (int)K, (int)d, b);
+                with_team(frags, N, K, [&](auto l, auto ks, int64_t blocks) {
+                    const dim3 grid((unsigned)blocks, asca_column_blocks(ctx, blocks, frags, l()));
+                    unsort_rows_kernel<w(), l(), ks(), TS, TX><<<grid, 256, 0, ctx->stream>>>(a, slot, weights, N, (int)K, (int)d, b);
                 });
             });
         });
@@ -267,15 +261,15 @@ int asca_moe_unsort_rows_bwd(asca_ctx* ctx, const void* d_out, const void* ys, c
     ASCA_REQUIRE(ctx, !d_w || ys, "moe_unsort_rows_bwd: the weights' gradient needs ys");
     asca_device_scope on(ctx);
     const int v = std::min(asca_row_width(d, d_out, out_dtype, ys, ys_dtype), asca_row_width(d, d_out, out_dtype, d_ys, ys_dtype));
-    const Team team(asca_row_frags(d, v), K);
+    const int64_t frags = asca_row_frags(d, v);
     asca_with_dtype(d_out, out_dtype, [&](auto a) {
         asca_with_dtype(d_ys, ys_dtype, [&](auto b) {
             using TX = std::remove_const_t<std::remove_pointer_t<decltype(a)>>;
             using TS = std::remove_pointer_t<decltype(b)>;
             asca_with_width<TX, TS>(v, [&](auto w) {
-                team.with([&](auto l, auto ks) {
-                    unsort_rows_bwd_kernel<w(), l(), ks(), TX, TS><<<team.blocks(N), 256, 0, ctx->stream>>>(a, static_cast<const TS*>(ys), slot, weights, N,
-                                                                                                           (int)K, (int)d, b, d_w);
+                with_team(frags, N, K, [&](auto l, auto ks, int64_t blocks) {
+                    unsort_rows_bwd_kernel<w(), l(), ks(), TX, TS><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a, static_cast<const TS*>(ys), slot, weights, N,
+                                                                                                              (int)K, (int)d, b, d_w);
                 });
             });
         });

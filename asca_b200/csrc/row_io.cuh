@@ -54,6 +54,17 @@ inline dim3 asca_row_block(int64_t frags, int threads) {
     return dim3(tx, threads / tx);
 }
 #endif
+// f(std::integral_constant of 8, 16 or 32): the lanes of a warp that a row of `frags` groups of columns gets
+template <typename F>
+inline void asca_with_lanes(int64_t frags, F f) {
+    if (frags <= 8) f(std::integral_constant<int, 8>());
+    else if (frags <= 16) f(std::integral_constant<int, 16>());
+    else f(std::integral_constant<int, 32>());
+}
+// Blocks that share a row's columns, where `blocks` alone leave SMs without work.
+inline unsigned asca_column_blocks(const asca_ctx* ctx, int64_t blocks, int64_t frags, int lanes) {
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div64(frags, lanes), ctx->sm_count / std::max<int64_t>(blocks, 1)));
+}
 template <typename A, typename B, typename F>
 inline void asca_with_width(int v, F f) {
     if constexpr (sizeof(A) == 2 || sizeof(B) == 2)

@@ -3,8 +3,9 @@
 // Up to 4,096 items: one CTA does all passes in one launch. More: two launches a pass, a CTA to a tile of 2,048 items -- the first
 // counts the tile's digits, the second adds up what the tiles in front of its own counted and places its items; where that table has
 // more than 65,536 entries, a launch between the two scans it once instead of every CTA for itself.
-// In both, a warp owns a run of consecutive items; match_any gives a lane its rank among equal digits of its 32, a counter per warp
-// and digit what came before them in the run, a scan over the warps what came before the warp. The rank is by construction the order
+// In both, a warp owns a run of consecutive items; a ballot for every bit of the digit gives a lane its rank among equal digits of its 32
+// (match_any, which goes over the distinct digits one by one, takes longer where they are many), a counter per warp and digit what
+// came before them in the run, a scan over the warps what came before the warp. The rank is by construction the order
 // of the items, so the result is the same in every run. Bound by launches and the latency of a pass's steps, not by bytes.
 #pragma once
 #include "common.cuh"
@@ -36,7 +37,10 @@ inline size_t scratch_bytes(int64_t n, int bins) { return n <= SMALL ? 0 : ((siz
 
 #ifdef __CUDACC__
 __device__ __forceinline__ uint32_t mask_of(const Job& j) { return j.passes > 1 ? (1u << j.digit) - 1 : 0xffffffffu; }
-__device__ __forceinline__ uint32_t key_of(const Job& j, int pass, int64_t i) { return pass == 0 ? min(j.ids[i], j.limit) : j.keys[(pass & 1) ^ 1][i]; }
+// (no indexing by a variable: the arguments stay where they are)
+__device__ __forceinline__ uint32_t* keys_to(const Job& j, int pass) { return pass & 1 ? j.keys[1] : j.keys[0]; }
+__device__ __forceinline__ int32_t* items_to(const Job& j, int pass) { return pass & 1 ? j.items[1] : j.items[0]; }
+__device__ __forceinline__ uint32_t key_of(const Job& j, int pass, int64_t i) { return pass == 0 ? min(j.ids[i], j.limit) : keys_to(j, pass + 1)[i]; }
 
 // A CTA's scan of one value a thread; `total` in every thread.
 template <int THREADS>
@@ -74,9 +78,10 @@ __device__ __forceinline__ void load_items(const Job& j, int pass, int64_t lo, i
     for (int i = 0; i < PER; ++i) {
         const int64_t at = lo + i * 32 + lane;
         t.item[i] = -1;
+        t.key[i] = 0;
         if (i < per && at < j.n) {
             t.key[i] = key_of(j, pass, at);
-            t.item[i] = pass == 0 ? (int32_t)at : j.items[(pass & 1) ^ 1][at];
+            t.item[i] = pass == 0 ? (int32_t)at : items_to(j, pass + 1)[at];
         }
     }
 }
@@ -84,18 +89,30 @@ __device__ __forceinline__ void rank_items(int bins, int shift, uint32_t mask, u
     const int lane = threadIdx.x & 31;
     for (int b = lane; b < bins; b += 32) run[b] = 0;
     __syncwarp();
+    const int bits = 32 - __clz(bins - 1);   // of a digit (one bin: none)
+    unsigned peers[PER];
+    int b[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const bool live = t.item[i] >= 0;
-        const unsigned act = __ballot_sync(0xffffffffu, live);
-        if (live) {
-            const int b = (int)((t.key[i] >> shift) & mask);
-            const unsigned peers = __match_any_sync(act, b);
-            const int before = __popc(peers & ((1u << lane) - 1u)), had = run[b];
-            t.rank[i] = had + before;
-            __syncwarp(act);
-            if (before == 0) run[b] = (uint16_t)(had + __popc(peers));   // one leader per distinct digit
+        b[i] = (int)((t.key[i] >> shift) & mask);
+        peers[i] = __ballot_sync(0xffffffffu, t.item[i] >= 0);
+    }
+    for (int k = 0; k < bits; ++k) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const bool set = b[i] >> k & 1;
+            const unsigned m = __ballot_sync(0xffffffffu, set);
+            peers[i] &= set ? m : ~m;
         }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int before = __popc(peers[i] & ((1u << lane) - 1u));
+        int had = 0;
+        if (t.item[i] >= 0) had = run[b[i]];
+        t.rank[i] = had + before;
+        __syncwarp();
+        if (t.item[i] >= 0 && before == 0) run[b[i]] = (uint16_t)(had + __popc(peers[i]));   // one leader per distinct digit
         __syncwarp();
     }
 }
@@ -147,8 +164,8 @@ __device__ __forceinline__ void rank_cta(int bins, int shift, uint32_t mask, uin
 __device__ __forceinline__ void put_items(const Job& j, int pass, const Items& t, const int32_t* base, const uint16_t* run) {
     const int shift = pass * j.digit;
     const uint32_t mask = mask_of(j);
-    uint32_t* keys = j.keys[pass & 1];
-    int32_t* items = j.items[pass & 1];
+    uint32_t* keys = keys_to(j, pass);
+    int32_t* items = items_to(j, pass);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         if (t.item[i] < 0) continue;

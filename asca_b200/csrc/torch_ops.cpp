@@ -96,7 +96,12 @@ struct Call {
     }
     T make(at::IntArrayRef shape, at::ScalarType type) const { return T(at::detail::empty_cuda(shape, type, at::Device(at::kCUDA, (c10::DeviceIndex)device), c10::nullopt)); }
     // scratch (negative: sizes that the entry point will refuse)
-    T scratch(int64_t bytes) const { return make({bytes > 0 ? bytes : 0}, at::kByte); }
+    struct Scratch {
+        T t;
+        void* p() const { return t.defined() ? t.data_ptr() : nullptr; }
+        size_t n() const { return t.defined() ? (size_t)t.numel() : 0; }
+    };
+    Scratch scratch(int64_t bytes) const { return {bytes > 0 ? make({bytes}, at::kByte) : T()}; }
     void ok(int rc) const {
         if (rc == ASCA_OK) return;
         PyObject* m = PyImport_ImportModule("asca_b200");
@@ -204,8 +209,8 @@ PyObject* embed_bwd(Call& c) {   // dx, ids, vocab, scale, d_table, accumulate
     const bool accumulate = c.truth();
     if (accumulate && fresh) raise(PyExc_ValueError, "embed_bwd: accumulate needs the d_table to add to");
     const int64_t bytes = asca_embed_scaled_bwd_ws(n, d, vocab);
-    const T ws = c.scratch(bytes);
-    c.ok(asca_embed_scaled_bwd(c.ctx, dx.data_ptr(), id, n, d, vocab, scale, type, accumulate, ptr<float>(&d_table), ws.data_ptr(), (size_t)ws.numel()));
+    const auto ws = c.scratch(bytes);
+    c.ok(asca_embed_scaled_bwd(c.ctx, dx.data_ptr(), id, n, d, vocab, scale, type, accumulate, ptr<float>(&d_table), ws.p(), ws.n()));
     return wrap(d_table);
 }
 
@@ -282,11 +287,11 @@ PyObject* join_bwd(Call& c) {   // y, x_out, d_xn, d_out, (join), grads
         contiguous(sums[i], names[i]);
     }
     const T d_x = c.make({a.rows, a.cols}, F32), d_y = c.make({a.rows, a.cols}, y.scalar_type());
-    const T ws = c.scratch(asca_gated_residual_rmsnorm_bwd_ws(c.ctx, a.rows, a.cols));
+    const auto ws = c.scratch(asca_gated_residual_rmsnorm_bwd_ws(c.ctx, a.rows, a.cols));
     auto sum = [&](int i) { return of[i] ? ptr<float>(&sums[i]) : nullptr; };
     c.ok(asca_gated_residual_rmsnorm_bwd(c.ctx, y.data_ptr(), ptr<float>(&x_out), ptr<void>(d_xn), ptr<float>(d_out), ptr<float>(a.w_post), ptr<float>(a.gate),
                                          a.gate_rows, ptr<float>(a.w_pre), a.post, a.skip, a.branch, a.eps, a.rows, a.cols, a.type, grads != Py_None,
-                                         ptr<float>(&d_x), d_y.data_ptr(), sum(0), sum(1), sum(2), ws.data_ptr(), (size_t)ws.numel()));
+                                         ptr<float>(&d_x), d_y.data_ptr(), sum(0), sum(1), sum(2), ws.p(), ws.n()));
     PyObject* d = PyDict_New();
     if (!d) throw Raised{};
     auto put = [&](const char* name, const T& t) {
@@ -309,9 +314,8 @@ PyObject* moe_dispatch(Call& c) {   // experts, E
     contiguous(experts, "experts");
     const int64_t e = c.integer(), n = experts.size(0), k = experts.size(1);
     const T perm = c.make({n * k}, I32), offsets = c.make({e >= 0 ? e + 1 : 1}, I32), slot = c.make({n, k}, I32);
-    const T ws = c.scratch(asca_moe_topk_dispatch_ws(n, k, e));
-    c.ok(asca_moe_topk_dispatch(c.ctx, ptr<int32_t>(&experts), n, k, e, ptr<int32_t>(&perm), ptr<int32_t>(&offsets), ptr<int32_t>(&slot), ws.data_ptr(),
-                                (size_t)ws.numel()));
+    const auto ws = c.scratch(asca_moe_topk_dispatch_ws(n, k, e));
+    c.ok(asca_moe_topk_dispatch(c.ctx, ptr<int32_t>(&experts), n, k, e, ptr<int32_t>(&perm), ptr<int32_t>(&offsets), ptr<int32_t>(&slot), ws.p(), ws.n()));
     return tuple({wrap(perm), wrap(offsets), wrap(slot)});
 }
 
@@ -405,8 +409,8 @@ struct List {
 PyObject* grad_norm(Call& c) {   // grads, out
     const List l(c);
     const T out = output(c, "out", F32, {1});
-    const T ws = c.scratch(asca_grad_norm_ws(c.ctx, l.count()));
-    c.ok(asca_grad_norm(c.ctx, l.p.data(), l.n.data(), l.dtype.data(), l.count(), ptr<float>(&out), ws.data_ptr(), (size_t)ws.numel()));
+    const auto ws = c.scratch(asca_grad_norm_ws(c.ctx, l.count()));
+    c.ok(asca_grad_norm(c.ctx, l.p.data(), l.n.data(), l.dtype.data(), l.count(), ptr<float>(&out), ws.p(), ws.n()));
     return wrap(out);
 }
 

@@ -348,8 +348,8 @@ int asca_moe_step(asca_ctx* ctx, const float* x, const uint32_t* ids, const void
  *   perm    (N*K) the assignments by expert, ascending inside one; those that go nowhere behind them
  *   offsets (E+1) the experts' bounds in perm -- what asca_moe_fwd takes; offsets[E] = assignments that go somewhere
  *   slot    (N, K) the inverse: where assignment a lies in perm, -1 if it goes nowhere
- * Integer only. At most 2048 experts. ws: asca_moe_topk_dispatch_ws bytes of device scratch, 256-byte aligned, the caller's
- * until the call's work has run. */
+ * Integer only. At most 2048 experts. ws: asca_moe_topk_dispatch_ws bytes of device scratch (0 for few assignments: ws may be
+ * NULL then), 256-byte aligned, the caller's until the call's work has run. */
 int64_t asca_moe_topk_dispatch_ws(int64_t N, int64_t K, int64_t E);
 int asca_moe_topk_dispatch(asca_ctx* ctx, const int32_t* experts, int64_t N, int64_t K, int64_t E, int32_t* perm,
                            int32_t* offsets, int32_t* slot, void* ws, size_t ws_bytes);
@@ -417,7 +417,8 @@ int asca_embed_bwd(asca_ctx* ctx, const float* dx, const uint32_t* ids, int64_t 
  * (no counterpart in the reference): x[t] = scale * table[ids[t]]; d_table[v] (f32) = scale * sum over tokens with ids[t] == v of
  * dx[t] (`dtype`), or += with `accumulate`, which touches the rows of the tokens that occur and no other. An id at or past vocab
  * (as unsigned) is padding: a row of zeros, no part of any sum. The tokens are sorted by id; the sums run in a fixed order.
- * ws: asca_embed_scaled_bwd_ws bytes of device scratch, 256-byte aligned, the caller's until the call's work has run. */
+ * ws: asca_embed_scaled_bwd_ws bytes of device scratch (0 for few tokens: ws may be NULL then), 256-byte aligned, the caller's until
+ * the call's work has run. */
 int asca_embed_scaled_fwd(asca_ctx* ctx, const void* table, const uint32_t* ids, int64_t N, int64_t d, int64_t vocab,
                           float scale, int table_dtype, int out_dtype, void* x);
 int64_t asca_embed_scaled_bwd_ws(int64_t N, int64_t d, int64_t vocab);
