@@ -227,14 +227,14 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const Sum a) {
 // and then owns some rows of the table and some columns. A row of up to SHORT tokens is summed by the lanes that share a row, others of
 // the CTA doing other rows meanwhile; a longer one by the whole CTA, each of the lanes beside each other taking tokens in turn.
 constexpr int SHORT = 16;
-template <int W, typename T>
-__global__ void __launch_bounds__(1024) embed_small_kernel(const Sum a, const stable_sort::Job j, int lanes, int rows) {
+template <int W, int THREADS, typename T>
+__global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const stable_sort::Job j, int lanes, int rows) {
     using F = frag<W, T>;
     constexpr int E = F::E;
     extern __shared__ uint32_t sh[];   // keys and tokens, twice; places; counters. Behind the sort: the sums of the lanes beside each other
     __shared__ int32_t wsum[32];
     __shared__ int32_t long_rows[stable_sort::SMALL / SHORT], n_long;
-    const int n = (int)j.n, per = (n + 1023) / 1024, room = (n + 7) & ~7;
+    const int n = (int)j.n, per = (n + THREADS - 1) / THREADS, room = (n + 7) & ~7;
     uint32_t* keys[2] = {sh, sh + room};
     int32_t* items[2] = {reinterpret_cast<int32_t*>(sh) + 2 * room, reinterpret_cast<int32_t*>(sh) + 3 * room};
     int32_t* first = reinterpret_cast<int32_t*>(sh) + 4 * room;
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(1024) embed_small_kernel(const Sum a, const st
             }
         }
         const int shift = pass * j.digit;
-        stable_sort::rank_cta(j.bins, shift, mask, counts, first, wsum, t);
+        stable_sort::rank_cta<THREADS>(j.bins, shift, mask, counts, first, wsum, t);
         now ^= pass > 0;
 #pragma unroll
         for (int i = 0; i < stable_sort::PER; ++i) {
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(1024) embed_small_kernel(const Sum a, const st
     }
     const uint32_t* key = keys[now];
     const int32_t* item = items[now];
-    const int d = a.d, beside = 1024 / lanes, x = threadIdx.x % lanes, y = threadIdx.x / lanes;
+    const int d = a.d, beside = THREADS / lanes, x = threadIdx.x % lanes, y = threadIdx.x / lanes;
     const T* dx = static_cast<const T*>(a.dx);
     const int wide = lanes * E, c = blockIdx.y * wide + frag_first<W>(x);
     const bool in = c < d;
@@ -436,15 +436,17 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
         while (lanes < frags && lanes < 256) lanes *= 2;
         const int64_t across = ceil_div64(frags, lanes), rows = ceil_div64(vocab, std::max<int64_t>(1, ctx->sm_count / across));   // one CTA an SM
         const dim3 grid((unsigned)ceil_div64(vocab, rows), (unsigned)across);
-        const size_t sums = 1024 * 4 * (size_t)(v == 1 ? 4 : v), sorts = (size_t)j.bins * 4 + 32 * (size_t)j.bins * 2;
-        const size_t smem = 4 * (((size_t)N + 7) & ~(size_t)7) * 4 + std::max(sums, sorts);
         cudaError_t e = cudaSuccess;
         asca_with_dtype(dx, dtype, [&](auto src) {
             using T = std::remove_const_t<std::remove_pointer_t<decltype(src)>>;
             asca_with_width<T, T>(v, [&](auto wd) {
-                auto kern = embed_small_kernel<wd(), T>;
-                if (smem > 32 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-                if (e == cudaSuccess) kern<<<grid, 1024, smem, ctx->stream>>>(a, j, lanes, (int)rows);
+                stable_sort::with_threads(N, [&](auto threads) {
+                    auto kern = embed_small_kernel<wd(), threads(), T>;
+                    const size_t sums = (size_t)threads() * 4 * frag<wd(), T>::E, sorts = stable_sort::smem_bytes(threads(), j.bins);
+                    const size_t smem = 4 * (((size_t)N + 7) & ~(size_t)7) * 4 + std::max(sums, sorts);
+                    if (smem > 32 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+                    if (e == cudaSuccess) kern<<<grid, threads(), smem, ctx->stream>>>(a, j, lanes, (int)rows);
+                });
             });
         });
         ASCA_CUDA(ctx, e);

@@ -116,23 +116,22 @@ __device__ __forceinline__ void rank_items(int bins, int shift, uint32_t mask, u
         __syncwarp();
     }
 }
-// Exclusive scan of each bin over the CTA's warps, in place, four lanes a bin; the totals to tot (nullable).
-template <int THREADS>
+// Exclusive scan of each bin over the CTA's warps, in place, PARTS lanes a bin; the totals to tot.
+template <int THREADS, int PARTS>
 __device__ __forceinline__ void scan_warps(uint16_t* counts, int bins, int32_t* tot) {
-    constexpr int Q = THREADS / 32 / 4;   // a lane's warps
-    const int part = threadIdx.x & 3;
-    for (int b0 = 0; b0 < bins; b0 += THREADS / 4) {
-        const int b = b0 + (threadIdx.x >> 2);
+    constexpr int Q = THREADS / 32 / PARTS;   // a lane's warps
+    const int part = threadIdx.x % PARTS;
+    for (int b0 = 0; b0 < bins; b0 += THREADS / PARTS) {
+        const int b = b0 + threadIdx.x / PARTS;
         int c[Q], s = 0;
 #pragma unroll
-        for (int i = 0; i < Q; ++i) {
-            c[i] = b < bins ? counts[(part * Q + i) * bins + b] : 0;
-            s += c[i];
-        }
+        for (int i = 0; i < Q; ++i) c[i] = b < bins ? counts[(part * Q + i) * bins + b] : 0;
+#pragma unroll
+        for (int i = 0; i < Q; ++i) s += c[i];
         int inc = s;
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, inc, o, 4);
+        for (int o = 1; o < PARTS; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, inc, o, PARTS);
             if (part >= o) inc += y;
         }
         int at = inc - s;
@@ -142,24 +141,35 @@ __device__ __forceinline__ void scan_warps(uint16_t* counts, int bins, int32_t* 
                 counts[(part * Q + i) * bins + b] = (uint16_t)at;
                 at += c[i];
             }
-            if (tot && part == 3) tot[b] = at;
+            if (part == PARTS - 1) tot[b] = at;
         }
     }
 }
-// Ranks the items of one CTA of 1,024 threads: `first` gets the first place of each bin, t.rank and the warps' counters the rest.
+template <int THREADS>
+__device__ __forceinline__ void scan_warps(uint16_t* counts, int bins, int32_t* tot) {
+    if (bins <= THREADS / 4) scan_warps<THREADS, 4>(counts, bins, tot);
+    else scan_warps<THREADS, 1>(counts, bins, tot);
+}
+// In place: totals of the bins -> the first place of each. The caller's barrier is in front, one is behind.
+template <int THREADS>
+__device__ __forceinline__ void scan_bins(int32_t* v, int bins, int32_t* wsum) {
+    for (int b0 = 0, carry = 0; b0 < bins; b0 += THREADS) {
+        const int b = b0 + threadIdx.x, x = b < bins ? v[b] : 0;
+        int total;
+        const int at = carry + exclusive_scan<THREADS>(x, wsum, total);
+        carry += total;
+        if (b < bins) v[b] = at;
+    }
+    __syncthreads();
+}
+// Ranks the items of one CTA: `first` gets the first place of each bin, t.rank and the warps' counters the rest.
+template <int THREADS>
 __device__ __forceinline__ void rank_cta(int bins, int shift, uint32_t mask, uint16_t* counts, int32_t* first, int32_t* wsum, Items& t) {
     rank_items(bins, shift, mask, counts + (threadIdx.x >> 5) * bins, t);
     __syncthreads();
-    scan_warps<1024>(counts, bins, first);
+    scan_warps<THREADS>(counts, bins, first);
     __syncthreads();
-    for (int b0 = 0, carry = 0; b0 < bins; b0 += 1024) {
-        const int b = b0 + threadIdx.x, v = b < bins ? first[b] : 0;
-        int total;
-        const int at = carry + exclusive_scan<1024>(v, wsum, total);
-        carry += total;
-        if (b < bins) first[b] = at;
-    }
-    __syncthreads();
+    scan_bins<THREADS>(first, bins, wsum);
 }
 __device__ __forceinline__ void put_items(const Job& j, int pass, const Items& t, const int32_t* base, const uint16_t* run) {
     const int shift = pass * j.digit;
@@ -176,20 +186,29 @@ __device__ __forceinline__ void put_items(const Job& j, int pass, const Items& t
     }
 }
 
-inline size_t smem_bytes(int threads, int bins) { return (size_t)bins * 4 + (size_t)threads / 32 * bins * 2; }
+inline size_t smem_bytes(int threads, int bins) { return (size_t)bins * 8 + (size_t)threads / 32 * bins * 2; }
 
-static __global__ void __launch_bounds__(1024) sort_small_kernel(const Job j) {
-    extern __shared__ __align__(16) int32_t sh[];   // a bin's total, then first place; the warps' counters
+// f(std::integral_constant of 256, 512 or 1024): the threads that n items keep busy, four each
+template <typename F>
+inline void with_threads(int64_t n, F f) {
+    if (n <= 256 * PER) f(std::integral_constant<int, 256>());
+    else if (n <= 512 * PER) f(std::integral_constant<int, 512>());
+    else f(std::integral_constant<int, 1024>());
+}
+
+template <int THREADS>
+static __global__ void __launch_bounds__(THREADS) sort_small_kernel(const Job j) {
+    extern __shared__ __align__(16) int32_t sh[];   // a bin's first place; the warps' counters
     __shared__ int32_t wsum[32];
     pdl_launch_dependents();
     uint16_t *counts = reinterpret_cast<uint16_t*>(sh + j.bins), *run = counts + (threadIdx.x >> 5) * j.bins;
-    const int n = (int)j.n, per = (n + 1023) / 1024;
+    const int n = (int)j.n, per = (n + THREADS - 1) / THREADS;
     for (int pass = 0; pass < j.passes; ++pass) {
         Items t;
         load_items(j, pass, (threadIdx.x >> 5) * per * 32, per, t);
-        rank_cta(j.bins, pass * j.digit, mask_of(j), counts, sh, wsum, t);
+        rank_cta<THREADS>(j.bins, pass * j.digit, mask_of(j), counts, sh, wsum, t);
         if (j.offsets)
-            for (int b = threadIdx.x; b < j.bins; b += 1024) j.offsets[b] = sh[b];
+            for (int b = threadIdx.x; b < j.bins; b += THREADS) j.offsets[b] = sh[b];
         put_items(j, pass, t, sh, run);
         __syncthreads();   // (what the next pass reads)
     }
@@ -221,87 +240,127 @@ static __global__ void __launch_bounds__(1024) scan_kernel(const Job j, int32_t*
     pdl_launch_dependents();
     for (int b0 = 0, carry = 0; b0 < j.bins; b0 += 1024) {
         const int b = b0 + threadIdx.x;
-        int all = 0;
-        if (b < j.bins) {
-#pragma unroll 16
-            for (int t = 0; t < n_tiles; ++t) all += counts[(int64_t)t * j.bins + b];
-        }
-        int total;
+        int32_t* column = counts + b;
+        auto each = [&](auto f) {   // sixteen tiles' entries in flight
+            if (b >= j.bins) return;
+            for (int t0 = 0; t0 < n_tiles; t0 += 16) {
+                int c[16];
+#pragma unroll
+                for (int u = 0; u < 16; ++u) c[u] = t0 + u < n_tiles ? column[(int64_t)(t0 + u) * j.bins] : 0;
+#pragma unroll
+                for (int u = 0; u < 16; ++u)
+                    if (t0 + u < n_tiles) f(t0 + u, c[u]);
+            }
+        };
+        int all = 0, total;
+        each([&](int, int c) { all += c; });
         int at = carry + exclusive_scan<1024>(all, wsum, total);
         carry += total;
-        if (b < j.bins) {
-            if (j.offsets) j.offsets[b] = at;
-#pragma unroll 16
-            for (int t = 0; t < n_tiles; ++t) {
-                const int c = counts[(int64_t)t * j.bins + b];
-                counts[(int64_t)t * j.bins + b] = at;
-                at += c;
-            }
-        }
+        if (b < j.bins && j.offsets) j.offsets[b] = at;
+        each([&](int t, int c) {
+            column[(int64_t)t * j.bins] = at;
+            at += c;
+        });
     }
 }
 
 // SCANNED: the table holds first places (scan_kernel); otherwise counts, which the CTA adds up: 512 / Q bins at a time, Q threads a bin.
+// The items are put in order inside the tile first, so that what goes out together goes to neighbouring places.
 template <bool SCANNED>
-static __global__ void __launch_bounds__(512) place_kernel(const Job j, int pass, const int32_t* __restrict__ table, int n_tiles, int q) {
-    extern __shared__ __align__(16) int32_t sh[];   // first places [bin]; the warps' counters
+static __global__ void __launch_bounds__(512) place_kernel(const Job j, int pass, const int32_t* __restrict__ table, int n_tiles, int q_log) {
+    extern __shared__ __align__(16) int32_t sh[];   // first places [bin]; places inside the tile [bin]; the warps' counters
     __shared__ int32_t wsum[32];
-    uint16_t *counts = reinterpret_cast<uint16_t*>(sh + j.bins), *run = counts + (threadIdx.x >> 5) * j.bins;
-    const int mine = blockIdx.x;
+    __shared__ uint32_t keys[TILE];
+    __shared__ int32_t items[TILE];
+    int32_t *first = sh, *inside = sh + j.bins;
+    uint16_t *counts = reinterpret_cast<uint16_t*>(sh + 2 * j.bins), *run = counts + (threadIdx.x >> 5) * j.bins;
+    const int mine = blockIdx.x, shift = pass * j.digit;
+    const uint32_t mask = mask_of(j);
     pdl_wait();
     pdl_launch_dependents();
     Items t;
     load_items(j, pass, (int64_t)mine * TILE + (threadIdx.x >> 5) * PER * 32, PER, t);
     if (SCANNED) {
-        for (int b = threadIdx.x; b < j.bins; b += 512) sh[b] = table[(int64_t)mine * j.bins + b];
+        for (int b = threadIdx.x; b < j.bins; b += 512) first[b] = table[(int64_t)mine * j.bins + b];
     } else {
-        for (int b0 = 0, carry = 0; b0 < j.bins; b0 += 512 / q) {
-            const int b = b0 + threadIdx.x / q;
+        const int q = 1 << q_log, lane = threadIdx.x & (q - 1);
+        for (int b0 = 0, carry = 0; b0 < j.bins; b0 += 512 >> q_log) {
+            const int b = b0 + (threadIdx.x >> q_log);
             int before = 0, all = 0;
             if (b < j.bins) {
-#pragma unroll 8
-                for (int i = threadIdx.x % q; i < n_tiles; i += q) {
-                    const int c = table[(int64_t)i * j.bins + b];
-                    all += c;
-                    if (i < mine) before += c;
+                for (int i0 = lane; i0 < n_tiles; i0 += 16 << q_log) {
+                    int c[16];
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) c[u] = i0 + (u << q_log) < n_tiles ? table[(i0 + (u << q_log)) * j.bins + b] : 0;
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) {
+                        all += c[u];
+                        if (i0 + (u << q_log) < mine) before += c[u];
+                    }
                 }
             }
             for (int o = 1; o < q; o <<= 1) {
                 before += __shfl_xor_sync(0xffffffffu, before, o);
                 all += __shfl_xor_sync(0xffffffffu, all, o);
             }
-            const bool first_lane = threadIdx.x % q == 0;
             int total;
-            const int first = carry + exclusive_scan<512>(first_lane ? all : 0, wsum, total);
+            const int at = carry + exclusive_scan<512>(lane == 0 ? all : 0, wsum, total);
             carry += total;
-            if (b < j.bins && first_lane) {
-                sh[b] = first + before;
-                if (j.offsets && mine == 0) j.offsets[b] = first;
+            if (b < j.bins && lane == 0) {
+                first[b] = at + before;
+                if (j.offsets && mine == 0) j.offsets[b] = at;
             }
         }
     }
-    rank_items(j.bins, pass * j.digit, mask_of(j), run, t);   // (while the table's entries come in)
+    rank_items(j.bins, shift, mask, run, t);
     __syncthreads();
-    scan_warps<512>(counts, j.bins, nullptr);
+    scan_warps<512>(counts, j.bins, inside);
     __syncthreads();
-    put_items(j, pass, t, sh, run);
+    scan_bins<512>(inside, j.bins, wsum);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (t.item[i] < 0) continue;
+        const int b = (int)((t.key[i] >> shift) & mask), at = run[b] + t.rank[i];
+        keys[inside[b] + at] = t.key[i];
+        items[inside[b] + at] = t.item[i];
+        if (j.place) j.place[t.item[i]] = t.key[i] == j.limit ? -1 : first[b] + at;
+    }
+    __syncthreads();
+    uint32_t* to_keys = keys_to(j, pass);
+    int32_t* to_items = items_to(j, pass);
+    const int n = (int)min((int64_t)TILE, j.n - (int64_t)mine * TILE);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int p = i * 512 + threadIdx.x;
+        if (p >= n) break;
+        const uint32_t key = keys[p];
+        const int b = (int)((key >> shift) & mask), at = first[b] + p - inside[b];
+        if (to_keys) to_keys[at] = key;
+        to_items[at] = items[p];
+    }
 }
 
 // Leaves the result in keys / items [(passes - 1) & 1]; table: scratch_bytes(n, bins) of scratch. Every kernel lets the next one's
 // launch begin early.
 static inline int sort(asca_ctx* ctx, const Job& j, int32_t* table) {
-    const size_t smem = smem_bytes(j.n <= SMALL ? 1024 : 512, j.bins);
     if (j.n <= SMALL) {
-        if (smem > 40 * 1024) ASCA_CUDA(ctx, cudaFuncSetAttribute(sort_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        sort_small_kernel<<<1, 1024, smem, ctx->stream>>>(j);
+        cudaError_t e = cudaSuccess;
+        with_threads(j.n, [&](auto threads) {
+            auto kern = sort_small_kernel<threads()>;
+            const size_t smem = smem_bytes(threads(), j.bins);
+            if (smem > 40 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e == cudaSuccess) kern<<<1, threads(), smem, ctx->stream>>>(j);
+        });
+        ASCA_CUDA(ctx, e);
         ASCA_CHECK_LAUNCH(ctx);
         return ASCA_OK;
     }
+    const size_t smem = smem_bytes(512, j.bins);
     const int n = (int)tiles(j.n);
     const bool scanned = (int64_t)n * j.bins > OWN_SCAN;
-    int q = 1;   // threads a bin
-    while (q < 32 && (q * 2) * j.bins <= 512) q *= 2;
-    if (smem > 40 * 1024) {
+    int q_log = 0;   // threads a bin
+    while (q_log < 5 && (j.bins << (q_log + 1)) <= 512) ++q_log;
+    if (smem > 24 * 1024) {   // (16 KiB of static arrays beside it)
         ASCA_CUDA(ctx, cudaFuncSetAttribute(place_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         ASCA_CUDA(ctx, cudaFuncSetAttribute(place_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     }
@@ -309,7 +368,7 @@ static inline int sort(asca_ctx* ctx, const Job& j, int32_t* table) {
         if (p == 0) count_kernel<<<(unsigned)n, 512, (size_t)j.bins * 4, ctx->stream>>>(j, p, table);
         else ASCA_CUDA(ctx, asca_launch_after(ctx, count_kernel, dim3(n), dim3(512), (size_t)j.bins * 4, j, p, table));
         if (scanned) ASCA_CUDA(ctx, asca_launch_after(ctx, scan_kernel, dim3(1), dim3(1024), 0, j, table, n));
-        ASCA_CUDA(ctx, asca_launch_after(ctx, scanned ? place_kernel<true> : place_kernel<false>, dim3(n), dim3(512), smem, j, p, (const int32_t*)table, n, q));
+        ASCA_CUDA(ctx, asca_launch_after(ctx, scanned ? place_kernel<true> : place_kernel<false>, dim3(n), dim3(512), smem, j, p, (const int32_t*)table, n, q_log));
         ctx->launches += scanned ? 3 : 2;
     }
     ASCA_CUDA(ctx, cudaGetLastError());

@@ -645,16 +645,17 @@ def test_refusals(gpu):
         with pytest.raises(asca_b200.AscaError):
             ops.clip_grads(gpu, [x], bad)
     # scratch that is too small, through the C boundary
-    many, rows, table, out = text(1, 5000, 20, "zipf"), rand(1, 5000, 8), rand(1, 20, 8), torch.empty(10009, dtype=torch.int32, device="cuda")
-    calls = {"asca_embed_scaled_bwd": (gpu.lib.asca_embed_scaled_bwd_ws(5000, 8, 20), lambda at, n: gpu._run(
-                 "asca_embed_scaled_bwd", rows.data_ptr(), many.data_ptr(), 5000, 8, 20, 1.0, asca_b200.F32, 0, table.data_ptr(), at, n)),
-             "asca_moe_topk_dispatch": (gpu.lib.asca_moe_topk_dispatch_ws(5000, 1, 8), lambda at, n: gpu._run(
-                 "asca_moe_topk_dispatch", many.data_ptr(), 5000, 1, 8, out.data_ptr(), out.data_ptr() + 20000, out.data_ptr() + 20036, at, n))}
+    n = 40_000
+    many, rows, table, out = text(1, n, 20, "zipf"), rand(1, n, 8), rand(1, 20, 8), torch.empty(2 * n + 9, dtype=torch.int32, device="cuda")
+    calls = {"asca_embed_scaled_bwd": (gpu.lib.asca_embed_scaled_bwd_ws(n, 8, 20), lambda at, size: gpu._run(
+                 "asca_embed_scaled_bwd", rows.data_ptr(), many.data_ptr(), n, 8, 20, 1.0, asca_b200.F32, 0, table.data_ptr(), at, size)),
+             "asca_moe_topk_dispatch": (gpu.lib.asca_moe_topk_dispatch_ws(n, 1, 8), lambda at, size: gpu._run(
+                 "asca_moe_topk_dispatch", many.data_ptr(), n, 1, 8, out.data_ptr(), out.data_ptr() + 4 * n, out.data_ptr() + 4 * n + 36, at, size))}
     for nbytes, call in calls.values():
         ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
-        for at, n in ((ws.data_ptr(), nbytes - 1), (ws.data_ptr() + 4, nbytes), (0, 0), (0, nbytes)):
+        for at, size in ((ws.data_ptr(), nbytes - 1), (ws.data_ptr() + 4, nbytes), (0, 0), (0, nbytes)):
             with pytest.raises(asca_b200.AscaError) as err:
-                call(at, n)
+                call(at, size)
             assert err.value.code == -1
         call(ws.data_ptr(), nbytes)
     # a context on another stream than torch's current one

@@ -17,7 +17,7 @@ def test_scratch_sizes():
     # sorted keys and tokens twice, at least; nothing that grows with vocabulary times tokens
     assert 4 * 4 * 100_000 < lib.asca_embed_scaled_bwd_ws(100_000, 64, 50_000) < 100_000 * 64 * 4
     assert lib.asca_embed_scaled_bwd_ws(-1, 8, 10) < 0 and lib.asca_embed_scaled_bwd_ws(1, 0, 10) < 0 and lib.asca_embed_scaled_bwd_ws(1, 8, 0) < 0
-    assert lib.asca_moe_topk_dispatch_ws(1, 1, 2048) == 0 and lib.asca_moe_topk_dispatch_ws(4097, 1, 2048) > 0 and lib.asca_moe_topk_dispatch_ws(1, 1, 2049) < 0 and lib.asca_moe_topk_dispatch_ws(1, 0, 4) < 0
+    assert lib.asca_moe_topk_dispatch_ws(1, 1, 2048) == 0 and lib.asca_moe_topk_dispatch_ws(40_000, 1, 2048) > 0 and lib.asca_moe_topk_dispatch_ws(1, 1, 2049) < 0 and lib.asca_moe_topk_dispatch_ws(1, 0, 4) < 0
     # without a context: refused, not followed
     assert lib.asca_gated_residual_rmsnorm_bwd_ws(None, 4, 4) < 0 and lib.asca_grad_norm_ws(None, 1) < 0
 
