@@ -73,6 +73,7 @@ struct Sum {
     float scale;
     float *d_table, *part;
     int64_t sums, zeros;    // blocks of the two kinds; they take turns in the grid
+    bool narrow;            // rows of the table
 };
 
 // The first place in the sorted keys that is not below v.
@@ -88,22 +89,44 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, 
     return lo;
 }
 
-// ZERO_ROWS rows of the table: those without a token are cleared.
+// The same from `at` on, by a warp: every round looks at 32 places.
+__device__ __forceinline__ int64_t warp_lower_bound(const uint32_t* keys, int64_t at, int64_t N, uint32_t v, int lane) {
+    int64_t n = N - at;   // the answer is in [at, at + n]
+    while (n > 0) {
+        const int64_t step = (n + 31) / 32, mine = lane * step;
+        const int below = __popc(__ballot_sync(0xffffffffu, mine < n && keys[at + mine] < v));
+        if (below == 0) return at;
+        const int64_t from = (below - 1) * step + 1;
+        n = min(step - 1, n - from);
+        at += from;
+    }
+    return at;
+}
+
+// ZERO_ROWS rows of the table: those without a token are cleared. Narrow rows: every warp of the block has rows of its own.
 template <int W>
 __device__ __forceinline__ void zero_rows(const Sum& a, int64_t block) {
-    const int lane = threadIdx.x + threadIdx.y * blockDim.x, threads = blockDim.x * blockDim.y;
-    const int64_t v = block * ZERO_ROWS + (lane & 31);
-    bool none = false;
-    if (v < a.vocab) {
-        const int64_t at = lower_bound(a.keys, a.N, (uint32_t)v);
-        none = at == a.N || a.keys[at] != v;
+    const int me = threadIdx.x + threadIdx.y * blockDim.x, threads = blockDim.x * blockDim.y, lane = me & 31;
+    const int64_t v0 = (a.narrow ? block * (threads >> 5) + (me >> 5) : block) * ZERO_ROWS;
+    if (v0 >= a.vocab) return;
+    const uint32_t rows = (uint32_t)min((int64_t)ZERO_ROWS, a.vocab - v0);
+    // the rows' tokens lie in [lo, hi) of the sorted order: few are looked at one by one, many are looked for row by row
+    const int64_t lo = warp_lower_bound(a.keys, 0, a.N, (uint32_t)v0, lane), hi = warp_lower_bound(a.keys, lo, a.N, (uint32_t)v0 + rows, lane);
+    unsigned met = 0;
+    if (hi - lo <= 128) {
+        for (int64_t at = lo + lane; at < hi; at += 32) met |= 1u << (a.keys[at] - (uint32_t)v0);
+        met = __reduce_or_sync(0xffffffffu, met);
+    } else {
+        const uint32_t v = (uint32_t)v0 + lane;
+        const int64_t at = lo + lower_bound(a.keys + lo, hi - lo, v);
+        met = __ballot_sync(0xffffffffu, at < hi && a.keys[at] == v);
     }
-    const unsigned rows = __ballot_sync(0xffffffffu, none);   // (each warp looks for itself)
     using F = frag<W, float>;
     const float zero[F::E] = {};
-    for (unsigned left = rows; left; left &= left - 1) {
-        float* p = a.d_table + (block * ZERO_ROWS + __ffs(left) - 1) * a.d;
-        for (int c = frag_first<W>(lane); c < a.d; c += threads * F::E) F::put(p, c, threads, a.d, zero);
+    const int x = a.narrow ? lane : me, lanes = a.narrow ? 32 : threads;
+    for (unsigned left = ~met & (rows < 32 ? (1u << rows) - 1 : 0xffffffffu); left; left &= left - 1) {
+        float* p = a.d_table + (v0 + __ffs(left) - 1) * a.d;
+        for (int c = frag_first<W>(x); c < a.d; c += lanes * F::E) F::put(p, c, lanes, a.d, zero);
     }
 }
 
@@ -430,7 +453,8 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
     a.items = j.items[(plan.passes - 1) & 1];
     a.part = (float*)(w + 4 * plan.list + plan.counts);
     a.sums = ceil_div64(pieces, block.y) * groups;
-    a.zeros = accumulate ? 0 : ceil_div64(vocab, ZERO_ROWS);
+    a.narrow = d <= 256;
+    a.zeros = accumulate ? 0 : ceil_div64(vocab, a.narrow ? ZERO_ROWS * (int64_t)(block.x * block.y / 32) : ZERO_ROWS);
     if (plan.small) {
         int lanes = 1;
         while (lanes < frags && lanes < 256) lanes *= 2;
