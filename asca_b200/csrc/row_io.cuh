@@ -22,7 +22,7 @@ inline size_t asca_dtype_size(int dtype) { return dtype == ASCA_BF16 ? 2 : 4; }
 inline bool asca_aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 // v (4 or 8) elements of a row of `cols` can be moved at once at every multiple of v columns (a null pointer has no rows)
 inline bool asca_rows_by(int v, const void* p, int64_t cols, int dtype) {
-    return cols % v == 0 && asca_aligned(p, std::min<size_t>(16, v * asca_dtype_size(dtype)));
+    return cols % v == 0 && asca_aligned(p, v * asca_dtype_size(dtype));
 }
 
 // f(pointer of the type that `dtype` names); a const pointer stays const
@@ -125,20 +125,29 @@ template <>
 struct raw_row<8, __nv_bfloat16> {
     uint4 v;
 };
-// V consecutive elements of a row: 8 or 4 through 16-byte accesses (8 for bf16 alone), 1 for rows off their grid or of another width
+// V consecutive elements of a row, in one access each
+// Eight f32 go in one 32-byte access: two of 16 bytes would each touch half of every sector, twice the sectors for the same bytes.
+__device__ __forceinline__ void ld8(const float* p, float4& a, float4& b) {
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(a.x), "=f"(a.y), "=f"(a.z), "=f"(a.w), "=f"(b.x), "=f"(b.y), "=f"(b.z), "=f"(b.w)
+                 : "l"(__cvta_generic_to_global(p)));
+}
+__device__ __forceinline__ void st8(float* p, float4 a, float4 b) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(__cvta_generic_to_global(p)), "f"(a.x), "f"(a.y), "f"(a.z), "f"(a.w), "f"(b.x), "f"(b.y), "f"(b.z),
+                 "f"(b.w)
+                 : "memory");
+}
 template <int V, typename T>
 __device__ __forceinline__ raw_row<V, T> ld_raw(const T* p) {
     raw_row<V, T> r;
-    if constexpr (V == 8 && sizeof(T) == 4) {
-        r.v = *reinterpret_cast<const float4*>(p);
-        r.w = *reinterpret_cast<const float4*>(p + 4);
-    } else r.v = *reinterpret_cast<const decltype(r.v)*>(p);
+    if constexpr (V == 8 && sizeof(T) == 4) ld8(p, r.v, r.w);
+    else r.v = *reinterpret_cast<const decltype(r.v)*>(p);
     return r;
 }
 template <int V, typename T>
 __device__ __forceinline__ void st_raw(T* p, const raw_row<V, T>& r) {
-    *reinterpret_cast<std::remove_const_t<decltype(r.v)>*>(p) = r.v;
-    if constexpr (V == 8 && sizeof(T) == 4) *reinterpret_cast<float4*>(p + 4) = r.w;
+    if constexpr (V == 8 && sizeof(T) == 4) st8(p, r.v, r.w);
+    else *reinterpret_cast<std::remove_const_t<decltype(r.v)>*>(p) = r.v;
 }
 __device__ __forceinline__ void unpack(const raw_row<1, float>& r, float (&v)[1]) { v[0] = r.v; }
 __device__ __forceinline__ void unpack(const raw_row<1, __nv_bfloat16>& r, float (&v)[1]) { v[0] = __bfloat162float(r.v); }
@@ -157,7 +166,8 @@ template <int V, typename T>
 __device__ __forceinline__ void ld_row(const T* p, float (&v)[V]) { unpack(ld_raw<V>(p), v); }
 template <int V, typename T>
 __device__ __forceinline__ void st_row(T* p, const float (&v)[V]) {
-    if constexpr (V == 8 && sizeof(T) == 2) {
+    if constexpr (V == 8 && sizeof(T) == 4) st8(p, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]));
+    else if constexpr (V == 8) {
         *reinterpret_cast<uint4*>(p) = make_uint4(f32_bf16x2(v[0], v[1]), f32_bf16x2(v[2], v[3]), f32_bf16x2(v[4], v[5]), f32_bf16x2(v[6], v[7]));
     } else if constexpr (V % 4 == 0) {
 #pragma unroll
