@@ -184,71 +184,81 @@ __global__ void __launch_bounds__(128) embed_pieces_kernel(const Sum a) {
     }
 }
 
-// A block owns a piece; it has work where a run begins in the piece and goes on past it. Its lanes beside each other (threadIdx.y) take the
-// run's pieces in turn, eight of them in flight.
+// A block owns `pieces` pieces; it has work where a run begins in one of them and goes on past it. Its lanes beside each other
+// (threadIdx.y) take the run's pieces in turn, eight of them in flight.
+constexpr int MOST_JOINED = 32;
 template <int W>
-__global__ void __launch_bounds__(256) embed_join_kernel(const Sum a) {
+__global__ void __launch_bounds__(256) embed_join_kernel(const Sum a, int pieces) {
     using F = frag<W, float>;
     constexpr int E = F::E;
     extern __shared__ uint32_t sh_raw[];
     float(*sh)[E] = reinterpret_cast<float(*)[E]>(sh_raw);   // [lane beside][column lane]
-    const int64_t p = blockIdx.x;
+    __shared__ bool begins[MOST_JOINED];
     const int piece = a.piece, d = a.d, lanes = blockDim.x, beside = blockDim.y, threads = lanes * beside, me = threadIdx.y * lanes + threadIdx.x;
     pdl_wait();
-    const int64_t end = (p + 1) * piece;
-    const uint32_t key = a.keys[end - 1], next = a.keys[end], left = p > 0 ? a.keys[p * piece - 1] : 0xffffffffu;   // (the last piece has no block)
-    if (key >= a.vocab || next != key || left == key) return;   // (the last: it began further left)
-    int64_t more = 0;   // pieces that the run comes into from the left
-    for (;; more += threads) {
-        const int64_t q = p + 1 + more + me;
-        const int in = __syncthreads_count(q * piece < a.N && a.keys[q * piece] == key);
-        if (in < threads) {
-            more += in;
-            break;
-        }
+    const int64_t p0 = (int64_t)blockIdx.x * pieces;
+    for (int i = me; i < pieces; i += threads) {
+        const int64_t p = p0 + i, end = (p + 1) * piece;
+        begins[i] = end < a.N && a.keys[end - 1] < a.vocab && a.keys[end] == a.keys[end - 1] &&
+                    !(p > 0 && a.keys[p * piece - 1] == a.keys[end - 1]);   // (the last: it began further left)
     }
-    for (int c = frag_first<W>(threadIdx.x); c - frag_first<W>(threadIdx.x) < d; c += lanes * E) {   // (the same turns for all)
-        float acc[E] = {};
-        auto add = [&](const F& r) {
-            float v[E];
-            r.get(v);
-#pragma unroll
-            for (int j = 0; j < E; ++j) acc[j] += v[j];
-        };
-        if (c < d) {
-            F r[AHEAD];
-            if (threadIdx.y == 0) {
-                r[0].load(a.part + (2 * p + 1) * d, c, lanes, d);
-                add(r[0]);
-            }
-            for (int64_t q0 = threadIdx.y; q0 < more; q0 += (int64_t)AHEAD * beside) {
-#pragma unroll
-                for (int u = 0; u < AHEAD; ++u)
-                    if (q0 + u * beside < more) r[u].load(a.part + 2 * (p + 1 + q0 + u * beside) * d, c, lanes, d);
-#pragma unroll
-                for (int u = 0; u < AHEAD; ++u)
-                    if (q0 + u * beside < more) add(r[u]);
+    __syncthreads();
+    for (int64_t p = p0; p < p0 + pieces; ++p) {
+        if (!begins[p - p0]) continue;
+        const uint32_t key = a.keys[(p + 1) * piece - 1];
+        int64_t more = 0;   // pieces that the run comes into from the left
+        for (;; more += threads) {
+            const int64_t q = p + 1 + more + me;
+            const int in = __syncthreads_count(q * piece < a.N && a.keys[q * piece] == key);
+            if (in < threads) {
+                more += in;
+                break;
             }
         }
-        if (beside > 1) {
+        for (int c = frag_first<W>(threadIdx.x); c - frag_first<W>(threadIdx.x) < d; c += lanes * E) {   // (the same turns for all)
+            float acc[E] = {};
+            auto add = [&](const F& r) {
+                float v[E];
+                r.get(v);
 #pragma unroll
-            for (int j = 0; j < E; ++j) sh[me][j] = acc[j];
-            __syncthreads();
-            if (threadIdx.y == 0) {
-                for (int i = 1; i < beside; ++i) {
+                for (int j = 0; j < E; ++j) acc[j] += v[j];
+            };
+            if (c < d) {
+                F r[AHEAD];
+                if (threadIdx.y == 0) {
+                    r[0].load(a.part + (2 * p + 1) * d, c, lanes, d);
+                    add(r[0]);
+                }
+                for (int64_t q0 = threadIdx.y; q0 < more; q0 += (int64_t)AHEAD * beside) {
 #pragma unroll
-                    for (int j = 0; j < E; ++j) acc[j] += sh[i * lanes + threadIdx.x][j];
+                    for (int u = 0; u < AHEAD; ++u)
+                        if (q0 + u * beside < more) r[u].load(a.part + 2 * (p + 1 + q0 + u * beside) * d, c, lanes, d);
+#pragma unroll
+                    for (int u = 0; u < AHEAD; ++u)
+                        if (q0 + u * beside < more) add(r[u]);
                 }
             }
-            __syncthreads();
+            if (beside > 1) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) sh[me][j] = acc[j];
+                __syncthreads();
+                if (threadIdx.y == 0) {
+                    for (int i = 1; i < beside; ++i) {
+#pragma unroll
+                        for (int j = 0; j < E; ++j) acc[j] += sh[i * lanes + threadIdx.x][j];
+                    }
+                }
+                __syncthreads();
+            }
+            if (threadIdx.y == 0 && c < d) add_row<W>(a.d_table + (int64_t)key * d, c, lanes, d, acc, a.scale, a.accumulate);
         }
-        if (threadIdx.y == 0 && c < d) add_row<W>(a.d_table + (int64_t)key * d, c, lanes, d, acc, a.scale, a.accumulate);
     }
 }
 
 // Few tokens: everything in one launch. Every CTA sorts all of them in its own shared memory (the same few microseconds at the same time)
-// and then owns some rows of the table and some columns. A row of up to SHORT tokens is summed by the lanes that share a row, others of
-// the CTA doing other rows meanwhile; a longer one by the whole CTA, each of the lanes beside each other taking tokens in turn.
+// and then owns some rows of the table and some columns, which it clears first where the table is overwritten. A row of up to SHORT
+// tokens is summed by the lanes that share a row, others of the CTA doing other rows meanwhile; a longer one by the whole CTA, each of
+// the lanes beside each other taking tokens in turn.
 constexpr int SHORT = 16;
 template <int W, int THREADS, typename T>
 __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const stable_sort::Job j, int lanes, int rows) {
@@ -256,13 +266,23 @@ __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const
     constexpr int E = F::E;
     extern __shared__ uint32_t sh[];   // keys and tokens, twice; places; counters. Behind the sort: the sums of the lanes beside each other
     __shared__ int32_t wsum[32];
-    __shared__ int32_t long_rows[stable_sort::SMALL / SHORT], n_long;
+    __shared__ int32_t long_runs[stable_sort::SMALL / SHORT], n_long;   // where they begin in the sorted order
     const int n = (int)j.n, per = (n + THREADS - 1) / THREADS, room = (n + 7) & ~7;
     uint32_t* keys[2] = {sh, sh + room};
     int32_t* items[2] = {reinterpret_cast<int32_t*>(sh) + 2 * room, reinterpret_cast<int32_t*>(sh) + 3 * room};
     int32_t* first = reinterpret_cast<int32_t*>(sh) + 4 * room;
     uint16_t *counts = reinterpret_cast<uint16_t*>(first + j.bins), *run = counts + (threadIdx.x >> 5) * j.bins;
     const uint32_t mask = stable_sort::mask_of(j);
+    const int d = a.d, beside = THREADS / lanes, x = threadIdx.x % lanes, y = threadIdx.x / lanes;
+    const int wide = lanes * E, c = blockIdx.y * wide + frag_first<W>(x);
+    const bool in = c < d;
+    const int64_t v0 = (int64_t)blockIdx.x * rows, v1 = min(v0 + rows, (int64_t)a.vocab);
+    if (!a.accumulate) {
+        const float zero[E] = {};
+        if (gridDim.y == 1) stable_sort::clear_floats(a.d_table + v0 * d, (v1 - v0) * d, threadIdx.x, THREADS);
+        else if (in)
+            for (int64_t v = v0 + y; v < v1; v += beside) frag<W, float>::put(a.d_table + v * d, c, lanes, d, zero);
+    }
     if (threadIdx.x == 0) n_long = 0;
     int now = 0;
     for (int pass = 0; pass < j.passes; ++pass) {
@@ -292,11 +312,7 @@ __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const
     }
     const uint32_t* key = keys[now];
     const int32_t* item = items[now];
-    const int d = a.d, beside = THREADS / lanes, x = threadIdx.x % lanes, y = threadIdx.x / lanes;
     const T* dx = static_cast<const T*>(a.dx);
-    const int wide = lanes * E, c = blockIdx.y * wide + frag_first<W>(x);
-    const bool in = c < d;
-    const int64_t v0 = (int64_t)blockIdx.x * rows;
     auto sum = [&](int lo, int step, int end, float (&acc)[E]) {
         for (int i0 = lo; i0 < end; i0 += AHEAD * step) {
             F r[AHEAD];
@@ -314,24 +330,25 @@ __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const
         }
     };
     auto bound = [&](uint32_t v) { return (int)lower_bound(key, n, v); };
-    for (int64_t v = v0 + y; v < v0 + rows && v < a.vocab && in; v += beside) {
-        const int lo = bound((uint32_t)v);
-        const bool some = lo < n && key[lo] == v;
-        if (!some && a.accumulate) continue;   // left as it was
-        const int end = some ? bound((uint32_t)v + 1) : lo;
-        if (end - lo > SHORT) {
-            if (x == 0) long_rows[atomicAdd(&n_long, 1)] = (int32_t)v;   // (rows are summed one by one: their order does not matter)
+    const int p0 = bound((uint32_t)v0), p1 = bound((uint32_t)v1);   // (behind barriers: the zeros are in place)
+    for (int p = p0 + y; p < p1; p += beside) {
+        if (p > p0 && key[p] == key[p - 1]) continue;   // (not where a row's run begins)
+        int end = p + 1;
+        while (end < p1 && key[end] == key[p] && end - p <= SHORT) ++end;
+        if (end - p > SHORT) {
+            if (x == 0) long_runs[atomicAdd(&n_long, 1)] = p;   // (rows are summed one by one: their order does not matter)
             continue;
         }
+        if (!in) continue;
         float acc[E] = {};
-        sum(lo, 1, end, acc);
-        add_row<W>(a.d_table + v * d, c, lanes, d, acc, a.scale, a.accumulate);
+        sum(p, 1, end, acc);
+        add_row<W>(a.d_table + (int64_t)key[p] * d, c, lanes, d, acc, a.scale, a.accumulate);
     }
     __syncthreads();
     float* part = reinterpret_cast<float*>(first);   // [lane beside][column lane][E]: the places and counters are no longer needed
     for (int l = 0; l < n_long; ++l) {
-        const uint32_t v = (uint32_t)long_rows[l];
-        const int lo = bound(v), end = bound(v + 1);
+        const int lo = long_runs[l], end = bound(key[lo] + 1);
+        const uint32_t v = key[lo];
         float acc[E] = {};
         if (in) sum(lo + y, beside, end, acc);
 #pragma unroll
@@ -364,11 +381,11 @@ struct Plan {
         passes = (int)ceil_div64(bits, 11);
         digit = (int)ceil_div64(bits, passes);
         bins = passes == 1 ? (int)vocab + 1 : 1 << digit;
-        // short pieces where the tokens are few: the walk down a piece is what such a call waits for
+        // short pieces where the tokens are few: 256 threads an SM walk down pieces at once, or the walk is what the call waits for
         piece = MOST_PIECE;
-        while (piece > AHEAD && N * d < (int64_t)piece * 148 * 4096) piece /= 2;
-        // (a CTA of the one launch may have to add all of dx's rows by itself)
-        small = N <= stable_sort::SMALL && N * d <= (1 << 20);
+        while (piece > AHEAD && ceil_div64(N, piece) * std::max<int64_t>(8, ceil_div64(d, 4)) < 148 * 256) piece /= 2;
+        // (a CTA of the one launch may have to add its columns of all of dx's rows by itself)
+        small = N <= stable_sort::SMALL && N * d <= (4 << 20);
         if (small) {
             list = counts = part = 0;
             return;
@@ -457,7 +474,7 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
     a.zeros = accumulate ? 0 : ceil_div64(vocab, a.narrow ? ZERO_ROWS * (int64_t)(block.x * block.y / 32) : ZERO_ROWS);
     if (plan.small) {
         int lanes = 1;
-        while (lanes < frags && lanes < 256) lanes *= 2;
+        while (lanes < frags && lanes < 64) lanes *= 2;
         const int64_t across = ceil_div64(frags, lanes), rows = ceil_div64(vocab, std::max<int64_t>(1, ctx->sm_count / across));   // one CTA an SM
         const dim3 grid((unsigned)ceil_div64(vocab, rows), (unsigned)across);
         cudaError_t e = cudaSuccess;
@@ -486,9 +503,10 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
             // (whole warps: a zeroing block votes)
             e = asca_launch_after(ctx, embed_pieces_kernel<wd(), T>, dim3((unsigned)(a.sums + a.zeros)), block, (size_t)block.y * place, a);
             const dim3 wide = asca_row_block(frags, 256);
+            const int64_t each = std::min<int64_t>(MOST_JOINED, ceil_div64(pieces, ctx->sm_count * 8));   // (most pieces have no work)
             if (e == cudaSuccess && pieces > 1)
-                e = asca_launch_after(ctx, embed_join_kernel<wd()>, dim3((unsigned)(pieces - 1)), wide,
-                                      wide.y > 1 ? (size_t)wide.x * wide.y * 4 * frag<wd(), float>::E : 0, a);
+                e = asca_launch_after(ctx, embed_join_kernel<wd()>, dim3((unsigned)ceil_div64(pieces, each)), wide,
+                                      wide.y > 1 ? (size_t)wide.x * wide.y * 4 * frag<wd(), float>::E : 0, a, (int)each);
         });
     });
     ASCA_CUDA(ctx, e);

@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(256) unsort_rows_kernel(const TS* __restrict__
     }
 }
 
-// The KS assignments of a token share one reading of d_out's row; d_w (nullable) is a sum over it. d_ys may be ys.
+// The KS assignments of a token share one reading of d_out's row; d_w (nullable) is a sum over it. d_ys may be ys. LANES = 256: few tokens
+// of wide rows, a CTA each.
 template <int W, int LANES, int KS, typename TX, typename TS>
 __global__ void __launch_bounds__(256) unsort_rows_bwd_kernel(const TX* __restrict__ d_out, const TS* ys, const int32_t* __restrict__ slot,
                                                               const float* __restrict__ weights, int64_t N, int K, int d, TS* d_ys,
@@ -144,7 +145,16 @@ __global__ void __launch_bounds__(256) unsort_rows_bwd_kernel(const TX* __restri
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
 #pragma unroll
-                    for (int o = LANES / 2; o > 0; o >>= 1) dot[i][j] += __shfl_xor_sync(0xffffffffu, dot[i][j], o);
+                    for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) dot[i][j] += __shfl_xor_sync(0xffffffffu, dot[i][j], o);
+                    if constexpr (LANES == 256) {
+                        __shared__ float sums[8];
+                        if (lane % 32 == 0) sums[lane / 32] = dot[i][j];
+                        __syncthreads();
+                        dot[i][j] = 0.0f;
+#pragma unroll
+                        for (int w = 0; w < 8; ++w) dot[i][j] += sums[w];
+                        __syncthreads();
+                    }
                     if (t0 + i < N && lane == 0 && k0 + j < K) d_w[(t0 + i) * K + k0 + j] = s[i][j] >= 0 ? dot[i][j] : 0.0f;
                 }
             }
@@ -152,15 +162,17 @@ __global__ void __launch_bounds__(256) unsort_rows_bwd_kernel(const TX* __restri
     }
 }
 
-// f(lanes that own a token, assignments they take at a time, blocks of N tokens)
+// f(lanes that own a token, assignments they take at a time, blocks of N tokens); wide: a CTA may own a token
 template <typename F>
-inline void with_team(int64_t frags, int64_t N, int64_t K, F f) {
-    asca_with_lanes(frags, [&](auto l) {
+inline void with_team(const asca_ctx* ctx, int64_t frags, int64_t N, int64_t K, bool wide, F f) {
+    auto with = [&](auto l) {
         auto go = [&](auto ks) { f(l, ks, ceil_div64(N, 256 / l() * (PAIRS / ks()))); };
         if (K == 1) go(std::integral_constant<int, 1>());
         else if (K <= 3) go(std::integral_constant<int, 2>());
         else go(std::integral_constant<int, 4>());
-    });
+    };
+    if (wide && frags > 32 && N <= ctx->sm_count) with(std::integral_constant<int, 256>());
+    else asca_with_lanes(frags, with);
 }
 
 int check_rows(asca_ctx* ctx, const char* who, int64_t N, int64_t K, int64_t d, int tok_dtype, int row_dtype) {
@@ -237,7 +249,7 @@ int asca_moe_unsort_rows(asca_ctx* ctx, const void* ys, const int32_t* slot, con
             using TS = std::remove_const_t<std::remove_pointer_t<decltype(a)>>;
             using TX = std::remove_pointer_t<decltype(b)>;
             asca_with_width<TX, TS>(v, [&](auto w) {
-                with_team(frags, N, K, [&](auto l, auto ks, int64_t blocks) {
+                with_team(ctx, frags, N, K, false, [&](auto l, auto ks, int64_t blocks) {
                     const dim3 grid((unsigned)blocks, asca_column_blocks(ctx, blocks, frags, l()));
                     unsort_rows_kernel<w(), l(), ks(), TS, TX><<<grid, 256, 0, ctx->stream>>>(a, slot, weights, N, (int)K, (int)d, b);
                 });
@@ -267,7 +279,7 @@ int asca_moe_unsort_rows_bwd(asca_ctx* ctx, const void* d_out, const void* ys, c
             using TX = std::remove_const_t<std::remove_pointer_t<decltype(a)>>;
             using TS = std::remove_pointer_t<decltype(b)>;
             asca_with_width<TX, TS>(v, [&](auto w) {
-                with_team(frags, N, K, [&](auto l, auto ks, int64_t blocks) {
+                with_team(ctx, frags, N, K, true, [&](auto l, auto ks, int64_t blocks) {
                     unsort_rows_bwd_kernel<w(), l(), ks(), TX, TS><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a, static_cast<const TS*>(ys), slot, weights, N,
                                                                                                               (int)K, (int)d, b, d_w);
                 });

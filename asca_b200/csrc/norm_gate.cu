@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(MOST, 2048 / MOST) join_fwd_kernel(const Join 
         for (int j = 0; j < EPT; ++j) y[j] = y[j] * r1 * w[j];
     }
     if (a.gate) {
-        ld_cols<FOUR>(a.gate + r / a.gate_rows * cols, team, tid, cols, w);
+        ld_cols<FOUR>(a.gate + (int64_t)((uint32_t)r / (uint32_t)a.gate_rows) * cols, team, tid, cols, w);
 #pragma unroll
         for (int j = 0; j < EPT; ++j) y[j] *= w[j];
     }
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
 #pragma unroll
         for (int j = 0; j < EPT / 2; ++j) w_pre[j] = pair(t[2 * j], t[2 * j + 1]);
     }
-    int64_t group = r0 / a.gate_rows, first = group * a.gate_rows, end = first + min(a.gate_rows, a.rows - first);
+    int64_t group = (uint32_t)r0 / (uint32_t)a.gate_rows, first = group * a.gate_rows, end = first + min(a.gate_rows, a.rows - first);
     auto set_u = [&](const float (&gate)[EPT], const float (&w)[EPT]) {   // branch gate w_post
 #pragma unroll
         for (int j = 0; j < EPT / 2; ++j)
@@ -450,46 +450,51 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
     }
 }
 
-// Adds what the strips left: blockIdx.y = 0, 1 the gains over all CTAs; behind them a gate's groups that reach over several strips.
-// A block owns eight columns (a 32-byte sector of every part), 128 lanes a column, each every 128th part.
-constexpr int SUM_COLS = 8;
-__global__ void __launch_bounds__(1024) join_sums_kernel(const Join a, int ctas) {
-    __shared__ float sh[32][SUM_COLS];
+// Adds what the strips left: blockIdx.y = 0, 1 the gains over all CTAs; behind them a gate's groups that reach over several strips,
+// as many of them a block as leave each 2^lanes_log lanes. A block owns eight columns (a 32-byte sector of every part), 128 lanes a column,
+// each of which takes every so many-th part.
+constexpr int SUM_COLS = 8, SUM_LANES = 128;
+__global__ void __launch_bounds__(SUM_COLS * SUM_LANES) join_sums_kernel(const Join a, int ctas, uint32_t lanes_log) {
+    __shared__ float sh[SUM_LANES / 4][SUM_COLS];   // [warp]
     pdl_wait();
     const int c = blockIdx.x * SUM_COLS + threadIdx.x % SUM_COLS, y = threadIdx.x / SUM_COLS, w = threadIdx.x >> 5, lane = threadIdx.x & 31, cols = a.cols;
-    constexpr int LANES = 1024 / SUM_COLS;
-    float* out;
+    const bool gains = blockIdx.y < 2;
+    if (gains && !(blockIdx.y == 0 ? a.d_w_pre : a.d_w_post)) return;
+    const uint32_t log = gains ? 7 : lanes_log, per = 1u << log, rows = (uint32_t)a.rows, gate_rows = (uint32_t)a.gate_rows, strip = (uint32_t)a.strip;
+    const uint32_t group0 = (blockIdx.y - 2) << (7 - log);
+    static_assert(SUM_LANES == 1 << 7, "lanes are powers of two");
     float v = 0.0f;
-    if (blockIdx.y < 2) {
-        out = blockIdx.y == 0 ? a.d_w_pre : a.d_w_post;
-        if (!out) return;
+    if (gains) {
         if (c < cols) {
 #pragma unroll 8
-            for (int i = y; i < ctas; i += LANES) v += a.part_w[(2 * (int64_t)i + blockIdx.y) * cols + c];
+            for (int i = y; i < ctas; i += SUM_LANES) v += a.part_w[(2 * (int64_t)i + blockIdx.y) * cols + c];
         }
     } else {
-        const int64_t group = blockIdx.y - 2, first = group * a.gate_rows, end = min(first + a.gate_rows, a.rows);
-        const int64_t s0 = first / a.strip, s1 = (end - 1) / a.strip;
-        if (s0 == s1) return;   // (written by the strip)
-        out = a.d_gate + group * cols;
-        if (c < cols) {
-            // the group begins in its first strip, whose sum goes to the right, and comes into the others from the left
-            if (y == 0) v = a.part_g[(2 * s0 + 1) * cols + c];
+        const uint64_t first = (uint64_t)(group0 + (y >> log)) * gate_rows;   // (32-bit divisions below: rows are)
+        if (first < rows) {
+            const uint32_t end = min(gate_rows, rows - (uint32_t)first) + (uint32_t)first, s0 = (uint32_t)first / strip, s1 = (end - 1) / strip, k = y & (per - 1);
+            if (s0 < s1 && c < cols) {   // (a group in one strip: written there)
+                // the group begins in its first strip, whose sum goes to the right, and comes into the others from the left
+                if (k == 0) v = a.part_g[(2 * (int64_t)s0 + 1) * cols + c];
 #pragma unroll 8
-            for (int64_t i = s0 + 1 + y; i <= s1; i += LANES) v += a.part_g[2 * i * cols + c];
+                for (uint32_t i = s0 + 1 + k; i <= s1; i += per) v += a.part_g[2 * (int64_t)i * cols + c];
+            }
         }
     }
     v += __shfl_xor_sync(0xffffffffu, v, 8);
     v += __shfl_xor_sync(0xffffffffu, v, 16);
     if (lane < SUM_COLS) sh[w][lane] = v;
     __syncthreads();
-    if (w > 0) return;
+    if (y >= SUM_LANES >> log || c >= cols) return;
+    float* out = gains ? (blockIdx.y == 0 ? a.d_w_pre : a.d_w_post) : a.d_gate + (int64_t)(group0 + y) * cols;
+    if (!gains) {
+        const uint64_t first = (uint64_t)(group0 + y) * gate_rows;
+        if (first >= rows || (uint32_t)first / strip == (min(gate_rows, rows - (uint32_t)first) + (uint32_t)first - 1) / strip) return;
+    }
     v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v += sh[lane / SUM_COLS * 8 + i][lane % SUM_COLS];
-    v += __shfl_xor_sync(0xffffffffu, v, 8);
-    v += __shfl_xor_sync(0xffffffffu, v, 16);
-    if (lane < SUM_COLS && c < cols) out[c] = a.accumulate ? out[c] + v : v;
+#pragma unroll 8
+    for (uint32_t i = 0; i < per / 4; ++i) v += sh[y * (per / 4) + i][threadIdx.x % SUM_COLS];
+    out[c] = a.accumulate ? out[c] + v : v;
 }
 
 // Lanes of a warp that make a team (0: a team is a CTA), and the team's threads.
@@ -582,6 +587,7 @@ int asca_gated_residual_rmsnorm_fwd(asca_ctx* ctx, const void* y, const float* x
     ASCA_TRY(check(ctx, "gated_residual_rmsnorm_fwd", a, cols, dtype));
     if (rows == 0) return ASCA_OK;
     ASCA_REQUIRE(ctx, y && x && x_out, "gated_residual_rmsnorm_fwd: null pointer");
+    a.gate_rows = std::min(gate_rows, rows);   // (32 bits)
     asca_device_scope on(ctx);
     const bool four = asca_rows_by(4, y, cols, dtype) && asca_rows_by(4, xn, cols, dtype) && asca_aligned(x, 16) && asca_aligned(x_out, 16) &&
                       asca_aligned(w_post, 16) && asca_aligned(gate, 16) && asca_aligned(w_pre, 16);
@@ -615,6 +621,7 @@ int asca_gated_residual_rmsnorm_bwd(asca_ctx* ctx, const void* y, const float* x
         return ASCA_OK;
     }
     ASCA_REQUIRE(ctx, y && x_out && d_x && d_y && ws, "%s: null pointer", who);
+    a.gate_rows = std::min(a.gate_rows, rows);   // (32 bits)
     const Strips s(ctx, rows, cols, d_gate ? a.gate_rows : 0);
     ASCA_REQUIRE(ctx, asca_aligned(ws, 256) && ws_bytes >= (size_t)asca_gated_residual_rmsnorm_bwd_ws(ctx, rows, cols),
                  "%s: the workspace has to have asca_gated_residual_rmsnorm_bwd_ws bytes, 256-byte aligned", who);
@@ -628,8 +635,11 @@ int asca_gated_residual_rmsnorm_bwd(asca_ctx* ctx, const void* y, const float* x
     ASCA_TRY(launch<Bwd>(ctx, a, dtype, four, s.strips));
     const bool gates = d_gate && a.gate_rows > s.strip;   // (else every group lies in one strip)
     if (d_w_post || d_w_pre || gates) {
-        const int64_t groups = gates ? ceil_div64(rows, a.gate_rows) : 0;
-        ASCA_CUDA(ctx, asca_launch_after(ctx, join_sums_kernel, dim3((unsigned)ceil_div64(cols, SUM_COLS), (unsigned)(2 + groups)), dim3(1024), 0, a, (int)s.ctas));
+        const int64_t groups = gates ? ceil_div64(rows, a.gate_rows) : 0, strips = gates ? ceil_div64(a.gate_rows, s.strip) : 1;   // a group's
+        uint32_t log = 2;
+        while (log < 7 && (1 << log) < strips) ++log;
+        const dim3 grid((unsigned)ceil_div64(cols, SUM_COLS), (unsigned)(2 + ceil_div64(groups, SUM_LANES >> log)));
+        ASCA_CUDA(ctx, asca_launch_after(ctx, join_sums_kernel, grid, dim3(SUM_COLS * SUM_LANES), 0, a, (int)s.ctas, log));
         ctx->launches++;
     }
     return ASCA_OK;

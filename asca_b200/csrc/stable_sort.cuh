@@ -188,6 +188,13 @@ __device__ __forceinline__ void put_items(const Job& j, int pass, const Items& t
 
 inline size_t smem_bytes(int threads, int bins) { return (size_t)bins * 8 + (size_t)threads / 32 * bins * 2; }
 
+// n floats of zeros, by threads `me` of `step`.
+__device__ __forceinline__ void clear_floats(float* p, int64_t n, int64_t me, int64_t step) {
+    const int64_t head = min(n, (int64_t)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / 4)), four = (n - head) / 4, rest = n - four * 4;
+    for (int64_t i = me; i < four; i += step) st4(p + head + 4 * i, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+    if (me < rest) p[me < head ? me : me + four * 4] = 0.0f;   // (at most six)
+}
+
 // f(std::integral_constant of 256, 512 or 1024): the threads that n items keep busy, four each
 template <typename F>
 inline void with_threads(int64_t n, F f) {
