@@ -184,8 +184,9 @@ __global__ void __launch_bounds__(128) embed_pieces_kernel(const Sum a) {
     }
 }
 
-// A block owns `pieces` pieces; it has work where a run begins in one of them and goes on past it. Its lanes beside each other
-// (threadIdx.y) take the run's pieces in turn, eight of them in flight.
+// A block owns `pieces` pieces; it has work where a run begins in one of them and goes on past it. A run that comes into up to AHEAD
+// further pieces is added up by one thread a column (a block has blockDim.y of them beside each other, each at its own run); for a
+// longer one those beside each other take its pieces in turn, eight of them in flight.
 constexpr int MOST_JOINED = 32;
 template <int W>
 __global__ void __launch_bounds__(256) embed_join_kernel(const Sum a, int pieces) {
@@ -193,19 +194,56 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const Sum a, int pieces
     constexpr int E = F::E;
     extern __shared__ uint32_t sh_raw[];
     float(*sh)[E] = reinterpret_cast<float(*)[E]>(sh_raw);   // [lane beside][column lane]
-    __shared__ bool begins[MOST_JOINED];
+    __shared__ int comes_into[MOST_JOINED];   // further pieces of the run that begins in a piece; AHEAD + 1: more than AHEAD
+    __shared__ uint32_t keys[MOST_JOINED];
     const int piece = a.piece, d = a.d, lanes = blockDim.x, beside = blockDim.y, threads = lanes * beside, me = threadIdx.y * lanes + threadIdx.x;
     pdl_wait();
     const int64_t p0 = (int64_t)blockIdx.x * pieces;
     for (int i = me; i < pieces; i += threads) {
         const int64_t p = p0 + i, end = (p + 1) * piece;
-        begins[i] = end < a.N && a.keys[end - 1] < a.vocab && a.keys[end] == a.keys[end - 1] &&
-                    !(p > 0 && a.keys[p * piece - 1] == a.keys[end - 1]);   // (the last: it began further left)
+        int more = 0;
+        if (end < a.N) {
+            const uint32_t key = a.keys[end - 1], left = p > 0 ? a.keys[p * piece - 1] : 0xffffffffu;   // (left the same: it began there)
+            uint32_t at[AHEAD + 1];
+#pragma unroll
+            for (int u = 0; u <= AHEAD; ++u) at[u] = end + (int64_t)u * piece < a.N ? a.keys[end + (int64_t)u * piece] : 0xffffffffu;
+            if (key < a.vocab && left != key) {
+#pragma unroll
+                for (int u = 0; u <= AHEAD; ++u) more += at[u] == key;   // (sorted: they are the first ones)
+            }
+            keys[i] = key;
+        }
+        comes_into[i] = more;
     }
     __syncthreads();
-    for (int64_t p = p0; p < p0 + pieces; ++p) {
-        if (!begins[p - p0]) continue;
-        const uint32_t key = a.keys[(p + 1) * piece - 1];
+    const auto add = [](const F& r, float (&acc)[E]) {
+        float v[E];
+        r.get(v);
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[j] += v[j];
+    };
+    for (int i = threadIdx.y; i < pieces; i += beside) {
+        const int more = comes_into[i];
+        if (more == 0 || more > AHEAD) continue;
+        const int64_t p = p0 + i;
+        for (int c = frag_first<W>(threadIdx.x); c < d; c += lanes * E) {
+            F first, r[AHEAD];
+            float acc[E] = {};
+            first.load(a.part + (2 * p + 1) * d, c, lanes, d);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+                if (u < more) r[u].load(a.part + 2 * (p + 1 + u) * d, c, lanes, d);
+            add(first, acc);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+                if (u < more) add(r[u], acc);
+            add_row<W>(a.d_table + (int64_t)keys[i] * d, c, lanes, d, acc, a.scale, a.accumulate);
+        }
+    }
+    for (int i = 0; i < pieces; ++i) {
+        if (comes_into[i] <= AHEAD) continue;
+        const int64_t p = p0 + i;
+        const uint32_t key = keys[i];
         int64_t more = 0;   // pieces that the run comes into from the left
         for (;; more += threads) {
             const int64_t q = p + 1 + more + me;
@@ -217,17 +255,11 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const Sum a, int pieces
         }
         for (int c = frag_first<W>(threadIdx.x); c - frag_first<W>(threadIdx.x) < d; c += lanes * E) {   // (the same turns for all)
             float acc[E] = {};
-            auto add = [&](const F& r) {
-                float v[E];
-                r.get(v);
-#pragma unroll
-                for (int j = 0; j < E; ++j) acc[j] += v[j];
-            };
             if (c < d) {
                 F r[AHEAD];
                 if (threadIdx.y == 0) {
                     r[0].load(a.part + (2 * p + 1) * d, c, lanes, d);
-                    add(r[0]);
+                    add(r[0], acc);
                 }
                 for (int64_t q0 = threadIdx.y; q0 < more; q0 += (int64_t)AHEAD * beside) {
 #pragma unroll
@@ -235,7 +267,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const Sum a, int pieces
                         if (q0 + u * beside < more) r[u].load(a.part + 2 * (p + 1 + q0 + u * beside) * d, c, lanes, d);
 #pragma unroll
                     for (int u = 0; u < AHEAD; ++u)
-                        if (q0 + u * beside < more) add(r[u]);
+                        if (q0 + u * beside < more) add(r[u], acc);
                 }
             }
             if (beside > 1) {
@@ -243,9 +275,10 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const Sum a, int pieces
                 for (int j = 0; j < E; ++j) sh[me][j] = acc[j];
                 __syncthreads();
                 if (threadIdx.y == 0) {
-                    for (int i = 1; i < beside; ++i) {
+#pragma unroll 8
+                    for (int y = 1; y < beside; ++y) {
 #pragma unroll
-                        for (int j = 0; j < E; ++j) acc[j] += sh[i * lanes + threadIdx.x][j];
+                        for (int j = 0; j < E; ++j) acc[j] += sh[y * lanes + threadIdx.x][j];
                     }
                 }
                 __syncthreads();

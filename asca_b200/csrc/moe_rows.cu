@@ -48,17 +48,21 @@ __global__ void __launch_bounds__(256) sort_rows_kernel(const TX* __restrict__ x
     }
 }
 
-// unsort and its gradient: LANES lanes own PAIRS / KS tokens, KS assignments of each at a time: PAIRS rows of the sorted side in flight.
+// unsort and its gradient: some lanes own PAIRS / KS tokens, KS assignments of each at a time: PAIRS rows of the sorted side in flight.
 constexpr int PAIRS = 4;
 
-// weights null: every weight is one. Few tokens: blocks beside each other (blockIdx.y) share the columns.
-template <int W, int LANES, int KS, typename TS, typename TX>
+// weights null: every weight is one. K = 1: up to 256 lanes a token, so that a block goes over four rows from end to end, which HBM
+// likes better than eight warps each at four rows of their own (16,000 x 4096 f32: 88 us, 159 by warps); with several assignments a
+// warp's tokens lie close together anyway, and a bf16 row would leave wide blocks lanes (32,768 x 2 x 2048 bf16: 90 us by warps, 99).
+// Few tokens: blocks beside each other (blockIdx.y) share the columns.
+template <int W, int KS, typename TS, typename TX>
 __global__ void __launch_bounds__(256) unsort_rows_kernel(const TS* __restrict__ ys, const int32_t* __restrict__ slot, const float* __restrict__ weights,
                                                           int64_t N, int K, int d, TX* __restrict__ out) {
     using F = frag<W, TS>;
     constexpr int T = PAIRS / KS;
-    const int64_t t0 = ((int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES) * T;
-    for (int c = blockIdx.y * LANES * F::E + frag_first<W>(threadIdx.x % LANES); c < d; c += gridDim.y * LANES * F::E) {
+    const int lanes = blockDim.x;
+    const int64_t t0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * T;
+    for (int c = blockIdx.y * lanes * F::E + frag_first<W>(threadIdx.x); c < d; c += gridDim.y * lanes * F::E) {
         float acc[T][F::E] = {};
         for (int k0 = 0; k0 < K; k0 += KS) {
             F r[T][KS];
@@ -70,7 +74,7 @@ __global__ void __launch_bounds__(256) unsort_rows_kernel(const TS* __restrict__
                 for (int j = 0; j < KS; ++j) {
                     s[i][j] = t0 + i < N && k0 + j < K ? slot[(t0 + i) * K + k0 + j] : -1;
                     w[i][j] = s[i][j] >= 0 && weights ? weights[(t0 + i) * K + k0 + j] : 1.0f;
-                    if (s[i][j] >= 0) r[i][j].load(ys + (int64_t)s[i][j] * d, c, LANES, d);
+                    if (s[i][j] >= 0) r[i][j].load(ys + (int64_t)s[i][j] * d, c, lanes, d);
                 }
             }
 #pragma unroll
@@ -87,12 +91,13 @@ __global__ void __launch_bounds__(256) unsort_rows_kernel(const TS* __restrict__
         }
 #pragma unroll
         for (int i = 0; i < T; ++i)
-            if (t0 + i < N) frag<W, TX>::put(out + (t0 + i) * d, c, LANES, d, acc[i]);
+            if (t0 + i < N) frag<W, TX>::put(out + (t0 + i) * d, c, lanes, d, acc[i]);
     }
 }
 
-// The KS assignments of a token share one reading of d_out's row; d_w (nullable) is a sum over it. d_ys may be ys. LANES = 256: few tokens
-// of wide rows, a CTA each.
+// The KS assignments of a token share one reading of d_out's row; d_w (nullable) is a sum over it. d_ys may be ys. LANES = 256: a CTA
+// a token, or four with K = 1, where tokens are too few to fill the SMs by warps (500 x 2 x 2048: 4.1 us, 10.4 by warps) or a single
+// assignment's row is long (16,000 x 4096 f32: 120 us, 141 by warps; 512 groups of eight bf16: 88 and 85).
 template <int W, int LANES, int KS, typename TX, typename TS>
 __global__ void __launch_bounds__(256) unsort_rows_bwd_kernel(const TX* __restrict__ d_out, const TS* ys, const int32_t* __restrict__ slot,
                                                               const float* __restrict__ weights, int64_t N, int K, int d, TS* d_ys,
@@ -162,17 +167,12 @@ __global__ void __launch_bounds__(256) unsort_rows_bwd_kernel(const TX* __restri
     }
 }
 
-// f(lanes that own a token, assignments they take at a time, blocks of N tokens); wide: a CTA may own a token
+// f(assignments of a token that are taken at a time)
 template <typename F>
-inline void with_team(const asca_ctx* ctx, int64_t frags, int64_t N, int64_t K, bool wide, F f) {
-    auto with = [&](auto l) {
-        auto go = [&](auto ks) { f(l, ks, ceil_div64(N, 256 / l() * (PAIRS / ks()))); };
-        if (K == 1) go(std::integral_constant<int, 1>());
-        else if (K <= 3) go(std::integral_constant<int, 2>());
-        else go(std::integral_constant<int, 4>());
-    };
-    if (wide && frags > 32 && N <= ctx->sm_count) with(std::integral_constant<int, 256>());
-    else asca_with_lanes(frags, with);
+inline void with_assignments(int64_t K, F f) {
+    if (K == 1) f(std::integral_constant<int, 1>());
+    else if (K == 2) f(std::integral_constant<int, 2>());
+    else f(std::integral_constant<int, 4>());
 }
 
 int check_rows(asca_ctx* ctx, const char* who, int64_t N, int64_t K, int64_t d, int tok_dtype, int row_dtype) {
@@ -249,9 +249,11 @@ int asca_moe_unsort_rows(asca_ctx* ctx, const void* ys, const int32_t* slot, con
             using TS = std::remove_const_t<std::remove_pointer_t<decltype(a)>>;
             using TX = std::remove_pointer_t<decltype(b)>;
             asca_with_width<TX, TS>(v, [&](auto w) {
-                with_team(ctx, frags, N, K, false, [&](auto l, auto ks, int64_t blocks) {
-                    const dim3 grid((unsigned)blocks, asca_column_blocks(ctx, blocks, frags, l()));
-                    unsort_rows_kernel<w(), l(), ks(), TS, TX><<<grid, 256, 0, ctx->stream>>>(a, slot, weights, N, (int)K, (int)d, b);
+                with_assignments(K, [&](auto ks) {
+                    const dim3 block = asca_row_block(ks() == 1 ? frags : std::min<int64_t>(frags, 32), 256);
+                    const int64_t blocks = ceil_div64(N, (int64_t)block.y * (PAIRS / ks()));
+                    const dim3 grid((unsigned)blocks, asca_column_blocks(ctx, blocks, frags, block.x));
+                    unsort_rows_kernel<w(), ks(), TS, TX><<<grid, block, 0, ctx->stream>>>(a, slot, weights, N, (int)K, (int)d, b);
                 });
             });
         });
@@ -279,9 +281,14 @@ int asca_moe_unsort_rows_bwd(asca_ctx* ctx, const void* d_out, const void* ys, c
             using TX = std::remove_const_t<std::remove_pointer_t<decltype(a)>>;
             using TS = std::remove_pointer_t<decltype(b)>;
             asca_with_width<TX, TS>(v, [&](auto w) {
-                with_team(ctx, frags, N, K, true, [&](auto l, auto ks, int64_t blocks) {
-                    unsort_rows_bwd_kernel<w(), l(), ks(), TX, TS><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a, static_cast<const TS*>(ys), slot, weights, N,
-                                                                                                              (int)K, (int)d, b, d_w);
+                with_assignments(K, [&](auto ks) {
+                    auto by = [&](auto l) {
+                        const unsigned blocks = (unsigned)ceil_div64(N, 256 / l() * (PAIRS / ks()));
+                        unsort_rows_bwd_kernel<w(), l(), ks(), TX, TS><<<blocks, 256, 0, ctx->stream>>>(a, static_cast<const TS*>(ys), slot, weights, N,
+                                                                                                        (int)K, (int)d, b, d_w);
+                    };
+                    if ((frags > 32 && N <= 8 * ctx->sm_count) || (ks() == 1 && w() < 8 && frags >= 512)) by(std::integral_constant<int, 256>());
+                    else asca_with_lanes(frags, by);
                 });
             });
         });

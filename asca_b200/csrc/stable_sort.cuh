@@ -2,11 +2,13 @@
 //
 // Up to 4,096 items: one CTA does all passes in one launch. More: two launches a pass, a CTA to a tile of 2,048 items -- the first
 // counts the tile's digits, the second adds up what the tiles in front of its own counted and places its items; where that table has
-// more than 65,536 entries, a launch between the two scans it once instead of every CTA for itself.
+// more than 16,384 entries, a launch between the two scans it once instead of every CTA for itself (200,000 ids of 50,000 in two passes
+// and their rows' sums: 48.6 us, 59.1 each for itself; where the table has 4,160 entries the launch costs 0.7 us more than it saves).
 // In both, a warp owns a run of consecutive items; a ballot for every bit of the digit gives a lane its rank among equal digits of its 32
 // (match_any, which goes over the distinct digits one by one, takes longer where they are many), a counter per warp and digit what
 // came before them in the run, a scan over the warps what came before the warp. The rank is by construction the order
-// of the items, so the result is the same in every run. Bound by launches and the latency of a pass's steps, not by bytes.
+// of the items, so the result is the same in every run. Bound by launches and the latency of a pass's steps, not by bytes:
+// 8,192 items 6.8 us, 131,072 7.4, two million 27.
 #pragma once
 #include "common.cuh"
 #include "row_io.cuh"
@@ -17,7 +19,7 @@ namespace stable_sort {
 
 constexpr int PER = 4;                           // items a lane
 constexpr int SMALL = 1024 * PER, TILE = 512 * PER;
-constexpr int64_t OWN_SCAN = 65536;              // entries of the table that every CTA may add up for itself
+constexpr int64_t OWN_SCAN = 16384;              // entries of the table that every CTA may add up for itself
 constexpr int MAX_BINS = 2049;
 
 // Item i of the first pass has key min(ids[i], limit): everything at or past `limit`, as unsigned, is one key. Pass p writes keys[p & 1]
@@ -33,7 +35,8 @@ struct Job {
 };
 
 inline int64_t tiles(int64_t n) { return ceil_div64(n, TILE); }
-inline size_t scratch_bytes(int64_t n, int bins) { return n <= SMALL ? 0 : ((size_t)tiles(n) * bins * 4 + 255) & ~(size_t)255; }
+// the table, and the totals of scan_kernel
+inline size_t scratch_bytes(int64_t n, int bins) { return n <= SMALL ? 0 : ((size_t)(tiles(n) + 1) * bins * 4 + 255) & ~(size_t)255; }
 
 #ifdef __CUDACC__
 __device__ __forceinline__ uint32_t mask_of(const Job& j) { return j.passes > 1 ? (1u << j.digit) - 1 : 0xffffffffu; }
@@ -240,38 +243,57 @@ static __global__ void __launch_bounds__(512) count_kernel(const Job j, int pass
     for (int b = threadIdx.x; b < j.bins; b += 512) counts[(int64_t)blockIdx.x * j.bins + b] = sh[b];
 }
 
-// counts[tile][bin] -> the first place of the tile's items of the bin; one CTA, a thread a bin.
+// counts[tile][bin] -> how many items of the bin the tiles in front have; totals[bin]. A CTA owns eight bins (a 32-byte sector of every
+// tile's row), 128 lanes a bin, four tiles a lane in a round.
+constexpr int SCAN_BINS = 8;
 static __global__ void __launch_bounds__(1024) scan_kernel(const Job j, int32_t* __restrict__ counts, int n_tiles) {
-    __shared__ int32_t wsum[32];
+    __shared__ int32_t sums[32][SCAN_BINS], all[SCAN_BINS];   // of a warp's tiles, then of the warps in front
     pdl_wait();
     pdl_launch_dependents();
-    for (int b0 = 0, carry = 0; b0 < j.bins; b0 += 1024) {
-        const int b = b0 + threadIdx.x;
-        int32_t* column = counts + b;
-        auto each = [&](auto f) {   // sixteen tiles' entries in flight
-            if (b >= j.bins) return;
-            for (int t0 = 0; t0 < n_tiles; t0 += 16) {
-                int c[16];
+    const int b = blockIdx.x * SCAN_BINS + threadIdx.x % SCAN_BINS, lane = threadIdx.x / SCAN_BINS, w = threadIdx.x >> 5, x = threadIdx.x & 31;
+    int carry = 0;
+    for (int t0 = 0; t0 < n_tiles; t0 += 512) {
+        int c[4], s = 0;
 #pragma unroll
-                for (int u = 0; u < 16; ++u) c[u] = t0 + u < n_tiles ? column[(int64_t)(t0 + u) * j.bins] : 0;
+        for (int u = 0; u < 4; ++u) {
+            const int t = t0 + lane * 4 + u;
+            c[u] = t < n_tiles && b < j.bins ? counts[(int64_t)t * j.bins + b] : 0;
+            s += c[u];
+        }
+        int inc = s;
 #pragma unroll
-                for (int u = 0; u < 16; ++u)
-                    if (t0 + u < n_tiles) f(t0 + u, c[u]);
+        for (int o = SCAN_BINS; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (x >= o) inc += y;
+        }
+        if (x >= 32 - SCAN_BINS) sums[w][x % SCAN_BINS] = inc;
+        __syncthreads();
+        if (w < SCAN_BINS) {   // a warp a bin
+            const int v = sums[x][w];
+            int y = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int z = __shfl_up_sync(0xffffffffu, y, o);
+                if (x >= o) y += z;
             }
-        };
-        int all = 0, total;
-        each([&](int, int c) { all += c; });
-        int at = carry + exclusive_scan<1024>(all, wsum, total);
-        carry += total;
-        if (b < j.bins && j.offsets) j.offsets[b] = at;
-        each([&](int t, int c) {
-            column[(int64_t)t * j.bins] = at;
-            at += c;
-        });
+            sums[x][w] = y - v;
+            if (x == 31) all[w] = y;
+        }
+        __syncthreads();
+        int at = carry + sums[w][x % SCAN_BINS] + inc - s;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int t = t0 + lane * 4 + u;
+            if (t < n_tiles && b < j.bins) counts[(int64_t)t * j.bins + b] = at;
+            at += c[u];
+        }
+        carry += all[x % SCAN_BINS];
+        __syncthreads();   // (written again)
     }
+    if (lane == 0 && b < j.bins) counts[(int64_t)n_tiles * j.bins + b] = carry;
 }
 
-// SCANNED: the table holds first places (scan_kernel); otherwise counts, which the CTA adds up: 512 / Q bins at a time, Q threads a bin.
+// SCANNED: the table holds what scan_kernel leaves; otherwise counts, which the CTA adds up: 512 / Q bins at a time, Q threads a bin.
 // The items are put in order inside the tile first, so that what goes out together goes to neighbouring places.
 template <bool SCANNED>
 static __global__ void __launch_bounds__(512) place_kernel(const Job j, int pass, const int32_t* __restrict__ table, int n_tiles, int q_log) {
@@ -288,7 +310,16 @@ static __global__ void __launch_bounds__(512) place_kernel(const Job j, int pass
     Items t;
     load_items(j, pass, (int64_t)mine * TILE + (threadIdx.x >> 5) * PER * 32, PER, t);
     if (SCANNED) {
-        for (int b = threadIdx.x; b < j.bins; b += 512) first[b] = table[(int64_t)mine * j.bins + b];
+        for (int b0 = 0, carry = 0; b0 < j.bins; b0 += 512) {
+            const int b = b0 + threadIdx.x, all = b < j.bins ? table[(int64_t)n_tiles * j.bins + b] : 0;
+            const int before = b < j.bins ? table[(int64_t)mine * j.bins + b] : 0;
+            int total;
+            const int at = carry + exclusive_scan<512>(all, wsum, total);
+            carry += total;
+            if (b >= j.bins) continue;
+            first[b] = at + before;
+            if (j.offsets && mine == 0) j.offsets[b] = at;
+        }
     } else {
         const int q = 1 << q_log, lane = threadIdx.x & (q - 1);
         for (int b0 = 0, carry = 0; b0 < j.bins; b0 += 512 >> q_log) {
@@ -374,7 +405,7 @@ static inline int sort(asca_ctx* ctx, const Job& j, int32_t* table) {
     for (int p = 0; p < j.passes; ++p) {
         if (p == 0) count_kernel<<<(unsigned)n, 512, (size_t)j.bins * 4, ctx->stream>>>(j, p, table);
         else ASCA_CUDA(ctx, asca_launch_after(ctx, count_kernel, dim3(n), dim3(512), (size_t)j.bins * 4, j, p, table));
-        if (scanned) ASCA_CUDA(ctx, asca_launch_after(ctx, scan_kernel, dim3(1), dim3(1024), 0, j, table, n));
+        if (scanned) ASCA_CUDA(ctx, asca_launch_after(ctx, scan_kernel, dim3((unsigned)ceil_div64(j.bins, SCAN_BINS)), dim3(1024), 0, j, table, n));
         ASCA_CUDA(ctx, asca_launch_after(ctx, scanned ? place_kernel<true> : place_kernel<false>, dim3(n), dim3(512), smem, j, p, (const int32_t*)table, n, q_log));
         ctx->launches += scanned ? 3 : 2;
     }

@@ -65,6 +65,7 @@ EMBED = [  # N, V, d, ids
     (1, 1, 1, "one"), (1, 256, 64, "zipf"), (12, 256, 768, "zipf"), (63, 300, 7, "zipf"), (64, 64, 32, "one"), (65, 70, 33, "distinct"),
     (777, 5, 130, "zipf"), (2048, 256, 64, "zipf"), (2049, 2047, 36, "past"), (5000, 70_001, 20, "zipf"), (4096, 4_200_000, 1, "zipf"),
     (129, 100, 1030, "one"), (40_000, 3, 12, "zipf"), (300, 1000, 8, "padding"), (140_000, 50_000, 4, "zipf"),
+    (1_100_000, 70_000, 2, "zipf"), (9000, 40, 1032, "zipf"), (20_000, 900, 40, "zipf"),
 ]
 
 
@@ -266,7 +267,8 @@ def test_gated_residual_of_zeros_and_of_what_is_no_number(gpu):
 # ------------------------------------------------------------------ rows by expert
 MOE = [  # N, K, E, d
     (1, 1, 1, 1), (1, 2, 16, 768), (12, 2, 16, 768), (33, 8, 8, 31), (500, 3, 5, 64), (1500, 2, 8, 192), (2048, 1, 64, 36), (2049, 4, 255, 20), (700, 5, 256, 17),
-    (900, 2, 2048, 8), (40_000, 8, 128, 4), (3, 6, 7, 1028),
+    (900, 2, 2048, 8), (40_000, 8, 128, 4), (3, 6, 7, 1028), (1_060_000, 1, 40, 1), (30_000, 3, 2048, 5), (1300, 1, 4, 2048),
+    (1190, 3, 5, 264),
 ]
 
 
