@@ -2,6 +2,7 @@
 // row gather / scatter, AdamW.
 // Every reduction is a fixed tree (no float atomics), so results are run-to-run identical.
 #include "common.cuh"
+#include "row_io.cuh"
 
 #include <cuda_bf16.h>
 
@@ -498,6 +499,7 @@ int asca_adamw_segmented_clip(asca_ctx* ctx, float* p, const float* g, float* m,
                               void* p_bf16, const float* norm, float max_norm) {
     if (!ctx) return ASCA_ERR_ARG;
     ASCA_REQUIRE(ctx, norm && max_norm > 0.0f && std::isfinite(max_norm), "adamw_segmented_clip: needs the norm and a positive, finite largest one");
+    asca_device_scope on(ctx);
     return adamw_segmented(ctx, p, g, m, v, seg_off, lr_t, eps_t, n_seg, beta1, beta2, wd_eff, p_bf16, norm, max_norm);
 }
 

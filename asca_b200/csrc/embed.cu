@@ -442,6 +442,8 @@ int asca_embed_scaled_fwd(asca_ctx* ctx, const void* table, const uint32_t* ids,
     if (N == 0) return ASCA_OK;
     ASCA_REQUIRE(ctx, table && ids && x, "embed_scaled_fwd: null pointer");
     ASCA_REQUIRE(ctx, N < ((int64_t)1 << 31), "embed_scaled_fwd: at most 2^31 - 1 tokens");
+    const asca_span_of out(x, N * d, asca_dtype_size(out_dtype));
+    ASCA_REQUIRE(ctx, asca_apart(out, {table, vocab * d, asca_dtype_size(table_dtype)}) && asca_apart(out, {ids, N, 4}), "embed_scaled_fwd: x lies over an input");
     asca_device_scope on(ctx);
     const int v = asca_row_width(d, table, table_dtype, x, out_dtype);
     const int64_t frags = asca_row_frags(d, v);
@@ -480,6 +482,8 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
         return ASCA_OK;
     }
     ASCA_REQUIRE(ctx, dx && ids, "embed_scaled_bwd: null pointer");
+    const asca_span_of out(d_table, vocab * d, 4);
+    ASCA_REQUIRE(ctx, asca_apart(out, {dx, N * d, asca_dtype_size(dtype)}) && asca_apart(out, {ids, N, 4}), "embed_scaled_bwd: d_table lies over an input");
     const Plan plan(N, d, vocab);
     ASCA_REQUIRE(ctx, asca_aligned(ws, 256) && ws_bytes >= plan.bytes() && (ws || ws_bytes == 0), "embed_scaled_bwd: the workspace has to have asca_embed_scaled_bwd_ws bytes, 256-byte aligned");
     const int v = asca_row_width(d, dx, dtype, d_table, ASCA_F32);

@@ -3,6 +3,7 @@
 // rust/src/model.rs:631-802 and rust/src/delta.rs:121-207 / :615-674, composed from the
 // library's own entry points with every activation resident in HBM. f32 arithmetic.
 #include "common.cuh"
+#include "row_io.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -1587,6 +1588,7 @@ static int model_grad_norm(asca_ctx* ctx, asca_model* m, const char* who) {
     if (m->dp) return asca_fail(ctx, ASCA_ERR_UNSUPPORTED, "%s: not with a communicator attached", who);
     ASCA_TRY(materialize_zero_grads(ctx, m));
     const size_t ws = (size_t)asca_grad_norm_ws(ctx, 1);
+    asca_device_scope on(ctx);
     if (!m->norm && cudaMalloc((void**)&m->norm, 256 + ws) != cudaSuccess) {
         m->norm = nullptr;
         cudaGetLastError();

@@ -24,6 +24,7 @@ __global__ void __launch_bounds__(256) sort_rows_kernel(const TX* __restrict__ x
                                                         TS* __restrict__ xs) {
     using F = frag<W, TX>;
     const int lanes = blockDim.x;
+    const uint32_t rows = (uint32_t)N * (uint32_t)K;
     const int64_t t0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * TOKENS;
     for (int c = frag_first<W>(threadIdx.x); c < d; c += lanes * F::E) {
         F r[TOKENS];
@@ -35,7 +36,7 @@ __global__ void __launch_bounds__(256) sort_rows_kernel(const TX* __restrict__ x
             if (t0 + i >= N) break;
             for (int k = 0; k < K; ++k) {
                 const int32_t s = slot[(t0 + i) * K + k];
-                if (s < 0) continue;
+                if ((uint32_t)s >= rows) continue;
                 TS* p = xs + (int64_t)s * d;
                 if constexpr (std::is_same_v<TX, TS>) r[i].store(p, c, lanes, d);   // bit for bit
                 else {
@@ -50,6 +51,12 @@ __global__ void __launch_bounds__(256) sort_rows_kernel(const TX* __restrict__ x
 
 // unsort and its gradient: some lanes own PAIRS / KS tokens, KS assignments of each at a time: PAIRS rows of the sorted side in flight.
 constexpr int PAIRS = 4;
+
+// The place of an assignment's row, -1: nowhere (an assignment that is none, or a place that there is not).
+__device__ __forceinline__ int32_t slot_of(const int32_t* __restrict__ slot, int64_t t, int k, int64_t N, int K) {
+    const int32_t s = t < N && k < K ? slot[t * K + k] : -1;
+    return (uint32_t)s < (uint32_t)N * (uint32_t)K ? s : -1;
+}
 
 // weights null: every weight is one. K = 1: up to 256 lanes a token, so that a block goes over four rows from end to end, which HBM
 // likes better than eight warps each at four rows of their own (16,000 x 4096 f32: 88 us, 159 by warps); with several assignments a
@@ -72,7 +79,7 @@ __global__ void __launch_bounds__(256) unsort_rows_kernel(const TS* __restrict__
             for (int i = 0; i < T; ++i) {
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
-                    s[i][j] = t0 + i < N && k0 + j < K ? slot[(t0 + i) * K + k0 + j] : -1;
+                    s[i][j] = slot_of(slot, t0 + i, k0 + j, N, K);
                     w[i][j] = s[i][j] >= 0 && weights ? weights[(t0 + i) * K + k0 + j] : 1.0f;
                     if (s[i][j] >= 0) r[i][j].load(ys + (int64_t)s[i][j] * d, c, lanes, d);
                 }
@@ -112,7 +119,7 @@ __global__ void __launch_bounds__(256) unsort_rows_bwd_kernel(const TX* __restri
         for (int i = 0; i < T; ++i) {
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
-                s[i][j] = t0 + i < N && k0 + j < K ? slot[(t0 + i) * K + k0 + j] : -1;
+                s[i][j] = slot_of(slot, t0 + i, k0 + j, N, K);
                 w[i][j] = s[i][j] >= 0 && weights ? weights[(t0 + i) * K + k0 + j] : 1.0f;
             }
         }
@@ -186,7 +193,7 @@ int check_rows(asca_ctx* ctx, const char* who, int64_t N, int64_t K, int64_t d, 
 extern "C" {
 
 int64_t asca_moe_topk_dispatch_ws(int64_t N, int64_t K, int64_t E) {
-    if (N < 0 || K <= 0 || E <= 0 || E + 1 > stable_sort::MAX_BINS) return ASCA_ERR_ARG;
+    if (N < 0 || K <= 0 || K >= (1 << 16) || N >= ((int64_t)1 << 31) / K || E <= 0 || E + 1 > stable_sort::MAX_BINS) return ASCA_ERR_ARG;
     return (int64_t)stable_sort::scratch_bytes(N * K, (int)E + 1);   // (few assignments: none)
 }
 
@@ -202,6 +209,9 @@ int asca_moe_topk_dispatch(asca_ctx* ctx, const int32_t* experts, int64_t N, int
         return ASCA_OK;
     }
     ASCA_REQUIRE(ctx, experts && perm && slot, "moe_topk_dispatch: null pointer");
+    const asca_span_of in(experts, N * K, 4), out[3] = {{perm, N * K, 4}, {offsets, E + 1, 4}, {slot, N * K, 4}};
+    for (int i = 0; i < 3; ++i)
+        ASCA_REQUIRE(ctx, asca_apart(out[i], in) && asca_apart(out[i], out[(i + 1) % 3]), "moe_topk_dispatch: an output lies over an input or another output");
     ASCA_REQUIRE(ctx, asca_aligned(ws, 256) && ws_bytes >= (size_t)asca_moe_topk_dispatch_ws(N, K, E) && (ws || ws_bytes == 0),
                  "moe_topk_dispatch: the workspace has to have asca_moe_topk_dispatch_ws bytes, 256-byte aligned");
     stable_sort::Job j{};
@@ -221,6 +231,8 @@ int asca_moe_sort_rows(asca_ctx* ctx, const void* x, const int32_t* slot, int64_
     ASCA_TRY(check_rows(ctx, "moe_sort_rows", N, K, d, x_dtype, xs_dtype));
     if (N == 0) return ASCA_OK;
     ASCA_REQUIRE(ctx, x && slot && xs, "moe_sort_rows: null pointer");
+    const asca_span_of out(xs, N * K * d, asca_dtype_size(xs_dtype));
+    ASCA_REQUIRE(ctx, asca_apart(out, {x, N * d, asca_dtype_size(x_dtype)}) && asca_apart(out, {slot, N * K, 4}), "moe_sort_rows: xs lies over an input");
     asca_device_scope on(ctx);
     const int v = asca_row_width(d, x, x_dtype, xs, xs_dtype);
     const dim3 block = asca_row_block(asca_row_frags(d, v), 256), grid((unsigned)ceil_div64(N, (int64_t)block.y * TOKENS));
@@ -241,6 +253,9 @@ int asca_moe_unsort_rows(asca_ctx* ctx, const void* ys, const int32_t* slot, con
     ASCA_TRY(check_rows(ctx, "moe_unsort_rows", N, K, d, out_dtype, ys_dtype));
     if (N == 0) return ASCA_OK;
     ASCA_REQUIRE(ctx, ys && slot && out, "moe_unsort_rows: null pointer");
+    const asca_span_of to(out, N * d, asca_dtype_size(out_dtype));
+    ASCA_REQUIRE(ctx, asca_apart(to, {ys, N * K * d, asca_dtype_size(ys_dtype)}) && asca_apart(to, {slot, N * K, 4}) && asca_apart(to, {weights, N * K, 4}),
+                 "moe_unsort_rows: out lies over an input");
     asca_device_scope on(ctx);
     const int v = asca_row_width(d, ys, ys_dtype, out, out_dtype);
     const int64_t frags = asca_row_frags(d, v);
@@ -273,6 +288,11 @@ int asca_moe_unsort_rows_bwd(asca_ctx* ctx, const void* d_out, const void* ys, c
     if (N == 0) return ASCA_OK;
     ASCA_REQUIRE(ctx, d_out && slot && d_ys, "moe_unsort_rows_bwd: null pointer");
     ASCA_REQUIRE(ctx, !d_w || ys, "moe_unsort_rows_bwd: the weights' gradient needs ys");
+    const asca_span_of g(d_out, N * d, asca_dtype_size(out_dtype)), rows(d_w ? ys : nullptr, N * K * d, asca_dtype_size(ys_dtype)), at(slot, N * K, 4),
+        w(weights, N * K, 4), to(d_ys, N * K * d, asca_dtype_size(ys_dtype)), to_w(d_w, N * K, 4);
+    ASCA_REQUIRE(ctx, asca_in_place(to, rows) && asca_apart(to, g) && asca_apart(to, at) && asca_apart(to, w) && asca_apart(to, to_w) && asca_apart(to_w, g) &&
+                          asca_apart(to_w, rows) && asca_apart(to_w, at) && asca_apart(to_w, w),
+                 "moe_unsort_rows_bwd: an output lies over an input (d_ys may be ys) or the other output");
     asca_device_scope on(ctx);
     const int v = std::min(asca_row_width(d, d_out, out_dtype, ys, ys_dtype), asca_row_width(d, d_out, out_dtype, d_ys, ys_dtype));
     const int64_t frags = asca_row_frags(d, v);

@@ -588,6 +588,15 @@ int asca_gated_residual_rmsnorm_fwd(asca_ctx* ctx, const void* y, const float* x
     if (rows == 0) return ASCA_OK;
     ASCA_REQUIRE(ctx, y && x && x_out, "gated_residual_rmsnorm_fwd: null pointer");
     a.gate_rows = std::min(gate_rows, rows);   // (32 bits)
+    const int64_t n = rows * cols;
+    const size_t size = asca_dtype_size(dtype);
+    const asca_span_of in[2] = {{y, n, size}, {x, n, 4}}, out[2] = {{x_out, n, 4}, {xn, n, size}};
+    const asca_span_of par[3] = {{w_post, cols, 4}, {gate, ceil_div64(rows, std::max<int64_t>(a.gate_rows, 1)) * cols, 4}, {w_pre, cols, 4}};
+    for (const auto& o : out) {
+        for (const auto& i : in) ASCA_REQUIRE(ctx, asca_in_place(o, i), "gated_residual_rmsnorm_fwd: an output lies over an input");
+        for (const auto& i : par) ASCA_REQUIRE(ctx, asca_apart(o, i), "gated_residual_rmsnorm_fwd: an output lies over a gain or gate");
+    }
+    ASCA_REQUIRE(ctx, asca_apart(out[0], out[1]), "gated_residual_rmsnorm_fwd: x_out and xn overlap");
     asca_device_scope on(ctx);
     const bool four = asca_rows_by(4, y, cols, dtype) && asca_rows_by(4, xn, cols, dtype) && asca_aligned(x, 16) && asca_aligned(x_out, 16) &&
                       asca_aligned(w_post, 16) && asca_aligned(gate, 16) && asca_aligned(w_pre, 16);
@@ -625,6 +634,16 @@ int asca_gated_residual_rmsnorm_bwd(asca_ctx* ctx, const void* y, const float* x
     const Strips s(ctx, rows, cols, d_gate ? a.gate_rows : 0);
     ASCA_REQUIRE(ctx, asca_aligned(ws, 256) && ws_bytes >= (size_t)asca_gated_residual_rmsnorm_bwd_ws(ctx, rows, cols),
                  "%s: the workspace has to have asca_gated_residual_rmsnorm_bwd_ws bytes, 256-byte aligned", who);
+    const int64_t n = rows * cols, groups_all = ceil_div64(rows, a.gate_rows);
+    const size_t size = asca_dtype_size(dtype);
+    const asca_span_of in[4] = {{y, n, size}, {x_out, n, 4}, {d_xn, n, size}, {d_out, n, 4}};
+    const asca_span_of par[3] = {{w_post, cols, 4}, {gate, groups_all * cols, 4}, {w_pre, cols, 4}};
+    const asca_span_of out[5] = {{d_x, n, 4}, {d_y, n, size}, {d_w_post, cols, 4}, {d_w_pre, cols, 4}, {d_gate, groups_all * cols, 4}};
+    for (int o = 0; o < 5; ++o) {
+        for (const auto& i : in) ASCA_REQUIRE(ctx, asca_in_place(out[o], i), "%s: an output lies over an input", who);
+        for (const auto& i : par) ASCA_REQUIRE(ctx, asca_apart(out[o], i), "%s: an output lies over a gain or gate", who);
+        for (int p = 0; p < o; ++p) ASCA_REQUIRE(ctx, asca_apart(out[o], out[p]), "%s: two outputs overlap", who);
+    }
     a.strip = s.strip;
     a.strips = s.strips;
     a.part_w = (float*)ws;

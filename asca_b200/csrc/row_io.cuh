@@ -25,6 +25,16 @@ inline bool asca_rows_by(int v, const void* p, int64_t cols, int dtype) {
     return cols % v == 0 && asca_aligned(p, v * asca_dtype_size(dtype));
 }
 
+// Memory that a call writes and other memory of it: apart, or (asca_in_place) the same elements in the same places, which is sound where
+// whoever writes an element has read it before.
+struct asca_span_of {
+    uintptr_t at;
+    size_t bytes;
+    asca_span_of(const void* p, int64_t n, size_t size) : at(reinterpret_cast<uintptr_t>(p)), bytes(p ? (size_t)n * size : 0) {}
+};
+inline bool asca_apart(const asca_span_of& a, const asca_span_of& b) { return a.at + a.bytes <= b.at || b.at + b.bytes <= a.at || !a.bytes || !b.bytes; }
+inline bool asca_in_place(const asca_span_of& a, const asca_span_of& b) { return (a.at == b.at && a.bytes == b.bytes) || asca_apart(a, b); }
+
 // f(pointer of the type that `dtype` names); a const pointer stays const
 template <typename F>
 inline void asca_with_dtype(const void* p, int dtype, F f) {

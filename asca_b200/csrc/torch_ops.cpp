@@ -24,6 +24,11 @@ namespace {
 
 struct Raised {};   // a Python error is set
 
+struct Ref {   // a reference of our own
+    PyObject* p;
+    ~Ref() { Py_XDECREF(p); }
+};
+
 [[noreturn]] void raise(PyObject* type, const char* fmt, ...) {
     char buf[512];
     va_list ap;
@@ -278,10 +283,9 @@ PyObject* join_bwd(Call& c) {   // y, x_out, d_xn, d_out, (join), grads
             sums[i] = c.make(of[i]->sizes(), F32);
             continue;
         }
-        PyObject* o = PyMapping_GetItemString(grads, names[i]);
-        if (!o) throw Raised{};
-        Py_DECREF(o);   // (the mapping holds it)
-        sums[i] = *c.as_tensor(o, names[i]);
+        const Ref o{PyMapping_GetItemString(grads, names[i])};
+        if (!o.p) throw Raised{};
+        sums[i] = *c.as_tensor(o.p, names[i]);
         typed(sums[i], names[i], F32);
         shaped(sums[i], names[i], of[i]->sizes());
         contiguous(sums[i], names[i]);
@@ -381,27 +385,21 @@ PyObject* moe_unsort_bwd(Call& c) {   // d_out, ys, slot, weights, d_ys
 
 // ------------------------------------------------------------------ gradient norm, clipping, AdamW
 struct List {
+    const Ref seq;   // (kept to the end of the call: tensors that only an iterator made live as long)
     std::vector<void*> p;
     std::vector<int64_t> n;
     std::vector<int> dtype;
-    explicit List(Call& c) {
-        PyObject* seq = PySequence_Fast(c.next(), "grads: expected a sequence of tensors");
-        if (!seq) throw Raised{};
-        const Py_ssize_t count = PySequence_Fast_GET_SIZE(seq);
+    explicit List(Call& c) : seq{PySequence_Fast(c.next(), "grads: expected a sequence of tensors")} {
+        if (!seq.p) throw Raised{};
+        const Py_ssize_t count = PySequence_Fast_GET_SIZE(seq.p);
         p.reserve(count), n.reserve(count), dtype.reserve(count);
-        try {
-            for (Py_ssize_t i = 0; i < count; ++i) {
-                const T& t = *c.as_tensor(PySequence_Fast_GET_ITEM(seq, i), "grads");
-                dtype.push_back(floating(t, "grads"));
-                contiguous(t, "grads");
-                p.push_back(t.data_ptr());
-                n.push_back(t.numel());
-            }
-        } catch (...) {
-            Py_DECREF(seq);
-            throw;
+        for (Py_ssize_t i = 0; i < count; ++i) {
+            const T& t = *c.as_tensor(PySequence_Fast_GET_ITEM(seq.p, i), "grads");
+            dtype.push_back(floating(t, "grads"));
+            contiguous(t, "grads");
+            p.push_back(t.data_ptr());
+            n.push_back(t.numel());
         }
-        Py_DECREF(seq);
     }
     int count() const { return (int)p.size(); }
 };

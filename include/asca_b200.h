@@ -137,7 +137,8 @@ int asca_residual_rmsnorm(asca_ctx* ctx, const float* x, const float* y, float* 
  * token. w_post, gate, w_pre nullable (ones); xn nullable (residual only); x_out may be x. cols <= 8192.
  * Backward, from d_xn (nullable) and d_out (nullable: the gradient that reaches x_out from further on; one of the two is
  * needed): d_x, d_y, and where their pointers are given d_w_post, d_gate, d_w_pre, which `accumulate` adds to instead of
- * overwriting. The sums over rows run in a fixed order. d_x may be d_out, d_y may be d_xn. ws: asca_gated_residual_rmsnorm_bwd_ws
+ * overwriting. The sums over rows run in a fixed order. d_x may be d_out, d_y may be d_xn (any
+ * output of both calls may take the place of an input of its size, element for element; other overlaps are refused). ws: asca_gated_residual_rmsnorm_bwd_ws
  * bytes of device scratch, 256-byte aligned, the caller's until the call's work has run. */
 int asca_gated_residual_rmsnorm_fwd(asca_ctx* ctx, const void* y, const float* x, const float* w_post, const float* gate,
                                     int64_t gate_rows, const float* w_pre, int post_norm, float skip_scale, float branch_scale,
@@ -360,6 +361,7 @@ int asca_moe_topk_dispatch(asca_ctx* ctx, const int32_t* experts, int64_t N, int
  *   asca_moe_unsort_rows      out[t] = sum_k weights[t,k] ys[slot[t,k]]      (weights nullable: ones)
  *   asca_moe_unsort_rows_bwd  d_ys[slot[t,k]] = weights[t,k] d_out[t]; d_w[t,k] = <d_out[t], ys[slot[t,k]]>, 0 where the
  *                             assignment goes nowhere (d_w nullable, ys then too; d_ys may be ys)
+ * A slot outside [0, N*K) goes nowhere. Outputs that lie over an input are refused, d_ys over ys apart.
  * The sorted rows with the identity as permutation are what asca_moe_fwd / asca_moe_bwd take as N*K tokens; d_b2 of the latter is a
  * sum over all N*K rows, so the rows of dout behind offsets[E] have to be zero there. */
 int asca_moe_sort_rows(asca_ctx* ctx, const void* x, const int32_t* slot, int64_t N, int64_t K, int64_t d, int x_dtype,

@@ -667,6 +667,98 @@ def test_refusals(gpu):
     assert torch.equal(ops.moe_unsort_rows(gpu, rand(1, 20, 8) * 0, slot), torch.zeros(10, 8, device="cuda"))   # the context is usable
 
 
+def test_outputs_over_inputs(gpu):
+    """In place where whoever writes an element has read it; refused elsewhere."""
+    n, d = 12, 16
+    buf, ids = rand(1, 4 * n * d), text(1, n, 8, "zipf")
+    part = lambda at, rows: buf[at:at + rows * d].view(rows, d)  # noqa: E731
+    _, _, slot = ops.moe_topk_dispatch(gpu, route(1, n, 1, 3, "any"), 3)
+    w = rand(2, n, 1)
+    refused = [
+        lambda: ops.embed_fwd(gpu, part(0, n), ids, out=part(d, n)),
+        lambda: ops.embed_bwd(gpu, part(0, n), ids, 8, d_table=part(5 * d, 8)),
+        lambda: ops.moe_sort_rows(gpu, part(0, n), slot, out=part(0, n)),
+        lambda: ops.moe_unsort_rows(gpu, part(0, n), slot, w, out=part(0, n)),
+        lambda: ops.moe_unsort_rows_bwd(gpu, part(0, n), part(n * d, n), slot, w, d_ys=part(0, n)),
+        lambda: ops.moe_unsort_rows_bwd(gpu, part(2 * n * d, n), part(0, n), slot, w, d_ys=part(d, n)),
+        lambda: ops.gated_residual_rmsnorm_fwd(gpu, part(0, n), part(n * d, n), x_out=part(n * d + 4, n)),
+        lambda: ops.gated_residual_rmsnorm_fwd(gpu, part(0, n), part(n * d, n), w_pre=buf[2 * n * d:][:d], x_out=part(2 * n * d, n)),
+    ]
+    gain, grad = rand(3, d), rand(4, d)   # one parameter in both places: its gradient would be added to by two sums at once
+    refused.append(lambda: ops.gated_residual_rmsnorm_bwd(gpu, part(0, n), part(n * d, n), part(2 * n * d, n), None, w_post=gain, w_pre=gain,
+                                                          grads={"d_w_post": grad, "d_w_pre": grad}))
+    before = buf.clone()
+    for call in refused:
+        with pytest.raises(asca_b200.AscaError) as err:
+            call()
+        assert err.value.code == -1
+    assert torch.equal(buf, before)
+    both = ops.gated_residual_rmsnorm_bwd(gpu, part(0, n), part(n * d, n), part(2 * n * d, n), None, w_post=gain, w_pre=gain)
+    y, x, d_xn = (part(i * n * d, n).clone() for i in range(3))
+    gpu._run("asca_gated_residual_rmsnorm_bwd", y.data_ptr(), x.data_ptr(), d_xn.data_ptr(), None, gain.data_ptr(), None, 0, gain.data_ptr(), 1, 1.0, 1.0, 1e-6,
+             n, d, asca_b200.F32, 0, x.data_ptr(), d_xn.data_ptr(), None, None, None,
+             (ws := torch.empty(gpu.lib.asca_gated_residual_rmsnorm_bwd_ws(gpu._ctx, n, d), dtype=torch.uint8, device="cuda")).data_ptr(), ws.numel())
+    assert torch.equal(x, both["d_x"]) and torch.equal(d_xn, both["d_y"])   # d_x over x_out, d_y over d_xn
+
+
+def test_slots_that_are_none(gpu):
+    slot = torch.tensor([[0, 99], [-7, 3], [1, 2]], dtype=torch.int32, device="cuda")   # six rows: 99 and -7 go nowhere
+    x, ys, w = rand(1, 3, 8), rand(2, 6, 8), rand(3, 3, 2)
+    xs = ops.moe_sort_rows(gpu, x, slot, out=torch.full((6, 8), 7.0, device="cuda"))
+    assert torch.equal(xs[:4], x[[0, 2, 2, 1]]) and (xs[4:] == 7).all()
+    out = ops.moe_unsort_rows(gpu, ys, slot, w)
+    assert torch.equal(out[0], w[0, 0] * ys[0]) and torch.equal(out[1], w[1, 1] * ys[3])
+    d_ys, d_w = ops.moe_unsort_rows_bwd(gpu, x, ys, slot, w, d_ys=torch.full((6, 8), 7.0, device="cuda"))
+    assert torch.equal(d_ys[0], w[0, 0] * x[0]) and (d_ys[4:] == 7).all() and d_w[0, 1] == 0 and d_w[1, 0] == 0
+
+
+def test_gradients_that_only_an_iterator_holds(gpu):
+    grads = tensors(1, [50_000] * 40, [torch.float32])
+    kept = [g * 2 for g in grads]
+    assert torch.equal(ops.grad_norm(gpu, (g * 2 for g in grads)), ops.grad_norm(gpu, kept))
+    norm = ops.clip_grads(gpu, iter(kept), 1.0)
+    within(kept[3], grads[3].double() * 2 / float(norm), (6 * U) * grads[3].double().abs() * 2 / float(norm) + 1e-6 * 2 * grads[3].double().abs() / float(norm) ** 2, "clipped")
+
+
+def test_matrices_of_more_than_2_31_elements(gpu):
+    """What the last rows get is what they get alone."""
+    cols, rows = 2048, (1 << 31) // 2048 + 70
+    last = slice(rows - 50, rows)
+    y = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda").normal_()
+    x = torch.empty(rows, cols, device="cuda").normal_()
+    kw = dict(w_post=rand(1, cols), w_pre=rand(2, cols), skip_scale=0.9, branch_scale=0.3)
+    alone = ops.gated_residual_rmsnorm_fwd(gpu, y[last], x[last].clone(), **kw)
+    x_out, xn = ops.gated_residual_rmsnorm_fwd(gpu, y, x, x_out=x, **kw)
+    assert torch.equal(x_out[last], alone[0]) and torch.equal(xn[last], alone[1])
+    got = ops.gated_residual_rmsnorm_bwd(gpu, y, x_out, xn, None, **kw)
+    want = ops.gated_residual_rmsnorm_bwd(gpu, y[last], x_out[last], xn[last], None, **kw)
+    assert torch.equal(got["d_x"][last], want["d_x"]) and torch.equal(got["d_y"][last], want["d_y"])
+    del x, x_out, got, want
+    # the same matrix as a table, as rows in expert order, and as rows of gradients
+    ids = torch.randint(rows - 40, rows, (33,), dtype=torch.int32, device="cuda")
+    assert torch.equal(ops.embed_fwd(gpu, y, ids), y[ids.long()])
+    experts = torch.zeros(rows, 1, dtype=torch.int32, device="cuda")
+    experts[:rows // 2] = 1
+    _, _, slot = ops.moe_topk_dispatch(gpu, experts, 2)
+    xs = ops.moe_sort_rows(gpu, y, slot, out=xn)
+    half = rows - rows // 2
+    assert torch.equal(xs[half:], y[:rows // 2]) and torch.equal(xs[:half], y[rows // 2:])
+    back = ops.moe_unsort_rows(gpu, xs, slot, out_dtype=torch.bfloat16)
+    assert torch.equal(back, y)
+    del back
+    d_ys, d_w = ops.moe_unsort_rows_bwd(gpu, y, xs, slot, torch.ones(rows, 1, device="cuda"), d_ys=xs)
+    assert torch.equal(d_ys[:half], y[rows // 2:])
+    square = (y[last].double() ** 2).sum(1)
+    within(d_w[last, 0], square, (cols + 2) * U * square, "d_w")
+    ids = torch.randint(0, 1000, (rows,), dtype=torch.int32, device="cuda")
+    ids[:-50] = -1   # (padding: nothing but the last rows is summed)
+    ids[-50:] = torch.arange(50, dtype=torch.int32, device="cuda")
+    assert torch.equal(ops.embed_bwd(gpu, y, ids, 1000)[:50], y[last].float())
+    norm = ops.grad_norm(gpu, [y])
+    want = float(torch.sqrt(sum((part.double() ** 2).sum() for part in y.split(1 << 17))))
+    assert abs(float(norm) - want) <= want * (U + 1e-10)
+
+
 def test_another_context_on_another_stream(gpu):
     other, stream = asca_b200.Gpu(0), torch.cuda.Stream()
     a, b = state_of(50), state_of(60)
