@@ -35,8 +35,8 @@ __global__ void __launch_bounds__(256) sort_rows_kernel(const TX* __restrict__ x
         for (int i = 0; i < TOKENS; ++i) {
             if (t0 + i >= N) break;
             for (int k = 0; k < K; ++k) {
-                const int32_t s = slot[(t0 + i) * K + k];
-                if ((uint32_t)s >= rows) continue;
+                const uint32_t s = slot[(t0 + i) * K + k];
+                if (s >= rows) continue;   // (nowhere)
                 TS* p = xs + (int64_t)s * d;
                 if constexpr (std::is_same_v<TX, TS>) r[i].store(p, c, lanes, d);   // bit for bit
                 else {
@@ -52,12 +52,6 @@ __global__ void __launch_bounds__(256) sort_rows_kernel(const TX* __restrict__ x
 // unsort and its gradient: some lanes own PAIRS / KS tokens, KS assignments of each at a time: PAIRS rows of the sorted side in flight.
 constexpr int PAIRS = 4;
 
-// The place of an assignment's row, -1: nowhere (an assignment that is none, or a place that there is not).
-__device__ __forceinline__ int32_t slot_of(const int32_t* __restrict__ slot, int64_t t, int k, int64_t N, int K) {
-    const int32_t s = t < N && k < K ? slot[t * K + k] : -1;
-    return (uint32_t)s < (uint32_t)N * (uint32_t)K ? s : -1;
-}
-
 // weights null: every weight is one. K = 1: up to 256 lanes a token, so that a block goes over four rows from end to end, which HBM
 // likes better than eight warps each at four rows of their own (16,000 x 4096 f32: 88 us, 159 by warps); with several assignments a
 // warp's tokens lie close together anyway, and a bf16 row would leave wide blocks lanes (32,768 x 2 x 2048 bf16: 90 us by warps, 99).
@@ -68,27 +62,28 @@ __global__ void __launch_bounds__(256) unsort_rows_kernel(const TS* __restrict__
     using F = frag<W, TS>;
     constexpr int T = PAIRS / KS;
     const int lanes = blockDim.x;
+    const uint32_t rows = (uint32_t)N * (uint32_t)K;
     const int64_t t0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * T;
     for (int c = blockIdx.y * lanes * F::E + frag_first<W>(threadIdx.x); c < d; c += gridDim.y * lanes * F::E) {
         float acc[T][F::E] = {};
         for (int k0 = 0; k0 < K; k0 += KS) {
             F r[T][KS];
             float w[T][KS];
-            int32_t s[T][KS];
+            uint32_t s[T][KS];
 #pragma unroll
             for (int i = 0; i < T; ++i) {
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
-                    s[i][j] = slot_of(slot, t0 + i, k0 + j, N, K);
-                    w[i][j] = s[i][j] >= 0 && weights ? weights[(t0 + i) * K + k0 + j] : 1.0f;
-                    if (s[i][j] >= 0) r[i][j].load(ys + (int64_t)s[i][j] * d, c, lanes, d);
+                    s[i][j] = t0 + i < N && k0 + j < K ? (uint32_t)slot[(t0 + i) * K + k0 + j] : ~0u;
+                    w[i][j] = s[i][j] < rows && weights ? weights[(t0 + i) * K + k0 + j] : 1.0f;
+                    r[i][j].load(ys + (int64_t)(s[i][j] < rows ? s[i][j] : 0) * d, c, lanes, d);
                 }
             }
 #pragma unroll
             for (int i = 0; i < T; ++i) {
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
-                    if (s[i][j] < 0) continue;   // (adds nothing, whatever its weight)
+                    if (s[i][j] >= rows) continue;   // (adds nothing, whatever its weight)
                     float v[F::E];
                     r[i][j].get(v);
 #pragma unroll
@@ -111,16 +106,17 @@ __global__ void __launch_bounds__(256) unsort_rows_bwd_kernel(const TX* __restri
                                                               float* __restrict__ d_w) {
     constexpr int T = PAIRS / KS, E = frag<W, TX>::E;
     const int lane = threadIdx.x % LANES;
+    const uint32_t rows = (uint32_t)N * (uint32_t)K;
     const int64_t t0 = ((int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES) * T;
     for (int k0 = 0; k0 < K; k0 += KS) {
-        int32_t s[T][KS];
+        uint32_t s[T][KS];
         float w[T][KS], dot[T][KS] = {};
 #pragma unroll
         for (int i = 0; i < T; ++i) {
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
-                s[i][j] = slot_of(slot, t0 + i, k0 + j, N, K);
-                w[i][j] = s[i][j] >= 0 && weights ? weights[(t0 + i) * K + k0 + j] : 1.0f;
+                s[i][j] = t0 + i < N && k0 + j < K ? (uint32_t)slot[(t0 + i) * K + k0 + j] : ~0u;
+                w[i][j] = s[i][j] < rows && weights ? weights[(t0 + i) * K + k0 + j] : 1.0f;
             }
         }
         for (int c = frag_first<W>(lane); c < d; c += LANES * E) {
@@ -128,18 +124,18 @@ __global__ void __launch_bounds__(256) unsort_rows_bwd_kernel(const TX* __restri
             frag<W, TS> ry[T][KS];
 #pragma unroll
             for (int i = 0; i < T; ++i) {
-                if (t0 + i < N) rg[i].load(d_out + (t0 + i) * d, c, LANES, d);
+                rg[i].load(d_out + min(t0 + i, N - 1) * d, c, LANES, d);
 #pragma unroll
                 for (int j = 0; j < KS; ++j)
-                    if (d_w && s[i][j] >= 0) ry[i][j].load(ys + (int64_t)s[i][j] * d, c, LANES, d);
+                    if (d_w) ry[i][j].load(ys + (int64_t)(s[i][j] < rows ? s[i][j] : 0) * d, c, LANES, d);
             }
 #pragma unroll
             for (int i = 0; i < T; ++i) {
                 float g[E];
-                if (t0 + i < N) rg[i].get(g);
+                rg[i].get(g);
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
-                    if (s[i][j] < 0) continue;
+                    if (s[i][j] >= rows) continue;
                     float y[E], o[E];
                     if (d_w) ry[i][j].get(y);
 #pragma unroll
@@ -167,7 +163,7 @@ __global__ void __launch_bounds__(256) unsort_rows_bwd_kernel(const TX* __restri
                         for (int w = 0; w < 8; ++w) dot[i][j] += sums[w];
                         __syncthreads();
                     }
-                    if (t0 + i < N && lane == 0 && k0 + j < K) d_w[(t0 + i) * K + k0 + j] = s[i][j] >= 0 ? dot[i][j] : 0.0f;
+                    if (t0 + i < N && lane == 0 && k0 + j < K) d_w[(t0 + i) * K + k0 + j] = s[i][j] < rows ? dot[i][j] : 0.0f;
                 }
             }
         }

@@ -553,18 +553,22 @@ def step_of(gpu, s):
     o["back"] = ops.moe_unsort_rows(gpu, o["xs"], o["slot"], s["weights"])
     o["d_ys"], o["d_w"] = ops.moe_unsort_rows_bwd(gpu, s["y"], o["xs"], o["slot"], s["weights"])
     o["norm"] = ops.grad_norm(gpu, [o["d_table"], o["d_x"], o["d_gate"]])
+    o["p"], o["m"], o["v"] = s["p"].clone(), torch.zeros_like(s["p"]), torch.zeros_like(s["p"])
+    ops.adamw_segmented(gpu, o["p"], o["d_table"], o["m"], o["v"], np.array([0, 500 * 200]), np.float32([1e-3]), np.float32([1e-8]), 0.9, 0.95, 0.0, norm=o["norm"],
+                        max_norm=1.0)
     s["out"] = o
 
 
-def state_of(seed):
-    n, d = 700, 200
-    return dict(table=rand(seed, 500, d), ids=text(seed, n, 500, "zipf"), x=rand(seed + 1, n, d), y=rand(seed + 2, n, d), gate=rand(seed + 3, 7, d), w=rand(seed + 4, d),
-                experts=route(seed, n, 2, 8, "any"), weights=rand(seed + 5, n, 2))
+def state_of(seed, n=700):
+    d = 200
+    return dict(table=rand(seed, 500, d), ids=text(seed, n, 500, "zipf"), x=rand(seed + 1, n, d), y=rand(seed + 2, n, d), gate=rand(seed + 3, n // 100, d), w=rand(seed + 4, d),
+                experts=route(seed, n, 2, 8, "any"), weights=rand(seed + 5, n, 2), p=rand(seed + 6, 500, d))
 
 
-def test_captured_and_replayed_beside_each_other(gpu):
+@pytest.mark.parametrize("n", [700, 9000])   # sorted in one launch, in several
+def test_captured_and_replayed_beside_each_other(gpu, n):
     """Two graphs of one context, replayed on two streams at once with new inputs: each has scratch of its own."""
-    states, graphs, streams = [state_of(10), state_of(20)], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    states, graphs, streams = [state_of(10, n), state_of(20, n)], [], [torch.cuda.Stream(), torch.cuda.Stream()]
     torch.cuda.synchronize()
     try:
         for s, stream in zip(states, streams):
@@ -578,7 +582,7 @@ def test_captured_and_replayed_beside_each_other(gpu):
                 graphs.append(graph)
         gpu.use_torch_stream()
         for seed in (30, 40):
-            fresh = [state_of(seed), state_of(seed + 5)]
+            fresh = [state_of(seed, n), state_of(seed + 5, n)]
             want = []
             for f in fresh:
                 step_of(gpu, f)
