@@ -8,9 +8,11 @@
 // order. The order is cut into pieces; a thread owns a few columns of a piece and walks down it with the running sum in registers,
 // and a run that lies inside its piece goes straight into the table. A run over several pieces leaves one partial sum a piece (at
 // most two of a piece belong to such runs: the one that comes in from the left and the one that goes on to the right), which a last
-// launch adds, eight lanes a column. Where the table is overwritten, blocks among the pieces' write the zeros of the rows that
-// no token has: every row of the table is written once. Nothing depends on the order in which blocks run. Bound by HBM: dx is read
-// once and the table written once; a scan of all ids for every row of the table, as asca_embed_bwd does it, reads N * V ids.
+// launch adds. Where the table is overwritten, the SMs that the sort leaves idle clear its first rows, and blocks among the
+// pieces' write the zeros of those behind that no token has. Nothing depends on the order in which blocks run. Bound by HBM
+// where the table is large: dx is read once and the table written once (32,768 ids, 48,000 x 2048, bf16 dx: 527 MB in 110 us =
+// 4.8 TB/s, of which the sort takes 17 us at little traffic); by the latency of six launches where it is not. A scan of all ids for
+// every row of the table, as asca_embed_bwd does it, reads N * V ids.
 #include "row_io.cuh"
 #include "stable_sort.cuh"
 
@@ -62,6 +64,9 @@ __device__ __forceinline__ void add_row(float* row, int c, int lanes, int d, con
 }
 
 constexpr int MOST_PIECE = 64, AHEAD = 8, ZERO_ROWS = 32;
+// Bytes of the table that a CTA beside a sort's tiles clears in each of its launches: about what it has time for. 32,768 ids, 48,000 x
+// 2048: 116 us with none, 112 with 128 KiB, 110 with 256, 114 with 512; 6728 ids, 52,608 x 319: 41, 31, 31, 31.
+constexpr int64_t FILL_SHARE = 256 << 10;
 
 struct Sum {
     const void* dx;
@@ -73,6 +78,7 @@ struct Sum {
     float scale;
     float *d_table, *part;
     int64_t sums, zeros;    // blocks of the two kinds; they take turns in the grid
+    int64_t cleared;        // rows of the table, from the first on, that the sort's launches clear
     bool narrow;            // rows of the table
 };
 
@@ -107,7 +113,7 @@ __device__ __forceinline__ int64_t warp_lower_bound(const uint32_t* keys, int64_
 template <int W>
 __device__ __forceinline__ void zero_rows(const Sum& a, int64_t block) {
     const int me = threadIdx.x + threadIdx.y * blockDim.x, threads = blockDim.x * blockDim.y, lane = me & 31;
-    const int64_t v0 = (a.narrow ? block * (threads >> 5) + (me >> 5) : block) * ZERO_ROWS;
+    const int64_t v0 = a.cleared + (a.narrow ? block * (threads >> 5) + (me >> 5) : block) * ZERO_ROWS;
     if (v0 >= a.vocab) return;
     const uint32_t rows = (uint32_t)min((int64_t)ZERO_ROWS, a.vocab - v0);
     // the rows' tokens lie in [lo, hi) of the sorted order: few are looked at one by one, many are looked for row by row
@@ -164,7 +170,7 @@ __global__ void __launch_bounds__(128) embed_pieces_kernel(const Sum a) {
         F r[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
-            if (i0 + u < n && key[i0 + u] < a.vocab) r[u].load(dx + (int64_t)item[i0 + u] * d, c, lanes, d);
+            r[u].load(dx + (int64_t)item[min(i0 + u, n - 1)] * d, c, lanes, d);
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int i = i0 + u;
@@ -508,7 +514,15 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
     a.part = (float*)(w + 4 * plan.list + plan.counts);
     a.sums = ceil_div64(pieces, block.y) * groups;
     a.narrow = d <= 256;
-    a.zeros = accumulate ? 0 : ceil_div64(vocab, a.narrow ? ZERO_ROWS * (int64_t)(block.x * block.y / 32) : ZERO_ROWS);
+    // What SMs the sort leaves idle clear a part of the table meanwhile, rows that have tokens among them (written over afterwards).
+    stable_sort::Fill fill;
+    if (!accumulate && !plan.small && N > stable_sort::SMALL && stable_sort::tiles(N) < ctx->sm_count) {
+        fill.ctas = (int)(ctx->sm_count - stable_sort::tiles(N));
+        a.cleared = std::min<int64_t>(vocab, fill.ctas * (FILL_SHARE / 4) * 2 * plan.passes / d);
+        fill.p = d_table;
+        fill.n = a.cleared * d;
+    }
+    a.zeros = accumulate ? 0 : ceil_div64(vocab - a.cleared, a.narrow ? ZERO_ROWS * (int64_t)(block.x * block.y / 32) : ZERO_ROWS);
     if (plan.small) {
         int lanes = 1;
         while (lanes < frags && lanes < 64) lanes *= 2;
@@ -532,7 +546,7 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
         return ASCA_OK;
     }
     ASCA_REQUIRE(ctx, a.sums + a.zeros < ((int64_t)1 << 31) && ceil_div64(frags, 32) <= 65535, "embed_scaled_bwd: too large");
-    ASCA_TRY(stable_sort::sort(ctx, j, (int32_t*)(w + 4 * plan.list)));
+    ASCA_TRY(stable_sort::sort(ctx, j, (int32_t*)(w + 4 * plan.list), fill));
     cudaError_t e = cudaSuccess;
     asca_with_dtype(dx, dtype, [&](auto src) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(src)>>;

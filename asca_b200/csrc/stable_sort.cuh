@@ -34,6 +34,14 @@ struct Job {
     int32_t *place, *offsets;     // of a single pass, nullable: where each item went, -1 for key `limit`; the first place of each bin
 };
 
+// Memory that the launches of a sort clear besides: `ctas` more CTAs in each of the two launches of a pass, an equal share a launch. (A sort
+// of more than SMALL items; one of fewer clears nothing.)
+struct Fill {
+    float* p = nullptr;
+    int64_t n = 0;
+    int ctas = 0;
+};
+
 inline int64_t tiles(int64_t n) { return ceil_div64(n, TILE); }
 // the table, and the totals of scan_kernel
 inline size_t scratch_bytes(int64_t n, int bins) { return n <= SMALL ? 0 : ((size_t)(tiles(n) + 1) * bins * 4 + 255) & ~(size_t)255; }
@@ -224,9 +232,18 @@ static __global__ void __launch_bounds__(THREADS) sort_small_kernel(const Job j)
     }
 }
 
+// (nothing in front of it on the stream but this sort's own launches, which do not touch that memory: no wait for them)
+__device__ __forceinline__ bool filled(const Fill& fill, int n_tiles) {
+    if ((int)blockIdx.x < n_tiles) return false;
+    pdl_launch_dependents();
+    clear_floats(fill.p, fill.n, (int64_t)(blockIdx.x - n_tiles) * blockDim.x + threadIdx.x, (int64_t)fill.ctas * blockDim.x);
+    return true;
+}
+
 // counts[tile][bin]
-static __global__ void __launch_bounds__(512) count_kernel(const Job j, int pass, int32_t* __restrict__ counts) {
+static __global__ void __launch_bounds__(512) count_kernel(const Job j, int pass, int32_t* __restrict__ counts, int n_tiles, const Fill fill) {
     extern __shared__ __align__(16) int32_t sh[];
+    if (filled(fill, n_tiles)) return;
     pdl_wait();
     pdl_launch_dependents();
     for (int b = threadIdx.x; b < j.bins; b += 512) sh[b] = 0;
@@ -296,13 +313,14 @@ static __global__ void __launch_bounds__(1024) scan_kernel(const Job j, int32_t*
 // SCANNED: the table holds what scan_kernel leaves; otherwise counts, which the CTA adds up: 512 / Q bins at a time, Q threads a bin.
 // The items are put in order inside the tile first, so that what goes out together goes to neighbouring places.
 template <bool SCANNED>
-static __global__ void __launch_bounds__(512) place_kernel(const Job j, int pass, const int32_t* __restrict__ table, int n_tiles, int q_log) {
+static __global__ void __launch_bounds__(512) place_kernel(const Job j, int pass, const int32_t* __restrict__ table, int n_tiles, int q_log, const Fill fill) {
     extern __shared__ __align__(16) int32_t sh[];   // first places [bin]; places inside the tile [bin]; the warps' counters
     __shared__ int32_t wsum[32];
     __shared__ uint32_t keys[TILE];
     __shared__ int32_t items[TILE];
     int32_t *first = sh, *inside = sh + j.bins;
     uint16_t *counts = reinterpret_cast<uint16_t*>(sh + 2 * j.bins), *run = counts + (threadIdx.x >> 5) * j.bins;
+    if (filled(fill, n_tiles)) return;
     const int mine = blockIdx.x, shift = pass * j.digit;
     const uint32_t mask = mask_of(j);
     pdl_wait();
@@ -380,7 +398,7 @@ static __global__ void __launch_bounds__(512) place_kernel(const Job j, int pass
 
 // Leaves the result in keys / items [(passes - 1) & 1]; table: scratch_bytes(n, bins) of scratch. Every kernel lets the next one's
 // launch begin early.
-static inline int sort(asca_ctx* ctx, const Job& j, int32_t* table) {
+static inline int sort(asca_ctx* ctx, const Job& j, int32_t* table, const Fill& fill = Fill()) {
     if (j.n <= SMALL) {
         cudaError_t e = cudaSuccess;
         with_threads(j.n, [&](auto threads) {
@@ -402,11 +420,16 @@ static inline int sort(asca_ctx* ctx, const Job& j, int32_t* table) {
         ASCA_CUDA(ctx, cudaFuncSetAttribute(place_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         ASCA_CUDA(ctx, cudaFuncSetAttribute(place_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     }
+    auto share = [&](int launch) {
+        const int64_t from = fill.n * launch / (2 * j.passes);
+        return Fill{fill.p + from, fill.n * (launch + 1) / (2 * j.passes) - from, fill.ctas};
+    };
+    const dim3 grid((unsigned)(n + fill.ctas));
     for (int p = 0; p < j.passes; ++p) {
-        if (p == 0) count_kernel<<<(unsigned)n, 512, (size_t)j.bins * 4, ctx->stream>>>(j, p, table);
-        else ASCA_CUDA(ctx, asca_launch_after(ctx, count_kernel, dim3(n), dim3(512), (size_t)j.bins * 4, j, p, table));
+        if (p == 0) count_kernel<<<grid, 512, (size_t)j.bins * 4, ctx->stream>>>(j, p, table, n, share(0));
+        else ASCA_CUDA(ctx, asca_launch_after(ctx, count_kernel, grid, dim3(512), (size_t)j.bins * 4, j, p, table, n, share(2 * p)));
         if (scanned) ASCA_CUDA(ctx, asca_launch_after(ctx, scan_kernel, dim3((unsigned)ceil_div64(j.bins, SCAN_BINS)), dim3(1024), 0, j, table, n));
-        ASCA_CUDA(ctx, asca_launch_after(ctx, scanned ? place_kernel<true> : place_kernel<false>, dim3(n), dim3(512), smem, j, p, (const int32_t*)table, n, q_log));
+        ASCA_CUDA(ctx, asca_launch_after(ctx, scanned ? place_kernel<true> : place_kernel<false>, grid, dim3(512), smem, j, p, (const int32_t*)table, n, q_log, share(2 * p + 1)));
         ctx->launches += scanned ? 3 : 2;
     }
     ASCA_CUDA(ctx, cudaGetLastError());
