@@ -18,22 +18,24 @@
 
 namespace {
 
-// LANES lanes own TOKENS tokens, all of whose rows they have in flight; where that leaves SMs without work, blocks beside each other
-// (blockIdx.y) share the columns.
-constexpr int TOKENS = 4;
-template <int W, int LANES, typename TT, typename TX>
+// Up to LANES lanes own TOKENS tokens, all of whose rows they have in flight (32,768 rows of 2048 bf16 from 48,000: 33.6 us with 32 lanes,
+// 30.9 with 64, 32.7 with 256; of f32: 66, 63, 61); where that leaves SMs without work, blocks beside each other (blockIdx.y)
+// share the columns.
+constexpr int TOKENS = 4, LANES = 64;
+template <int W, typename TT, typename TX>
 __global__ void __launch_bounds__(256) embed_scaled_fwd_kernel(const TT* __restrict__ table, const uint32_t* __restrict__ ids, int64_t N, int d,
                                                                uint32_t vocab, float scale, TX* __restrict__ x) {
     using F = frag<W, TT>;
-    const int64_t r0 = ((int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES) * TOKENS;
+    const int lanes = blockDim.x;
+    const int64_t r0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * TOKENS;
     uint32_t id[TOKENS];
 #pragma unroll
     for (int i = 0; i < TOKENS; ++i) id[i] = r0 + i < N ? ids[r0 + i] : 0xffffffffu;
-    for (int c = blockIdx.y * LANES * F::E + frag_first<W>(threadIdx.x % LANES); c < d; c += gridDim.y * LANES * F::E) {
+    for (int c = blockIdx.y * lanes * F::E + frag_first<W>(threadIdx.x); c < d; c += gridDim.y * lanes * F::E) {
         F r[TOKENS];
 #pragma unroll
         for (int i = 0; i < TOKENS; ++i)
-            if (id[i] < vocab) r[i].load(table + (int64_t)id[i] * d, c, LANES, d);
+            if (id[i] < vocab) r[i].load(table + (int64_t)id[i] * d, c, lanes, d);
 #pragma unroll
         for (int i = 0; i < TOKENS; ++i) {
             if (r0 + i >= N) break;
@@ -43,7 +45,7 @@ __global__ void __launch_bounds__(256) embed_scaled_fwd_kernel(const TT* __restr
 #pragma unroll
                 for (int j = 0; j < F::E; ++j) v[j] *= scale;
             }
-            frag<W, TX>::put(x + (r0 + i) * d, c, LANES, d, v);
+            frag<W, TX>::put(x + (r0 + i) * d, c, lanes, d, v);
         }
     }
 }
@@ -458,11 +460,10 @@ int asca_embed_scaled_fwd(asca_ctx* ctx, const void* table, const uint32_t* ids,
             using TT = std::remove_const_t<std::remove_pointer_t<decltype(tab)>>;
             using TX = std::remove_pointer_t<decltype(out)>;
             asca_with_width<TT, TX>(v, [&](auto w) {
-                asca_with_lanes(frags, [&](auto l) {
-                    const int64_t blocks = ceil_div64(N, 256 / l() * TOKENS);
-                    const dim3 grid((unsigned)blocks, asca_column_blocks(ctx, blocks, frags, l()));
-                    embed_scaled_fwd_kernel<w(), l(), TT, TX><<<grid, 256, 0, ctx->stream>>>(tab, ids, N, (int)d, (uint32_t)vocab, scale, out);
-                });
+                const dim3 block = asca_row_block(std::min<int64_t>(frags, LANES), 256);
+                const int64_t blocks = ceil_div64(N, (int64_t)block.y * TOKENS);
+                const dim3 grid((unsigned)blocks, asca_column_blocks(ctx, blocks, frags, block.x));
+                embed_scaled_fwd_kernel<w(), TT, TX><<<grid, block, 0, ctx->stream>>>(tab, ids, N, (int)d, (uint32_t)vocab, scale, out);
             });
         });
     });

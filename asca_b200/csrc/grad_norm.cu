@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(256) norm_parts_kernel(const __grid_constant__
 __global__ void __launch_bounds__(1024) norm_cluster_kernel(const __grid_constant__ Tensors t, float* __restrict__ norm) {
     __shared__ double red[32];
     __shared__ double mine;
+    pdl_wait();   // (the context may launch it early)
     const double s = squares(t, red);
     if (threadIdx.x == 0) mine = s;
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");

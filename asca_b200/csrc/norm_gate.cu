@@ -118,8 +118,9 @@ __device__ __forceinline__ float team_sum(float v, float (*red)[32], int& turn) 
     return v;
 }
 // Six sums. The first three steps halve what a lane has (it keeps the sums that three bits of its number name), so that six sums take
-// 7 shuffles and more where one takes 5; the way back to all lanes is one shuffle a sum.
-template <int LANES>
+// 7 shuffles and more where one takes 5; the way back to all lanes is one shuffle a sum. PAIR: the team is the two CTAs of a cluster, each
+// of which gets the other's warps' sums too, and the barrier is the cluster's.
+template <int LANES, bool PAIR>
 __device__ __forceinline__ void team_sums(float (&v)[6], float (*red)[32][8], int& turn) {
     constexpr int L = LANES ? LANES : 32;
     const int lane = threadIdx.x & 31;
@@ -140,10 +141,25 @@ __device__ __forceinline__ void team_sums(float (&v)[6], float (*red)[32][8], in
         // every warp adds the warps' sums: lane l those of its pair l % 4 and of every eighth warp from l / 4 on
         float(*r)[8] = red[turn];
         turn ^= 1;
-        if ((lane & 3) == 0) r[threadIdx.x >> 5][lane >> 2] = c;
-        __syncthreads();
+        int warps = blockDim.x >> 5, w0 = threadIdx.x >> 5;
+        if (PAIR) {
+            const uint32_t me = blockIdx.x & 1;
+            w0 += me * warps;
+            warps *= 2;
+            if ((lane & 3) == 0) {
+                float* to = &r[w0][lane >> 2];
+                uint32_t there;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(to)), "r"(me ^ 1u));
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(c) : "memory");
+                *to = c;
+            }
+            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        } else {
+            if ((lane & 3) == 0) r[w0][lane >> 2] = c;
+            __syncthreads();
+        }
         float2 s = make_float2(0.0f, 0.0f);
-        for (int w = lane >> 2; w < (int)(blockDim.x >> 5); w += 8) {
+        for (int w = lane >> 2; w < warps; w += 8) {
             const float2 x = *reinterpret_cast<const float2*>(&r[w][(lane & 3) * 2]);
             s.x += x.x; s.y += x.y;
         }
@@ -232,31 +248,32 @@ __device__ __forceinline__ void put_sum(float* p, int team, int tid, int cols, f
 // Rows ahead. A thread copies the columns that it will itself read (no barrier), asynchronously into its places in shared memory:
 // [stage][EPT columns][thread], a place of 16 bytes for four f32, 8 for four bf16, 4 for one f32. Single bf16 columns, which are too
 // small for such a copy, are read straight when their row's turn comes.
-// STAGES: rows in flight and in work, 0: every row is read straight.
-template <bool FOUR, int STAGES, typename T>
-constexpr bool ahead() { return STAGES > 0 && (FOUR || sizeof(T) == 4); }
+// STAGES: rows in flight and in work. Three fit twice into an SM up to 256 threads and once up to 512.
+constexpr int STAGES = 3;
+template <bool FOUR, typename T>
+constexpr bool ahead() { return FOUR || sizeof(T) == 4; }
 template <int BYTES>
 __device__ __forceinline__ void copy_ahead(uint32_t dst, const void* src) {
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 // place: of this thread's first columns; row: its first columns'
-template <bool FOUR, int STAGES, typename T>
+template <bool FOUR, typename T>
 __device__ __forceinline__ void ask_row(uint32_t place, const T* row, int team, int left) {
-    if constexpr (ahead<FOUR, STAGES, T>()) {
+    if constexpr (ahead<FOUR, T>()) {
         constexpr int V = FOUR ? 4 : 1;
 #pragma unroll
         for (int q = 0; q < EPT / V; ++q)
             if (q * team * V < left) copy_ahead<V * sizeof(T)>(place + q * blockDim.x * (uint32_t)(V * sizeof(T)), row + q * team * V);
     }
 }
-template <bool FOUR, int STAGES, typename T>
+template <bool FOUR, typename T>
 __device__ __forceinline__ void take_row(const T* place, const T* row, int team, int left, float (&v)[EPT]) {
     constexpr int V = FOUR ? 4 : 1;
 #pragma unroll
     for (int q = 0; q < EPT / V; ++q) {
         float t[V] = {};
-        if (q * team * V < left) ld_row<V>(ahead<FOUR, STAGES, T>() ? place + q * blockDim.x * V : row + q * team * V, t);
+        if (q * team * V < left) ld_row<V>(ahead<FOUR, T>() ? place + q * blockDim.x * V : row + q * team * V, t);
 #pragma unroll
         for (int i = 0; i < V; ++i) v[q * V + i] = t[i];
     }
@@ -267,14 +284,16 @@ constexpr size_t stage_bytes(int threads) { return (size_t)threads * EPT * (8 + 
 
 // EACH: every row has a gate of its own, which is asked for a row ahead. (In the other form that costs a shared gate 9 % of the pass;
 // without it a gate a row waits for its gate in every row: 351 us for 32,768 x 2048 where this form takes 297.)
-template <typename T, bool FOUR, int LANES, int MOST, int STAGES, bool EACH>
+template <typename T, bool FOUR, int LANES, int MOST, bool PAIR, bool EACH>
 __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(const Join a) {
     extern __shared__ __align__(16) char smem[];
+    pdl_wait();   // (the context may launch it early)
     pdl_launch_dependents();
     __shared__ __align__(16) float red[2][32][8];
     constexpr int L = LANES ? LANES : 1, TEAMS = LANES ? 256 / L : 1, V = FOUR ? 4 : 1;
-    const int team = LANES ? LANES : blockDim.x, tid = LANES ? threadIdx.x % L : threadIdx.x, cols = a.cols;
-    const int64_t s = (int64_t)blockIdx.x * TEAMS + (LANES ? threadIdx.x / L : 0);   // the strip
+    const int team = LANES ? LANES : PAIR ? 2 * blockDim.x : blockDim.x, cols = a.cols;
+    const int tid = LANES ? threadIdx.x % L : threadIdx.x + (PAIR ? (blockIdx.x & 1) * blockDim.x : 0);
+    const int64_t s = (int64_t)(PAIR ? blockIdx.x >> 1 : blockIdx.x) * TEAMS + (LANES ? threadIdx.x / L : 0);   // the strip
     const int64_t r0 = min(s * a.strip, a.rows), r1 = min(r0 + a.strip, a.rows);
     const int n = (int)(r1 - r0), left = cols - tid * V;   // columns from this thread's first one on
     int turn = 0;
@@ -290,11 +309,11 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
     auto ask = [&]() {
         if (asked < n) {
             const uint32_t p = mine32 + to * stage;
-            ask_row<FOUR, STAGES>(p, a.x_out + ask_at, team, left);
-            if (a.d_out) ask_row<FOUR, STAGES>(p + per * 4, a.d_out + ask_at, team, left);
+            ask_row<FOUR>(p, a.x_out + ask_at, team, left);
+            if (a.d_out) ask_row<FOUR>(p + per * 4, a.d_out + ask_at, team, left);
             const uint32_t t = half(p);
-            ask_row<FOUR, STAGES>(t, static_cast<const T*>(a.y) + ask_at, team, left);
-            if (a.d_xn) ask_row<FOUR, STAGES>(t + per * (uint32_t)sizeof(T), static_cast<const T*>(a.d_xn) + ask_at, team, left);
+            ask_row<FOUR>(t, static_cast<const T*>(a.y) + ask_at, team, left);
+            if (a.d_xn) ask_row<FOUR>(t + per * (uint32_t)sizeof(T), static_cast<const T*>(a.d_xn) + ask_at, team, left);
             ask_at += cols;
         }
         ++asked;
@@ -330,14 +349,14 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
         const int64_t r = r0 + i, at = (live ? r : 0) * cols, mine_at = at + tid * V;
         float next_g[EPT];
         if (EACH) ld_gain<FOUR>(a.gate && r + 1 < r1 ? a.gate + (r + 1) * cols : nullptr, team, tid, cols, next_g);
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES > 2 ? STAGES - 2 : 0) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         pair_t y[EPT / 2], xo[EPT / 2], dn[EPT / 2], d[EPT / 2];
         {
             const char* p = mine + from * stage;
             const T* t = reinterpret_cast<const T*>(half(p));
             auto take = [&](auto place, auto row, pair_t (&v)[EPT / 2]) {
                 float f[EPT];
-                take_row<FOUR, STAGES>(place, row, team, left, f);
+                take_row<FOUR>(place, row, team, left, f);
 #pragma unroll
                 for (int j = 0; j < EPT / 2; ++j) v[j] = pair(f[2 * j], f[2 * j + 1]);
             };
@@ -347,7 +366,7 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
             if (a.d_xn) take(t + per, static_cast<const T*>(a.d_xn) + mine_at, dn);
             from = from + 1 == STAGES ? 0 : from + 1;
         }
-        if (STAGES > 0) ask();   // into the places of the row before
+        ask();   // into the places of the row before
         pair_t sum2[6] = {};
 #pragma unroll
         for (int j = 0; j < EPT / 2; ++j) {
@@ -367,7 +386,7 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
             const float2 t = two(sum2[j]);
             sum[j] = t.x + t.y;
         }
-        team_sums<LANES>(sum, red, turn);
+        team_sums<LANES, PAIR>(sum, red, turn);
         // d = d_out + i2 t + c2 x_out; d_y = i1 u d + c1 y
         const float i2 = rsqrtf(sum[1] * over + a.eps), c2 = -i2 * (i2 * (sum[2] * i2 * over));
         const float i1 = a.post ? rsqrtf(sum[0] * over + a.eps) : 1.0f;
@@ -431,7 +450,7 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         if (which == 0 ? !a.d_w_pre : !a.d_w_post) continue;
-        float* out = a.part_w + (2 * (int64_t)blockIdx.x + which) * cols;
+        float* out = a.part_w + (2 * (int64_t)(PAIR ? blockIdx.x >> 1 : blockIdx.x) + which) * cols;
         if constexpr (LANES != 0) {
             float* part = reinterpret_cast<float*>(smem);   // [team][columns]: no more than a stage
             constexpr int WIDE = L * EPT;
@@ -506,7 +525,7 @@ struct Strips {
     // gate_rows 0: the most strips that any gate_rows gives
     Strips(const asca_ctx* ctx, int64_t rows, int64_t cols, int64_t gate_rows) {
         const int team = team_threads(cols);
-        const int64_t teams = (int64_t)ctx->sm_count * std::max(1, 512 / team);   // what is resident at once: 128 registers a thread
+        const int64_t teams = team > 512 ? ctx->sm_count / 2 : (int64_t)ctx->sm_count * (512 / team);   // what is resident at once: 128 registers a thread
         strip = std::max<int64_t>(1, ceil_div64(rows, teams));
         if (gate_rows > 0 && gate_rows <= 2 * strip) strip = ceil_div64(strip, gate_rows) * gate_rows;
         strips = ceil_div64(rows, strip);
@@ -526,7 +545,7 @@ int check(asca_ctx* ctx, const char* who, const Join& a, int64_t cols, int dtype
     return ASCA_OK;
 }
 
-// MOST: threads of a CTA at most, which is what bounds its registers
+// MOST: threads of a team at most, which is what bounds its registers
 template <template <typename, bool, int, int> class K>
 int launch(asca_ctx* ctx, const Join& a, int dtype, bool four, int64_t teams) {
     const int lanes = team_lanes(a.cols), threads = lanes ? 256 : team_threads(a.cols);
@@ -535,12 +554,12 @@ int launch(asca_ctx* ctx, const Join& a, int dtype, bool four, int64_t teams) {
     auto with = [&](auto t, auto f) {
         using T = decltype(t);
         constexpr bool FOUR = decltype(f)::value;
-        if (lanes == 8) e = K<T, FOUR, 8, 256>::go(grid, threads, ctx->stream, a);
-        else if (lanes == 16) e = K<T, FOUR, 16, 256>::go(grid, threads, ctx->stream, a);
-        else if (lanes == 32) e = K<T, FOUR, 32, 256>::go(grid, threads, ctx->stream, a);
-        else if (threads <= 256) e = K<T, FOUR, 0, 256>::go(grid, threads, ctx->stream, a);
-        else if (threads <= 512) e = K<T, FOUR, 0, 512>::go(grid, threads, ctx->stream, a);
-        else e = K<T, FOUR, 0, 1024>::go(grid, threads, ctx->stream, a);
+        if (lanes == 8) e = K<T, FOUR, 8, 256>::go(ctx, grid, threads, a);
+        else if (lanes == 16) e = K<T, FOUR, 16, 256>::go(ctx, grid, threads, a);
+        else if (lanes == 32) e = K<T, FOUR, 32, 256>::go(ctx, grid, threads, a);
+        else if (threads <= 256) e = K<T, FOUR, 0, 256>::go(ctx, grid, threads, a);
+        else if (threads <= 512) e = K<T, FOUR, 0, 512>::go(ctx, grid, threads, a);
+        else e = K<T, FOUR, 0, 1024>::go(ctx, grid, threads, a);
     };
     auto typed = [&](auto t) {
         if (four) with(t, std::true_type());
@@ -554,22 +573,24 @@ int launch(asca_ctx* ctx, const Join& a, int dtype, bool four, int64_t teams) {
 }
 template <typename T, bool FOUR, int LANES, int MOST>
 struct Fwd {
-    static cudaError_t go(dim3 grid, int threads, cudaStream_t s, const Join& a) {
-        join_fwd_kernel<T, FOUR, LANES, MOST><<<grid, threads, 0, s>>>(a);
+    static cudaError_t go(asca_ctx* ctx, dim3 grid, int threads, const Join& a) {
+        join_fwd_kernel<T, FOUR, LANES, MOST><<<grid, threads, 0, ctx->stream>>>(a);
         return cudaSuccess;
     }
 };
 template <typename T, bool FOUR, int LANES, int MOST>
 struct Bwd {
-    static cudaError_t go(dim3 grid, int threads, cudaStream_t s, const Join& a) {
-        // three rows' places fit twice into an SM up to 256 threads and once up to 512; above that two of bf16, none of f32
-        constexpr int STAGES = MOST <= 512 ? 3 : sizeof(T) == 2 ? 2 : 0;
-        constexpr bool EACH = MOST <= 512;   // (a team of more has no registers for a second gate)
-        auto kern = EACH && a.gate && a.gate_rows == 1 ? join_bwd_kernel<T, FOUR, LANES, MOST, STAGES, EACH> : join_bwd_kernel<T, FOUR, LANES, MOST, STAGES, false>;
-        const size_t smem = STAGES * stage_bytes<T>(threads);
+    static cudaError_t go(asca_ctx* ctx, dim3 grid, int threads, const Join& a) {
+        constexpr bool PAIR = MOST > 512;   // (a thread of a larger CTA would have half of the registers that it needs)
+        constexpr int CTA = PAIR ? MOST / 2 : MOST;
+        const int cta = PAIR ? (threads + 63) / 64 * 32 : threads;
+        auto kern = a.gate && a.gate_rows == 1 ? join_bwd_kernel<T, FOUR, LANES, CTA, PAIR, true> : join_bwd_kernel<T, FOUR, LANES, CTA, PAIR, false>;
+        const size_t smem = STAGES * stage_bytes<T>(cta);
         const cudaError_t e = smem > 40 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
-        if (e == cudaSuccess) kern<<<grid, threads, smem, s>>>(a);
-        return e;
+        if (e != cudaSuccess) return e;
+        if (PAIR) return asca_launch_cluster(ctx, kern, dim3(2 * grid.x), dim3(cta), smem, 2, a);
+        kern<<<grid, cta, smem, ctx->stream>>>(a);
+        return cudaSuccess;
     }
 };
 
