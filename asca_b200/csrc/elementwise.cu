@@ -344,6 +344,7 @@ __global__ void __launch_bounds__(256) adamw_seg_clip_kernel(float* __restrict__
                                                              const float* __restrict__ eps_t, int n_seg, float b1,
                                                              float b2, float wd, __nv_bfloat16* __restrict__ p16,
                                                              const float* __restrict__ norm, float max_norm) {
+    pdl_wait();
     adamw_seg_body<true>(p, g, m, v, seg_off, lr_t, eps_t, n_seg, b1, b2, wd, p16, asca_clip_coefficient(*norm, max_norm));
 }
 __global__ void __launch_bounds__(256) adamw_seg_tab_clip_kernel(float* __restrict__ p, const float* __restrict__ g,
@@ -351,6 +352,7 @@ __global__ void __launch_bounds__(256) adamw_seg_tab_clip_kernel(float* __restri
                                                                  const __grid_constant__ AdamSegTab tab, int n_seg, float b1,
                                                                  float b2, float wd, __nv_bfloat16* __restrict__ p16,
                                                                  const float* __restrict__ norm, float max_norm) {
+    pdl_wait();
     adamw_seg_body<true>(p, g, m, v, tab.off, tab.lr, tab.eps, n_seg, b1, b2, wd, p16, asca_clip_coefficient(*norm, max_norm));
 }
 
@@ -524,8 +526,8 @@ static int adamw_segmented(asca_ctx* ctx, float* p, const float* g, float* m, fl
         for (int i = 0; i < n_seg; ++i) tab.lr[i] = lr_t[i], tab.eps[i] = eps_t[i];
         asca_span sp(ctx, "adamw_seg_kernel", (double)n * (p_bf16 ? 30.0 : 28.0));   // bytes read + written
         if (norm)
-            adamw_seg_tab_clip_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(p, g, m, v, tab, n_seg, beta1, beta2, wd_eff, (__nv_bfloat16*)p_bf16,
-                                                                                 norm, max_norm);
+            ASCA_CUDA(ctx, asca_launch_after(ctx, adamw_seg_tab_clip_kernel, dim3((unsigned)blocks), dim3(256), 0, p, g, m, v, tab, n_seg, beta1, beta2,
+                                             wd_eff, (__nv_bfloat16*)p_bf16, norm, max_norm));
         else
             adamw_seg_tab_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(p, g, m, v, tab, n_seg, beta1, beta2, wd_eff, (__nv_bfloat16*)p_bf16);
         ASCA_CHECK_LAUNCH(ctx);

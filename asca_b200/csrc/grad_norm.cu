@@ -4,8 +4,9 @@
 //
 // A CTA owns an equal, contiguous share of all tensors laid end to end, eight 16-byte loads in flight a thread, and adds the squares in
 // 64 bits, in which neither the square of a large f32 overflows nor that of a small one vanishes, and a long sum loses nothing. A
-// second launch adds the CTAs' sums in a fixed order; up to 2 MiB of gradients one cluster does both in one launch through
-// distributed shared memory. Bound by reading the gradients. The tensors' addresses travel with the launch (no copy in front of
+// second launch adds the CTAs' sums in a fixed order. (One cluster for small gradients, in one launch, takes longer: 331,000 f32 5.5 us
+// by 16 CTAs, 3.7 by two launches.) Bound by reading the gradients (1.09 G f32:
+// 612 us = 7.1 TB/s). The tensors' addresses travel with the launch (no copy in front of
 // it, and a captured graph keeps them), 128 a launch.
 //
 // A norm that is not finite follows the formula: c is 0 for an infinite norm (an infinite gradient then gives NaN), NaN for NaN.
@@ -16,8 +17,8 @@
 
 namespace {
 
-constexpr int MAX_TENSORS = 128, CLUSTER = 8, CTAS_PER_SM = 32, LOADS = 8, GRAIN = 256;
-constexpr int64_t CLUSTER_BYTES = 2 << 20, SHARE = 128 << 10;   // bytes of a CTA at least
+constexpr int MAX_TENSORS = 128, CTAS_PER_SM = 32, LOADS = 8, GRAIN = 256;
+constexpr int64_t LEAST = 4 << 10, MOST = 128 << 10, ONE_CTA = 16 << 10, ONE_WARP = 4 << 10;   // bytes of a CTA, a warp
 struct Tensors {
     void* p[MAX_TENSORS];
     int64_t n[MAX_TENSORS];
@@ -26,7 +27,8 @@ struct Tensors {
     int count;
 };
 
-// f(pointer to the tensor's type, elements) for every tensor's part in this CTA's share
+// f(pointer to the tensor's type, elements, thread, number of threads) for every tensor's part in this CTA's share: all threads for a long
+// one; short ones, which a thread would wait for one after the other, go to the warps in turn.
 template <typename F>
 __device__ __forceinline__ void each_part(const Tensors& t, F f) {
     const int64_t grains = t.off[t.count] / GRAIN, start = grains * blockIdx.x / gridDim.x * GRAIN, end = grains * (blockIdx.x + 1) / gridDim.x * GRAIN;
@@ -39,8 +41,12 @@ __device__ __forceinline__ void each_part(const Tensors& t, F f) {
         const int size = t.bf16[lo] ? 2 : 4;
         const int64_t a = (start > t.off[lo] ? start - t.off[lo] : 0) / size, b = min((end - t.off[lo]) / size, t.n[lo]);
         if (a >= b) continue;   // (in the padding behind a tensor)
-        if (t.bf16[lo]) f(static_cast<__nv_bfloat16*>(t.p[lo]) + a, b - a);
-        else f(static_cast<float*>(t.p[lo]) + a, b - a);
+        auto with = [&](int me, auto threads) {
+            if (t.bf16[lo]) f(static_cast<__nv_bfloat16*>(t.p[lo]) + a, b - a, me, threads);
+            else f(static_cast<float*>(t.p[lo]) + a, b - a, me, threads);
+        };
+        if ((b - a) * size > ONE_WARP) with(threadIdx.x, std::integral_constant<int, 256>());
+        else if ((lo & 7) == (int)threadIdx.x >> 5) with(threadIdx.x & 31, std::integral_constant<int, 32>());
     }
 }
 
@@ -76,12 +82,12 @@ __device__ double block_sum_f64(double v, double* red) {
 // The CTA's sum, in every thread.
 __device__ __forceinline__ double squares(const Tensors& t, double* red) {
     double s[4] = {};
-    each_part(t, [&](auto* p, int64_t n) {
+    each_part(t, [&](auto* p, int64_t n, int me, auto by) {
         using T = std::remove_pointer_t<decltype(p)>;
-        constexpr int G = 16 / sizeof(T);
-        const int head = lead(p, n), threads = blockDim.x;
+        constexpr int G = 16 / sizeof(T), threads = decltype(by)::value;
+        const int head = lead(p, n);
         const int64_t groups = (n - head) / G;
-        int64_t i = threadIdx.x;
+        int64_t i = me;
         for (; i + (LOADS - 1) * threads < groups; i += LOADS * threads) {
             raw_row<G, T> r[LOADS];
 #pragma unroll
@@ -89,45 +95,37 @@ __device__ __forceinline__ double squares(const Tensors& t, double* red) {
 #pragma unroll
             for (int u = 0; u < LOADS; ++u) group_add(s, r[u]);
         }
+        if constexpr (threads == 32) {   // (a short part: all of it in flight)
+            for (; i < groups; i += LOADS * threads) {
+                raw_row<G, T> r[LOADS];
+#pragma unroll
+                for (int u = 0; u < LOADS; ++u) r[u] = ld_raw<G>(p + head + min(i + u * threads, groups - 1) * G);
+#pragma unroll
+                for (int u = 0; u < LOADS; ++u)
+                    if (i + u * threads < groups) group_add(s, r[u]);
+            }
+        }
         for (; i < groups; i += threads) group_add(s, ld_raw<G>(p + head + i * G));
         const int rest = (int)(n - groups * G);   // in front of the groups and behind them
-        for (i = threadIdx.x; i < rest; i += threads) square_add(s[0], to_f32(p[i < head ? i : i + groups * G]));
+        for (i = me; i < rest; i += threads) square_add(s[0], to_f32(p[i < head ? i : i + groups * G]));
     });
     return block_sum_f64((s[0] + s[1]) + (s[2] + s[3]), red);
 }
 
-__global__ void __launch_bounds__(256) norm_parts_kernel(const __grid_constant__ Tensors t, double* __restrict__ part) {
+template <bool ONE>   // the only CTA
+__global__ void __launch_bounds__(256) norm_parts_kernel(const __grid_constant__ Tensors t, double* __restrict__ part, float* __restrict__ norm) {
     __shared__ double red[32];
     pdl_launch_dependents();
     const double s = squares(t, red);
-    if (threadIdx.x == 0) part[blockIdx.x] = s;
-}
-
-// All of it in one cluster.
-__global__ void __launch_bounds__(1024) norm_cluster_kernel(const __grid_constant__ Tensors t, float* __restrict__ norm) {
-    __shared__ double red[32];
-    __shared__ double mine;
-    pdl_wait();   // (the context may launch it early)
-    const double s = squares(t, red);
-    if (threadIdx.x == 0) mine = s;
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        double sum = 0.0;
-        for (uint32_t c = 0; c < CLUSTER; ++c) {
-            uint32_t at;
-            double x;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&mine)), "r"(c));
-            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(x) : "r"(at) : "memory");
-            sum += x;
-        }
-        *norm = (float)sqrt(sum);
-    }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // nobody leaves before its sum is read
+    if (threadIdx.x > 0) return;
+    if constexpr (ONE) *norm = (float)sqrt(s);
+    else part[blockIdx.x] = s;
 }
 
 __global__ void __launch_bounds__(256) norm_join_kernel(const double* __restrict__ part, int n, float* __restrict__ norm) {
     __shared__ double red[32];
     pdl_wait();
+    pdl_launch_dependents();
     double s = 0.0;
     for (int i = threadIdx.x; i < n; i += 256) s += part[i];
     s = block_sum_f64(s, red);
@@ -137,9 +135,9 @@ __global__ void __launch_bounds__(256) norm_join_kernel(const double* __restrict
 __global__ void __launch_bounds__(256) clip_kernel(const __grid_constant__ Tensors t, const float* __restrict__ norm, float max_norm) {
     const float c = asca_clip_coefficient(*norm, max_norm);
     if (c == 1.0f) return;   // nothing changes
-    each_part(t, [&](auto* p, int64_t n) {
+    each_part(t, [&](auto* p, int64_t n, int me, auto by) {
         using T = std::remove_pointer_t<decltype(p)>;
-        constexpr int G = 16 / sizeof(T);
+        constexpr int G = 16 / sizeof(T), threads = decltype(by)::value;
         const int head = lead(p, n);
         const int64_t groups = (n - head) / G;
         auto scale = [&](T* q, const raw_row<G, T>& r) {
@@ -149,17 +147,17 @@ __global__ void __launch_bounds__(256) clip_kernel(const __grid_constant__ Tenso
             for (int e = 0; e < G; ++e) v[e] *= c;
             st_row<G>(q, v);
         };
-        int64_t i = threadIdx.x;
-        for (; i + 3 * 256 < groups; i += 4 * 256) {
+        int64_t i = me;
+        for (; i + 3 * threads < groups; i += 4 * threads) {
             raw_row<G, T> r[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) r[u] = ld_raw<G>(p + head + (i + u * 256) * G);
+            for (int u = 0; u < 4; ++u) r[u] = ld_raw<G>(p + head + (i + u * threads) * G);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) scale(p + head + (i + u * 256) * G, r[u]);
+            for (int u = 0; u < 4; ++u) scale(p + head + (i + u * threads) * G, r[u]);
         }
-        for (; i < groups; i += 256) scale(p + head + i * G, ld_raw<G>(p + head + i * G));
+        for (; i < groups; i += threads) scale(p + head + i * G, ld_raw<G>(p + head + i * G));
         const int rest = (int)(n - groups * G);
-        for (i = threadIdx.x; i < rest; i += 256) {
+        for (i = me; i < rest; i += threads) {
             T* q = p + (i < head ? i : i + groups * G);
             *q = from_f32<T>(c * to_f32<T>(*q));
         }
@@ -192,7 +190,14 @@ Tensors take(void* const* p, const int64_t* n, const int* dtype, int count, int&
     t.count = k;
     return t;
 }
-int ctas_of(const asca_ctx* ctx, const Tensors& t) { return (int)std::min<int64_t>(ceil_div64(t.off[t.count], SHARE), ctx->sm_count * CTAS_PER_SM); }
+// Two CTAs an SM where that leaves each of them a share worth a CTA (8 MB: 5.1 us, 7.1 by shares of 128 KiB; 1.3 MB: 3.7 and 6.0); more
+// CTAs only in shares of 128 KiB (51 MB: 9.5 us, 10.1 by 64). Few small tensors: one CTA,
+// and no second launch.
+int ctas_of(const asca_ctx* ctx, const Tensors& t) {
+    const int64_t all = t.off[t.count], share = std::min(MOST, std::max(LEAST, all / (2 * ctx->sm_count)));
+    if (all <= ONE_CTA && t.count <= 16) return all > 0;
+    return (int)std::min<int64_t>(ceil_div64(all, share), ctx->sm_count * CTAS_PER_SM);
+}
 
 }  // namespace
 
@@ -214,13 +219,13 @@ int asca_grad_norm(asca_ctx* ctx, void* const* grads, const int64_t* n, const in
     for (int at = 0; at < count; ) {
         const Tensors t = take(grads, n, dtype, count, at);
         const int grid = ctas_of(ctx, t);
-        if (parts == 0 && at == count && t.off[t.count] <= CLUSTER_BYTES) {
-            ASCA_CUDA(ctx, asca_launch_cluster(ctx, norm_cluster_kernel, dim3(CLUSTER), dim3(1024), 0, CLUSTER, t, norm));
-            ctx->launches++;
+        if (grid == 0) continue;
+        if (grid == 1 && parts == 0 && at == count) {
+            norm_parts_kernel<true><<<1, 256, 0, ctx->stream>>>(t, nullptr, norm);
+            ASCA_CHECK_LAUNCH(ctx);
             return ASCA_OK;
         }
-        if (grid == 0) continue;
-        norm_parts_kernel<<<(unsigned)grid, 256, 0, ctx->stream>>>(t, part + parts);
+        norm_parts_kernel<false><<<(unsigned)grid, 256, 0, ctx->stream>>>(t, part + parts, nullptr);
         ASCA_CHECK_LAUNCH(ctx);
         parts += grid;
     }

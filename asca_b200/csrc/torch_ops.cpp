@@ -9,6 +9,8 @@
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -100,13 +102,18 @@ struct Call {
         return reinterpret_cast<THPDtype*>(o)->scalar_type;
     }
     T make(at::IntArrayRef shape, at::ScalarType type) const { return T(at::detail::empty_cuda(shape, type, at::Device(at::kCUDA, (c10::DeviceIndex)device), c10::nullopt)); }
-    // scratch (negative: sizes that the entry point will refuse)
+    // scratch of torch's allocator, back in its hands at the end of the call (negative: sizes that the entry point will refuse)
     struct Scratch {
-        T t;
-        void* p() const { return t.defined() ? t.data_ptr() : nullptr; }
-        size_t n() const { return t.defined() ? (size_t)t.numel() : 0; }
+        c10::DataPtr at;
+        size_t bytes = 0;
+        void* p() const { return at.get(); }
+        size_t n() const { return bytes; }
     };
-    Scratch scratch(int64_t bytes) const { return {bytes > 0 ? make({bytes}, at::kByte) : T()}; }
+    Scratch scratch(int64_t bytes) const {
+        if (bytes <= 0) return {};
+        const c10::cuda::CUDAGuard on((c10::DeviceIndex)device);
+        return {c10::cuda::CUDACachingAllocator::get()->allocate((size_t)bytes), (size_t)bytes};
+    }
     void ok(int rc) const {
         if (rc == ASCA_OK) return;
         PyObject* m = PyImport_ImportModule("asca_b200");
