@@ -300,14 +300,14 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const Sum a, int pieces
 // and then owns some rows of the table and some columns, which it clears first where the table is overwritten. A row of up to SHORT
 // tokens is summed by the lanes that share a row, others of the CTA doing other rows meanwhile; a longer one by the whole CTA, each of
 // the lanes beside each other taking tokens in turn.
-constexpr int SHORT = 16;
+constexpr int SHORT = 16, MOST_SMALL = 2048;
 template <int W, int THREADS, typename T>
 __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const stable_sort::Job j, int lanes, int rows) {
     using F = frag<W, T>;
     constexpr int E = F::E;
     extern __shared__ uint32_t sh[];   // keys and tokens, twice; places; counters. Behind the sort: the sums of the lanes beside each other
     __shared__ int32_t wsum[32];
-    __shared__ int32_t long_runs[stable_sort::SMALL / SHORT], n_long;   // where they begin in the sorted order
+    __shared__ int32_t long_runs[MOST_SMALL / SHORT], n_long;   // where they begin in the sorted order
     const int n = (int)j.n, per = (n + THREADS - 1) / THREADS, room = (n + 7) & ~7;
     uint32_t* keys[2] = {sh, sh + room};
     int32_t* items[2] = {reinterpret_cast<int32_t*>(sh) + 2 * room, reinterpret_cast<int32_t*>(sh) + 3 * room};
@@ -425,8 +425,10 @@ struct Plan {
         // short pieces where the tokens are few: 256 threads an SM walk down pieces at once, or the walk is what the call waits for
         piece = MOST_PIECE;
         while (piece > AHEAD && ceil_div64(N, piece) * std::max<int64_t>(8, ceil_div64(d, 4)) < 148 * 256) piece /= 2;
-        // (a CTA of the one launch may have to add its columns of all of dx's rows by itself)
-        small = N <= stable_sort::SMALL && N * d <= (4 << 20);
+        // One launch or three (sort, pieces, join): every CTA of the one sorts all tokens and may have to add its columns of all of dx's
+        // rows by itself. In one launch and in three, N x d: 12 x 768 4.6 us, 6.6; 100 x 2048 of 48,000 70, 80; 2048 x 64 9.5, 10.8; 500 x 777
+        // of 30,000 31.6, 25.6; 1000 x 768 12.7, 9.0; 4096 x 64 of 1751 20.8, 18.6; 4096 x 512 of 48,000 45, 34.
+        small = N <= MOST_SMALL && N * d <= (1 << 18);
         if (small) {
             list = counts = part = 0;
             return;
@@ -517,9 +519,9 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
     a.narrow = d <= 256;
     // What SMs the sort leaves idle clear a part of the table meanwhile, rows that have tokens among them (written over afterwards).
     stable_sort::Fill fill;
-    if (!accumulate && !plan.small && N > stable_sort::SMALL && stable_sort::tiles(N) < ctx->sm_count) {
+    if (!accumulate && !plan.small && stable_sort::tiles(N) < ctx->sm_count) {
         fill.ctas = (int)(ctx->sm_count - stable_sort::tiles(N));
-        a.cleared = std::min<int64_t>(vocab, fill.ctas * (FILL_SHARE / 4) * 2 * plan.passes / d);
+        a.cleared = std::min<int64_t>(vocab, fill.ctas * (FILL_SHARE / 4) * stable_sort::launches(N, plan.passes) / d);
         fill.p = d_table;
         fill.n = a.cleared * d;
     }
@@ -533,13 +535,15 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
         asca_with_dtype(dx, dtype, [&](auto src) {
             using T = std::remove_const_t<std::remove_pointer_t<decltype(src)>>;
             asca_with_width<T, T>(v, [&](auto wd) {
-                stable_sort::with_threads(N, [&](auto threads) {
+                auto by = [&](auto threads) {
                     auto kern = embed_small_kernel<wd(), threads(), T>;
                     const size_t sums = (size_t)threads() * 4 * frag<wd(), T>::E, sorts = stable_sort::smem_bytes(threads(), j.bins);
                     const size_t smem = 4 * (((size_t)N + 7) & ~(size_t)7) * 4 + std::max(sums, sorts);
                     if (smem > 32 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
                     if (e == cudaSuccess) kern<<<grid, threads(), smem, ctx->stream>>>(a, j, lanes, (int)rows);
-                });
+                };
+                if (N <= 256 * stable_sort::PER) by(std::integral_constant<int, 256>());
+                else by(std::integral_constant<int, 512>());
             });
         });
         ASCA_CUDA(ctx, e);

@@ -34,15 +34,15 @@ struct Job {
     int32_t *place, *offsets;     // of a single pass, nullable: where each item went, -1 for key `limit`; the first place of each bin
 };
 
-// Memory that the launches of a sort clear besides: `ctas` more CTAs in each of the two launches of a pass, an equal share a launch. (A sort
-// of more than SMALL items; one of fewer clears nothing.)
+// Memory that the launches of a sort clear besides: `ctas` more CTAs in each of them, an equal share a launch.
 struct Fill {
     float* p = nullptr;
     int64_t n = 0;
     int ctas = 0;
 };
 
-inline int64_t tiles(int64_t n) { return ceil_div64(n, TILE); }
+inline int64_t tiles(int64_t n) { return n <= SMALL ? 1 : ceil_div64(n, TILE); }   // CTAs of a launch
+inline int launches(int64_t n, int passes) { return n <= SMALL ? 1 : 2 * passes; }
 // the table, and the totals of scan_kernel
 inline size_t scratch_bytes(int64_t n, int bins) { return n <= SMALL ? 0 : ((size_t)(tiles(n) + 1) * bins * 4 + 255) & ~(size_t)255; }
 
@@ -214,10 +214,19 @@ inline void with_threads(int64_t n, F f) {
     else f(std::integral_constant<int, 1024>());
 }
 
+// (nothing in front of it on the stream but this sort's own launches, which do not touch that memory: no wait for them)
+__device__ __forceinline__ bool filled(const Fill& fill, int n_tiles) {
+    if ((int)blockIdx.x < n_tiles) return false;
+    pdl_launch_dependents();
+    clear_floats(fill.p, fill.n, (int64_t)(blockIdx.x - n_tiles) * blockDim.x + threadIdx.x, (int64_t)fill.ctas * blockDim.x);
+    return true;
+}
+
 template <int THREADS>
-static __global__ void __launch_bounds__(THREADS) sort_small_kernel(const Job j) {
+static __global__ void __launch_bounds__(THREADS) sort_small_kernel(const Job j, const Fill fill) {
     extern __shared__ __align__(16) int32_t sh[];   // a bin's first place; the warps' counters
     __shared__ int32_t wsum[32];
+    if (filled(fill, 1)) return;
     pdl_launch_dependents();
     uint16_t *counts = reinterpret_cast<uint16_t*>(sh + j.bins), *run = counts + (threadIdx.x >> 5) * j.bins;
     const int n = (int)j.n, per = (n + THREADS - 1) / THREADS;
@@ -230,14 +239,6 @@ static __global__ void __launch_bounds__(THREADS) sort_small_kernel(const Job j)
         put_items(j, pass, t, sh, run);
         __syncthreads();   // (what the next pass reads)
     }
-}
-
-// (nothing in front of it on the stream but this sort's own launches, which do not touch that memory: no wait for them)
-__device__ __forceinline__ bool filled(const Fill& fill, int n_tiles) {
-    if ((int)blockIdx.x < n_tiles) return false;
-    pdl_launch_dependents();
-    clear_floats(fill.p, fill.n, (int64_t)(blockIdx.x - n_tiles) * blockDim.x + threadIdx.x, (int64_t)fill.ctas * blockDim.x);
-    return true;
 }
 
 // counts[tile][bin]
@@ -405,7 +406,7 @@ static inline int sort(asca_ctx* ctx, const Job& j, int32_t* table, const Fill& 
             auto kern = sort_small_kernel<threads()>;
             const size_t smem = smem_bytes(threads(), j.bins);
             if (smem > 40 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e == cudaSuccess) kern<<<1, threads(), smem, ctx->stream>>>(j);
+            if (e == cudaSuccess) kern<<<(unsigned)(1 + fill.ctas), threads(), smem, ctx->stream>>>(j, fill);
         });
         ASCA_CUDA(ctx, e);
         ASCA_CHECK_LAUNCH(ctx);

@@ -65,7 +65,7 @@ EMBED = [  # N, V, d, ids
     (1, 1, 1, "one"), (1, 256, 64, "zipf"), (12, 256, 768, "zipf"), (63, 300, 7, "zipf"), (64, 64, 32, "one"), (65, 70, 33, "distinct"),
     (777, 5, 130, "zipf"), (2048, 256, 64, "zipf"), (2049, 2047, 36, "past"), (5000, 70_001, 20, "zipf"), (4096, 4_200_000, 1, "zipf"),
     (129, 100, 1030, "one"), (40_000, 3, 12, "zipf"), (300, 1000, 8, "padding"), (140_000, 50_000, 4, "zipf"),
-    (1_100_000, 70_000, 2, "zipf"), (9000, 40, 1032, "zipf"), (20_000, 900, 40, "zipf"),
+    (1_100_000, 70_000, 2, "zipf"), (9000, 40, 1032, "zipf"), (20_000, 900, 40, "zipf"), (400, 90, 700, "zipf"), (2048, 31, 128, "zipf"),
 ]
 
 
