@@ -296,18 +296,18 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const Sum a, int pieces
     }
 }
 
-// Few tokens: everything in one launch. Every CTA sorts all of them in its own shared memory (the same few microseconds at the same time)
-// and then owns some rows of the table and some columns, which it clears first where the table is overwritten. A row of up to SHORT
-// tokens is summed by the lanes that share a row, others of the CTA doing other rows meanwhile; a longer one by the whole CTA, each of
+// Few tokens: everything in one launch. A CTA owns some rows of the table and some columns, which it clears first where the table is
+// overwritten; it picks the tokens of its rows from all of them, in their order, and sorts those (2048 x 64: 5.7 us; 9.5 where every
+// CTA sorted all tokens). A row of up to SHORT tokens is summed by the lanes that share a row, others of the CTA doing other rows meanwhile; a longer one by the whole CTA, each of
 // the lanes beside each other taking tokens in turn.
-constexpr int SHORT = 16, MOST_SMALL = 2048;
+constexpr int SHORT = 16;
 template <int W, int THREADS, typename T>
 __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const stable_sort::Job j, int lanes, int rows) {
     using F = frag<W, T>;
     constexpr int E = F::E;
     extern __shared__ uint32_t sh[];   // keys and tokens, twice; places; counters. Behind the sort: the sums of the lanes beside each other
     __shared__ int32_t wsum[32];
-    __shared__ int32_t long_runs[MOST_SMALL / SHORT], n_long;   // where they begin in the sorted order
+    __shared__ int32_t long_runs[stable_sort::SMALL / SHORT], n_long;   // where they begin in the sorted order
     const int n = (int)j.n, per = (n + THREADS - 1) / THREADS, room = (n + 7) & ~7;
     uint32_t* keys[2] = {sh, sh + room};
     int32_t* items[2] = {reinterpret_cast<int32_t*>(sh) + 2 * room, reinterpret_cast<int32_t*>(sh) + 3 * room};
@@ -325,23 +325,51 @@ __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const
             for (int64_t v = v0 + y; v < v1; v += beside) frag<W, float>::put(a.d_table + v * d, c, lanes, d, zero);
     }
     if (threadIdx.x == 0) n_long = 0;
+    int m;   // tokens of the CTA's rows
+    {
+        uint32_t k[stable_sort::PER];
+        unsigned mine[stable_sort::PER];
+        const int lo = (threadIdx.x >> 5) * per * 32 + (threadIdx.x & 31);
+        int of_warp = 0;
+#pragma unroll
+        for (int i = 0; i < stable_sort::PER; ++i) k[i] = i < per && lo + i * 32 < n ? j.ids[lo + i * 32] : 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < stable_sort::PER; ++i) {
+            mine[i] = __ballot_sync(0xffffffffu, k[i] < a.vocab && k[i] - (uint32_t)v0 < (uint32_t)(v1 - v0));
+            of_warp += __popc(mine[i]);
+        }
+        const bool first_lane = (threadIdx.x & 31) == 0;
+        int at = __shfl_sync(0xffffffffu, stable_sort::exclusive_scan<THREADS>(first_lane ? of_warp : 0, wsum, m), 0);
+#pragma unroll
+        for (int i = 0; i < stable_sort::PER; ++i) {
+            const unsigned below = (1u << (threadIdx.x & 31)) - 1u;
+            if (mine[i] >> (threadIdx.x & 31) & 1) {
+                const int p = at + __popc(mine[i] & below);
+                keys[0][p] = k[i] - (uint32_t)v0;
+                items[0][p] = lo + i * 32;
+            }
+            at += __popc(mine[i]);
+        }
+        __syncthreads();
+    }
     int now = 0;
+    const int per_m = (m + THREADS - 1) / THREADS;
     for (int pass = 0; pass < j.passes; ++pass) {
         stable_sort::Items t;
-        const int lo = (threadIdx.x >> 5) * per * 32 + (threadIdx.x & 31);
+        const int lo = (threadIdx.x >> 5) * per_m * 32 + (threadIdx.x & 31);
 #pragma unroll
         for (int i = 0; i < stable_sort::PER; ++i) {
             const int at = lo + i * 32;
             t.item[i] = -1;
             t.key[i] = 0;
-            if (i < per && at < n) {
-                t.key[i] = pass == 0 ? min(j.ids[at], j.limit) : keys[now][at];
-                t.item[i] = pass == 0 ? at : items[now][at];
+            if (i < per_m && at < m) {
+                t.key[i] = keys[now][at];
+                t.item[i] = items[now][at];
             }
         }
         const int shift = pass * j.digit;
         stable_sort::rank_cta<THREADS>(j.bins, shift, mask, counts, first, wsum, t);
-        now ^= pass > 0;
+        now ^= 1;
 #pragma unroll
         for (int i = 0; i < stable_sort::PER; ++i) {
             if (t.item[i] < 0) continue;
@@ -370,12 +398,10 @@ __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const
             }
         }
     };
-    auto bound = [&](uint32_t v) { return (int)lower_bound(key, n, v); };
-    const int p0 = bound((uint32_t)v0), p1 = bound((uint32_t)v1);   // (behind barriers: the zeros are in place)
-    for (int p = p0 + y; p < p1; p += beside) {
-        if (p > p0 && key[p] == key[p - 1]) continue;   // (not where a row's run begins)
+    for (int p = y; p < m; p += beside) {   // (behind barriers: the zeros are in place)
+        if (p > 0 && key[p] == key[p - 1]) continue;   // (not where a row's run begins)
         int end = p + 1;
-        while (end < p1 && key[end] == key[p] && end - p <= SHORT) ++end;
+        while (end < m && key[end] == key[p] && end - p <= SHORT) ++end;
         if (end - p > SHORT) {
             if (x == 0) long_runs[atomicAdd(&n_long, 1)] = p;   // (rows are summed one by one: their order does not matter)
             continue;
@@ -383,13 +409,13 @@ __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const
         if (!in) continue;
         float acc[E] = {};
         sum(p, 1, end, acc);
-        add_row<W>(a.d_table + (int64_t)key[p] * d, c, lanes, d, acc, a.scale, a.accumulate);
+        add_row<W>(a.d_table + (v0 + key[p]) * d, c, lanes, d, acc, a.scale, a.accumulate);
     }
     __syncthreads();
     float* part = reinterpret_cast<float*>(first);   // [lane beside][column lane][E]: the places and counters are no longer needed
     for (int l = 0; l < n_long; ++l) {
-        const int lo = long_runs[l], end = bound(key[lo] + 1);
-        const uint32_t v = key[lo];
+        const int lo = long_runs[l], end = (int)lower_bound(key, m, key[lo] + 1);
+        const int64_t v = v0 + key[lo];
         float acc[E] = {};
         if (in) sum(lo + y, beside, end, acc);
 #pragma unroll
@@ -405,7 +431,7 @@ __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const
         if (y == 0 && in) {
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] = part[x * E + e];
-            add_row<W>(a.d_table + (int64_t)v * d, c, lanes, d, acc, a.scale, a.accumulate);
+            add_row<W>(a.d_table + v * d, c, lanes, d, acc, a.scale, a.accumulate);
         }
         __syncthreads();
     }
@@ -425,10 +451,10 @@ struct Plan {
         // short pieces where the tokens are few: 256 threads an SM walk down pieces at once, or the walk is what the call waits for
         piece = MOST_PIECE;
         while (piece > AHEAD && ceil_div64(N, piece) * std::max<int64_t>(8, ceil_div64(d, 4)) < 148 * 256) piece /= 2;
-        // One launch or three (sort, pieces, join): every CTA of the one sorts all tokens and may have to add its columns of all of dx's
-        // rows by itself. In one launch and in three, N x d: 12 x 768 4.6 us, 6.6; 100 x 2048 of 48,000 70, 80; 2048 x 64 9.5, 10.8; 500 x 777
-        // of 30,000 31.6, 25.6; 1000 x 768 12.7, 9.0; 4096 x 64 of 1751 20.8, 18.6; 4096 x 512 of 48,000 45, 34.
-        small = N <= MOST_SMALL && N * d <= (1 << 18);
+        // One launch or three (sort, pieces, join): every CTA of the one looks at all tokens and may have to add its columns of all of dx's
+        // rows by itself. In one launch and in three, N x d: 12 x 768 4.3 us, 6.6; 100 x 2048 of 48,000 71, 80; 2048 x 64 5.7, 10.8; 4096 x 64
+        // 10.3, 15.6; 1000 x 768 8.8, 9.0; 500 x 777 of 30,000 28.3, 25.4; 2048 x 768 bf16 12.6, 11.4; 4096 x 512 of 48,000 45, 34.
+        small = N <= stable_sort::SMALL && N * d <= (1 << 18);
         if (small) {
             list = counts = part = 0;
             return;
@@ -529,21 +555,24 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
     if (plan.small) {
         int lanes = 1;
         while (lanes < frags && lanes < 64) lanes *= 2;
-        const int64_t across = ceil_div64(frags, lanes), rows = ceil_div64(vocab, std::max<int64_t>(1, ctx->sm_count / across));   // one CTA an SM
+        const int64_t across = ceil_div64(frags, lanes), rows = ceil_div64(vocab, std::max<int64_t>(1, 2 * ctx->sm_count / across));   // two CTAs an SM
         const dim3 grid((unsigned)ceil_div64(vocab, rows), (unsigned)across);
+        int bits = 0;   // keys 0 .. rows - 1 of a CTA
+        while (((int64_t)1 << bits) < rows) ++bits;
+        j.passes = (int)ceil_div64(bits, 11);
+        j.digit = j.passes > 0 ? (int)ceil_div64(bits, j.passes) : 0;
+        j.bins = j.passes == 1 ? (int)rows : 1 << j.digit;
         cudaError_t e = cudaSuccess;
         asca_with_dtype(dx, dtype, [&](auto src) {
             using T = std::remove_const_t<std::remove_pointer_t<decltype(src)>>;
             asca_with_width<T, T>(v, [&](auto wd) {
-                auto by = [&](auto threads) {
+                stable_sort::with_threads(N, [&](auto threads) {
                     auto kern = embed_small_kernel<wd(), threads(), T>;
                     const size_t sums = (size_t)threads() * 4 * frag<wd(), T>::E, sorts = stable_sort::smem_bytes(threads(), j.bins);
                     const size_t smem = 4 * (((size_t)N + 7) & ~(size_t)7) * 4 + std::max(sums, sorts);
                     if (smem > 32 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
                     if (e == cudaSuccess) kern<<<grid, threads(), smem, ctx->stream>>>(a, j, lanes, (int)rows);
-                };
-                if (N <= 256 * stable_sort::PER) by(std::integral_constant<int, 256>());
-                else by(std::integral_constant<int, 512>());
+                });
             });
         });
         ASCA_CUDA(ctx, e);
