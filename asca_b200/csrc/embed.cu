@@ -298,8 +298,9 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const Sum a, int pieces
 
 // Few tokens: everything in one launch. A CTA owns some rows of the table and some columns, which it clears first where the table is
 // overwritten; it picks the tokens of its rows from all of them, in their order, and sorts those (2048 x 64: 5.7 us; 9.5 where every
-// CTA sorted all tokens). A row of up to SHORT tokens is summed by the lanes that share a row, others of the CTA doing other rows meanwhile; a longer one by the whole CTA, each of
-// the lanes beside each other taking tokens in turn.
+// CTA sorted all tokens). A row of up to SHORT tokens is summed by the lanes that share a row, others of the CTA doing other rows
+// meanwhile; a longer one by the whole CTA, each of the lanes beside each other taking tokens in turn. Bound by its launch and the
+// latency of these steps.
 constexpr int SHORT = 16;
 template <int W, int THREADS, typename T>
 __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const stable_sort::Job j, int lanes, int rows) {
@@ -412,25 +413,25 @@ __global__ void __launch_bounds__(THREADS) embed_small_kernel(const Sum a, const
         add_row<W>(a.d_table + (v0 + key[p]) * d, c, lanes, d, acc, a.scale, a.accumulate);
     }
     __syncthreads();
-    float* part = reinterpret_cast<float*>(first);   // [lane beside][column lane][E]: the places and counters are no longer needed
+    float* part = reinterpret_cast<float*>(first);   // [E][thread]: the places and counters are no longer needed
     for (int l = 0; l < n_long; ++l) {
         const int lo = long_runs[l], end = (int)lower_bound(key, m, key[lo] + 1);
         const int64_t v = v0 + key[lo];
         float acc[E] = {};
         if (in) sum(lo + y, beside, end, acc);
 #pragma unroll
-        for (int e = 0; e < E; ++e) part[threadIdx.x * E + e] = acc[e];
+        for (int e = 0; e < E; ++e) part[e * THREADS + threadIdx.x] = acc[e];
         __syncthreads();
         for (int s = beside / 2; s > 0; s /= 2) {
             if (y < s) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) part[threadIdx.x * E + e] += part[(threadIdx.x + s * lanes) * E + e];
+                for (int e = 0; e < E; ++e) part[e * THREADS + threadIdx.x] += part[e * THREADS + threadIdx.x + s * lanes];
             }
             __syncthreads();
         }
         if (y == 0 && in) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = part[x * E + e];
+            for (int e = 0; e < E; ++e) acc[e] = part[e * THREADS + x];
             add_row<W>(a.d_table + v * d, c, lanes, d, acc, a.scale, a.accumulate);
         }
         __syncthreads();
