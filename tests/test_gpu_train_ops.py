@@ -149,6 +149,7 @@ JOIN = [  # rows, cols, rows a gate (None: all), norm after the block, gains
     (100, 128, 10, True, True), (333, 193, 111, True, True), (64, 256, None, False, True), (50, 257, 7, True, False), (1000, 512, 1000, True, True),
     (901, 516, 300, True, True), (2500, 96, 1250, True, True), (4700, 40, 900, False, True), (20, 2048, 3, True, True), (300, 2052, 299, True, True),
     (40, 4099, 13, True, True), (31, 8192, None, True, True), (9, 8191, 4, False, False), (3000, 64, 5, True, True), (1200, 260, 2, True, True),
+    (33, 5000, 1, True, True), (200, 8192, 1, True, True), (300, 4100, 120, True, True), (150, 6001, 50, False, True),
 ]
 
 
