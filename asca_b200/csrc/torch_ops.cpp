@@ -186,7 +186,7 @@ PyObject* tuple(std::initializer_list<PyObject*> items) {
 }
 PyObject* none() { return Py_NewRef(Py_None); }
 
-// A tensor of its own on a part of another's memory.
+// Small outputs of one call share an allocation, which takes half the time of one each: a tensor of its own on a part of it.
 constexpr int64_t SHARED = 1 << 16;   // elements
 T part(const T& whole, int64_t offset, at::IntArrayRef shape) {
     T t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
@@ -293,7 +293,6 @@ PyObject* join_bwd(Call& c) {   // y, x_out, d_xn, d_out, (join), grads
     const char* names[3] = {"d_w_post", "d_gate", "d_w_pre"};
     const T* of[3] = {a.w_post, a.gate, a.w_pre};
     T sums[3], together;
-    // new ones share an allocation where they are small, which takes half the time of one each
     int64_t offset = 0, all = 0;
     for (const T* t : of) all += t ? (t->numel() + 63) / 64 * 64 : 0;
     if (grads == Py_None && all > 0 && all <= SHARED) together = c.make({all}, F32);
@@ -338,7 +337,12 @@ PyObject* moe_dispatch(Call& c) {   // experts, E
     shaped(experts, "experts", {-1, -1});
     contiguous(experts, "experts");
     const int64_t e = c.integer(), n = experts.size(0), k = experts.size(1);
-    const T perm = c.make({n * k}, I32), offsets = c.make({e >= 0 ? e + 1 : 1}, I32), slot = c.make({n, k}, I32);
+    const int64_t bins = e >= 0 ? e + 1 : 1, list = (n * k + 63) / 64 * 64;
+    T perm, offsets, slot;
+    if (2 * list + bins <= SHARED) {
+        const T all = c.make({2 * list + bins}, I32);
+        perm = part(all, 0, {n * k}), slot = part(all, list, {n, k}), offsets = part(all, 2 * list, {bins});
+    } else perm = c.make({n * k}, I32), offsets = c.make({bins}, I32), slot = c.make({n, k}, I32);
     const auto ws = c.scratch(asca_moe_topk_dispatch_ws(n, k, e));
     c.ok(asca_moe_topk_dispatch(c.ctx, ptr<int32_t>(&experts), n, k, e, ptr<int32_t>(&perm), ptr<int32_t>(&offsets), ptr<int32_t>(&slot), ws.p(), ws.n()));
     return tuple({wrap(perm), wrap(offsets), wrap(slot)});
