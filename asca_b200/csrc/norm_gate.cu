@@ -292,6 +292,9 @@ constexpr size_t stage_bytes(int threads) { return (size_t)threads * EPT * (8 + 
 template <typename T, bool FOUR, int LANES, int MOST, bool PAIR, bool EACH>
 __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(const Join a) {
     extern __shared__ __align__(16) char smem[];
+    // Both CTAs of a pair have started before either writes into the other's shared memory (team_sums): arrived at here, waited for in
+    // front of the rows.
+    if (PAIR) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     pdl_wait();   // (the context may launch it early)
     pdl_launch_dependents();
     __shared__ __align__(16) float red[2][32][8];
@@ -347,6 +350,10 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
         ld_gain<FOUR>(a.w_post, team, tid, cols, w);
         ld_gain<FOUR>(a.gate && n > 0 ? a.gate + group * cols : nullptr, team, tid, cols, g);
         set_u(g, w);
+    }
+    if (PAIR) {
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     // (teams that share a warp take the same number of turns)
     for (int i = 0; i < (LANES ? (int)a.strip : n); ++i) {
