@@ -6,6 +6,7 @@
 
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <cmath>
 
 namespace {
@@ -256,8 +257,12 @@ __global__ void __launch_bounds__(256) adamw_kernel(float* __restrict__ p, const
     }
 }
 
-// One launch over a flat buffer of n_seg tensors with per-tensor lr_t / eps_t
-// (the counter advances per tensor, rust/src/tensor.rs:393).
+// A flat buffer of n_seg tensors with per-tensor lr_t / eps_t (the counter advances per tensor, rust/src/tensor.rs:393), by launches
+// of up to 128 of them. A launch's table travels with it by value: a captured graph keeps what it was given, and no copy stands in front
+// of the launch, where it would queue on a copy engine, behind whatever long peer-to-peer transfers the data-parallel exchange has in
+// flight. `begin`: the first element of the launch's first tensor (0 in the first launch).
+constexpr int ADAM_TAB = 128;
+struct AdamSegTab { int64_t off[ADAM_TAB + 1]; float lr[ADAM_TAB], eps[ADAM_TAB]; };
 // CLIP: the gradient enters as clip * g, rounded once, and the update goes on from there as from any gradient: the product is kept
 // from being contracted into the moments, so that the step is bit for bit the plain one on a gradient clipped before.
 __device__ __forceinline__ float clipped(float g, float clip) {
@@ -268,23 +273,21 @@ __device__ __forceinline__ float clipped(float g, float clip) {
 template <bool CLIP>
 __device__ __forceinline__ void adamw_seg_body(float* __restrict__ p, const float* __restrict__ g,
                                                float* __restrict__ m, float* __restrict__ v,
-                                               const int64_t* __restrict__ seg_off,
-                                               const float* __restrict__ lr_t,
-                                               const float* __restrict__ eps_t, int n_seg, float b1,
+                                               const AdamSegTab& tab, int64_t begin, int n_seg, float b1,
                                                float b2, float wd, __nv_bfloat16* __restrict__ p16, float clip = 1.0f) {
-    const int64_t n = seg_off[n_seg];
+    const int64_t n = tab.off[n_seg];
     const int64_t stride = (int64_t)gridDim.x * blockDim.x * 4;
     const bool vec_ok = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m) |
                           reinterpret_cast<uintptr_t>(v)) & 15) == 0;
-    for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4; i < n; i += stride) {
-        int lo = 0, hi = n_seg - 1;  // last segment with seg_off[s] <= i
+    for (int64_t i = begin / 4 * 4 + ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4; i < n; i += stride) {
+        int lo = 0, hi = n_seg - 1;  // last segment with off[s] <= i
         while (lo < hi) {
             int mid = (lo + hi + 1) >> 1;
-            if (seg_off[mid] <= i) lo = mid; else hi = mid - 1;
+            if (tab.off[mid] <= i) lo = mid; else hi = mid - 1;
         }
         int s = lo;
-        float lr = lr_t[s], ep = eps_t[s];
-        if (i + 4 <= seg_off[s + 1] && vec_ok) {   // the common case: four elements of one tensor, 16-byte accesses
+        float lr = tab.lr[s], ep = tab.eps[s];
+        if (i >= begin && i + 4 <= tab.off[s + 1] && vec_ok) {   // the common case: four elements of one tensor, 16-byte accesses
             float4 P = *reinterpret_cast<float4*>(p + i), M = *reinterpret_cast<float4*>(m + i),
                    V = *reinterpret_cast<float4*>(v + i);
             float4 G = *reinterpret_cast<const float4*>(g + i);
@@ -304,56 +307,32 @@ __device__ __forceinline__ void adamw_seg_body(float* __restrict__ p, const floa
             continue;
         }
         const int64_t end = i + 4 < n ? i + 4 : n;
-        for (int64_t j = i; j < end; ++j) {
-            while (j >= seg_off[s + 1]) {
+        for (int64_t j = i < begin ? begin : i; j < end; ++j) {
+            while (j >= tab.off[s + 1]) {
                 ++s;
-                lr = lr_t[s];
-                ep = eps_t[s];
+                lr = tab.lr[s];
+                ep = tab.eps[s];
             }
             adamw_one(p[j], CLIP ? clipped(g[j], clip) : g[j], m[j], v[j], lr, b1, b2, ep, wd);
             if (p16) p16[j] = __float2bfloat16(p[j]);
         }
     }
 }
-__global__ void __launch_bounds__(256) adamw_seg_kernel(float* __restrict__ p, const float* __restrict__ g,
-                                                        float* __restrict__ m, float* __restrict__ v,
-                                                        const int64_t* __restrict__ seg_off,
-                                                        const float* __restrict__ lr_t,
-                                                        const float* __restrict__ eps_t, int n_seg, float b1,
-                                                        float b2, float wd, __nv_bfloat16* __restrict__ p16) {
-    adamw_seg_body<false>(p, g, m, v, seg_off, lr_t, eps_t, n_seg, b1, b2, wd, p16);
-}
-// The same with the segment table passed by value (up to 128 tensors): no host-to-device copy in front of the launch. A
-// copy would queue on a copy engine, behind whatever long peer-to-peer transfers the data-parallel exchange has in flight.
-struct AdamSegTab {
-    int64_t off[129];
-    float lr[128], eps[128];
-};
 __global__ void __launch_bounds__(256) adamw_seg_tab_kernel(float* __restrict__ p, const float* __restrict__ g,
                                                             float* __restrict__ m, float* __restrict__ v,
-                                                            const __grid_constant__ AdamSegTab tab, int n_seg, float b1,
+                                                            const __grid_constant__ AdamSegTab tab, int64_t begin, int n_seg, float b1,
                                                             float b2, float wd, __nv_bfloat16* __restrict__ p16) {
-    adamw_seg_body<false>(p, g, m, v, tab.off, tab.lr, tab.eps, n_seg, b1, b2, wd, p16);
+    adamw_seg_body<false>(p, g, m, v, tab, begin, n_seg, b1, b2, wd, p16);
 }
-// Both with the gradient clipped by its norm (grad_norm.cu), which is read on the device: no pass that rewrites the gradient
+// With the gradient clipped by its norm (grad_norm.cu), which is read on the device: no pass that rewrites the gradient
 // (8 bytes an element of the step's 28), and no wait for the norm on the host.
-__global__ void __launch_bounds__(256) adamw_seg_clip_kernel(float* __restrict__ p, const float* __restrict__ g,
-                                                             float* __restrict__ m, float* __restrict__ v,
-                                                             const int64_t* __restrict__ seg_off,
-                                                             const float* __restrict__ lr_t,
-                                                             const float* __restrict__ eps_t, int n_seg, float b1,
-                                                             float b2, float wd, __nv_bfloat16* __restrict__ p16,
-                                                             const float* __restrict__ norm, float max_norm) {
-    pdl_wait();
-    adamw_seg_body<true>(p, g, m, v, seg_off, lr_t, eps_t, n_seg, b1, b2, wd, p16, asca_clip_coefficient(*norm, max_norm));
-}
 __global__ void __launch_bounds__(256) adamw_seg_tab_clip_kernel(float* __restrict__ p, const float* __restrict__ g,
                                                                  float* __restrict__ m, float* __restrict__ v,
-                                                                 const __grid_constant__ AdamSegTab tab, int n_seg, float b1,
+                                                                 const __grid_constant__ AdamSegTab tab, int64_t begin, int n_seg, float b1,
                                                                  float b2, float wd, __nv_bfloat16* __restrict__ p16,
                                                                  const float* __restrict__ norm, float max_norm) {
     pdl_wait();
-    adamw_seg_body<true>(p, g, m, v, tab.off, tab.lr, tab.eps, n_seg, b1, b2, wd, p16, asca_clip_coefficient(*norm, max_norm));
+    adamw_seg_body<true>(p, g, m, v, tab, begin, n_seg, b1, b2, wd, p16, asca_clip_coefficient(*norm, max_norm));
 }
 
 inline bool warp_rows_ok(int64_t cols, const void* a, const void* b) {
@@ -517,40 +496,22 @@ static int adamw_segmented(asca_ctx* ctx, float* p, const float* g, float* m, fl
         ASCA_REQUIRE(ctx, seg_off[i] <= seg_off[i + 1], "adamw_segmented: offsets must be non-decreasing");
     const int64_t n = seg_off[n_seg];
     if (n == 0) return ASCA_OK;
-    int64_t blocks = ceil_div64(n, 1024);
-    const int64_t cap = (int64_t)ctx->sm_count * 16;
-    if (blocks > cap) blocks = cap;
-    if (n_seg <= 128) {   // the table travels with the launch
+    for (int s0 = 0; s0 < n_seg; s0 += ADAM_TAB) {
+        const int segs = n_seg - s0 < ADAM_TAB ? n_seg - s0 : ADAM_TAB;
+        const int64_t begin = s0 ? std::max<int64_t>(seg_off[s0], 0) : 0, count = seg_off[s0 + segs] - begin;
+        if (count <= 0) continue;   // (empty tensors)
         AdamSegTab tab{};
-        for (int i = 0; i <= n_seg; ++i) tab.off[i] = seg_off[i];
-        for (int i = 0; i < n_seg; ++i) tab.lr[i] = lr_t[i], tab.eps[i] = eps_t[i];
-        asca_span sp(ctx, "adamw_seg_kernel", (double)n * (p_bf16 ? 30.0 : 28.0));   // bytes read + written
+        for (int i = 0; i <= segs; ++i) tab.off[i] = seg_off[s0 + i];
+        for (int i = 0; i < segs; ++i) tab.lr[i] = lr_t[s0 + i], tab.eps[i] = eps_t[s0 + i];
+        const int64_t groups = ceil_div64(count + begin % 4, 4), cap = (int64_t)ctx->sm_count * 16;   // of four elements
+        const dim3 blocks((unsigned)(ceil_div64(groups, 256) < cap ? ceil_div64(groups, 256) : cap));
+        asca_span sp(ctx, "adamw_seg_kernel", (double)count * (p_bf16 ? 30.0 : 28.0));   // bytes read + written
         if (norm)
-            ASCA_CUDA(ctx, asca_launch_after(ctx, adamw_seg_tab_clip_kernel, dim3((unsigned)blocks), dim3(256), 0, p, g, m, v, tab, n_seg, beta1, beta2,
+            ASCA_CUDA(ctx, asca_launch_after(ctx, adamw_seg_tab_clip_kernel, blocks, dim3(256), 0, p, g, m, v, tab, begin, segs, beta1, beta2,
                                              wd_eff, (__nv_bfloat16*)p_bf16, norm, max_norm));
         else
-            adamw_seg_tab_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(p, g, m, v, tab, n_seg, beta1, beta2, wd_eff, (__nv_bfloat16*)p_bf16);
+            adamw_seg_tab_kernel<<<blocks, 256, 0, ctx->stream>>>(p, g, m, v, tab, begin, segs, beta1, beta2, wd_eff, (__nv_bfloat16*)p_bf16);
         ASCA_CHECK_LAUNCH(ctx);
-        return ASCA_OK;
     }
-    // table -> device scratch: [seg_off (n_seg+1) i64][lr_t n_seg f32][eps_t n_seg f32]
-    size_t off_b = (size_t)(n_seg + 1) * 8, f_b = (size_t)n_seg * 4;
-    void* ws;
-    ASCA_TRY(asca_workspace(ctx, off_b + 2 * f_b + 256, &ws));
-    char* w = (char*)ws;
-    ASCA_CUDA(ctx, cudaMemcpyAsync(w, seg_off, off_b, cudaMemcpyHostToDevice, ctx->stream));
-    ASCA_CUDA(ctx, cudaMemcpyAsync(w + off_b, lr_t, f_b, cudaMemcpyHostToDevice, ctx->stream));
-    ASCA_CUDA(ctx, cudaMemcpyAsync(w + off_b + f_b, eps_t, f_b, cudaMemcpyHostToDevice, ctx->stream));
-    // pageable host arrays: the copies above have been staged by the time they return
-    asca_span sp(ctx, "adamw_seg_kernel", (double)n * (p_bf16 ? 30.0 : 28.0));   // bytes read + written
-    if (norm)
-        adamw_seg_clip_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(p, g, m, v, (const int64_t*)w, (const float*)(w + off_b),
-                                                                         (const float*)(w + off_b + f_b), n_seg, beta1, beta2,
-                                                                         wd_eff, (__nv_bfloat16*)p_bf16, norm, max_norm);
-    else
-        adamw_seg_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(p, g, m, v, (const int64_t*)w, (const float*)(w + off_b),
-                                                                     (const float*)(w + off_b + f_b), n_seg, beta1, beta2,
-                                                                     wd_eff, (__nv_bfloat16*)p_bf16);
-    ASCA_CHECK_LAUNCH(ctx);
     return ASCA_OK;
 }

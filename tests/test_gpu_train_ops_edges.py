@@ -1,11 +1,12 @@
 """The operators around the blocks of a training step where their plans change: pairs of CTAs, strips and gate groups, columns one by
 one, several contexts at once, what a graph keeps, what is refused. The statements in 64 bits and their bounds are those of
 test_gpu_train_ops.py."""
+import numpy as np
 import pytest
 import torch
 
 from asca_b200 import ops
-from test_gpu_train_ops import DTYPES, join_case, rand
+from test_gpu_train_ops import DTYPES, U, join_case, rand, within
 from test_gpu_train_ops import test_gated_residual_forward_and_gradients as check_join
 
 pytestmark = pytest.mark.gpu
@@ -24,3 +25,69 @@ def test_first_rows_of_a_pair(gpu, rows, cols, per, dtype):
     for _ in range(50):   # one behind the other: pairs that start while others leave
         again = ops.gated_residual_rmsnorm_bwd(gpu, t["y"], t["x"], d_xn, d_out, **args)
         assert all(torch.equal(v, again[k]) for k, v in first.items())
+
+
+# Optimizer steps over more tensors than one launch's table holds. Offsets that are no multiples of four: a group of four elements on
+# the border of two launches is done by both of them, each its own elements.
+SEGMENTS = [128, 129, 200, 256, 400]
+
+
+def adam_state(n_seg, seed=5):
+    rng = np.random.default_rng(seed)
+    sizes = rng.integers(0, 41, n_seg)
+    sizes[n_seg // 2:n_seg // 2 + 9] = 0   # empty tensors
+    off = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int64)
+    n = int(off[-1])
+    lr, eps = rng.uniform(1e-4, 1e-2, n_seg).astype(np.float32), rng.uniform(1e-8, 1e-6, n_seg).astype(np.float32)
+    return off, lr, eps, [rand(1, n), rand(2, n), rand(3, n, scale=0.1), rand(4, n).square()]
+
+
+@pytest.mark.parametrize("n_seg", SEGMENTS)
+@pytest.mark.parametrize("shift", [0, 1])   # on the 16-byte grid, off it
+@pytest.mark.parametrize("clip", [False, True])
+def test_adamw_of_many_tensors(gpu, n_seg, shift, clip):
+    """Against 64 bits. Roundings: three of a moment (two products, their sum; 1 - beta is exact), four of the second; a root halves
+    what its argument is off by, and it, the sum with eps and the quotient add one each, so the update is off by at most
+    3 u M / D + 5 u |m| / D <= 8 u M / D, M the magnitudes in the first moment and D the denominator; the decay is off by 2 u |p|, the last
+    product and sum by u (|p| + 2 lr M / D)."""
+    off, lr, eps, (g, p, m, v) = adam_state(n_seg)
+    place = lambda t: torch.cat([t.new_zeros(shift), t])[shift:]  # noqa: E731
+    norm = ops.grad_norm(gpu, [g])
+    got, gs = [place(t) for t in (p, m, v)], place(g)
+    ops.adamw_segmented(gpu, got[0], gs, got[1], got[2], off, lr, eps, 0.9, 0.95, 1e-4, **(dict(norm=norm, max_norm=1.0) if clip else {}))
+    assert torch.equal(gs, g)
+    gc = (g * (1.0 / (norm + 1e-6)).clamp(max=1.0) if clip else g).double()   # (rounded to f32 before it enters, as the step does it)
+    b1, b2, wd = (float(np.float32(x)) for x in (0.9, 0.95, 1e-4))
+    per = torch.from_numpy(np.diff(off)).cuda()
+    lr64, eps64 = (torch.from_numpy(x).cuda().double().repeat_interleave(per) for x in (lr, eps))
+    m64, big_m = b1 * m.double() + (1 - b1) * gc, (b1 * m.double()).abs() + ((1 - b1) * gc).abs()
+    v64 = b2 * v.double() + (1 - b2) * gc * gc
+    d64 = v64.sqrt() + eps64
+    within(got[1], m64, 3 * U * big_m, "m")
+    within(got[2], v64, 4.01 * U * v64, "v")
+    within(got[0], p.double() * (1 - wd) - lr64 * m64 / d64, 4 * U * p.double().abs() + 11 * U * lr64 * big_m / d64, "p")
+
+
+@pytest.mark.parametrize("n_seg", SEGMENTS)
+@pytest.mark.parametrize("clip", [False, True])
+def test_a_captured_adamw_keeps_its_rates(gpu, n_seg, clip):
+    """The host arrays belong to the caller again when the call returns."""
+    off, lr, eps, (g, p, m, v) = adam_state(n_seg)
+    want, got = ([t.clone() for t in (p, m, v)] for _ in range(2))
+    kw = dict(norm=ops.grad_norm(gpu, [g]), max_norm=1.0) if clip else {}
+    ops.adamw_segmented(gpu, want[0], g, want[1], want[2], off, lr, eps, 0.9, 0.95, 1e-4, **kw)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    try:
+        with torch.cuda.stream(stream):
+            gpu.use_torch_stream()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                ops.adamw_segmented(gpu, got[0], g, got[1], got[2], off, lr, eps, 0.9, 0.95, 1e-4, **kw)
+            lr[:] = 7.0
+            eps[:] = 1.0
+            graph.replay()
+            stream.synchronize()
+    finally:
+        gpu.use_torch_stream()
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
