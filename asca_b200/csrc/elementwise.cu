@@ -480,6 +480,12 @@ int asca_adamw_segmented_clip(asca_ctx* ctx, float* p, const float* g, float* m,
                               void* p_bf16, const float* norm, float max_norm) {
     if (!ctx) return ASCA_ERR_ARG;
     ASCA_REQUIRE(ctx, norm && max_norm > 0.0f && std::isfinite(max_norm), "adamw_segmented_clip: needs the norm and a positive, finite largest one");
+    if (seg_off && n_seg > 0 && seg_off[n_seg] > 0) {   // (every CTA reads the norm when it begins, some behind others' writes)
+        const int64_t n = seg_off[n_seg];
+        const asca_span_of at(norm, 1, 4);
+        ASCA_REQUIRE(ctx, asca_apart(at, {p, n, 4}) && asca_apart(at, {m, n, 4}) && asca_apart(at, {v, n, 4}) && asca_apart(at, {p_bf16, n, 2}),
+                     "adamw_segmented_clip: the norm lies in what the step writes");
+    }
     asca_device_scope on(ctx);
     return adamw_segmented(ctx, p, g, m, v, seg_off, lr_t, eps_t, n_seg, beta1, beta2, wd_eff, p_bf16, norm, max_norm);
 }

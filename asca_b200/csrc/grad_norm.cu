@@ -242,6 +242,8 @@ int asca_clip_grads(asca_ctx* ctx, void* const* grads, const int64_t* n, const i
     if (!ctx) return ASCA_ERR_ARG;
     ASCA_TRY(check_tensors(ctx, "clip_grads", grads, n, dtype, count));
     ASCA_REQUIRE(ctx, norm && max_norm >= 0.0f && std::isfinite(max_norm), "clip_grads: null pointer, or a largest norm that is none");
+    for (int i = 0; i < count; ++i)   // (every CTA reads the norm when it begins, some behind others' writes)
+        ASCA_REQUIRE(ctx, asca_apart({norm, 1, 4}, {grads[i], n[i], asca_dtype_size(dtype[i])}), "clip_grads: the norm lies in tensor %d", i);
     // an element that two tensors share would be scaled by both
     std::vector<std::pair<uintptr_t, uintptr_t>> span;
     for (int i = 0; i < count; ++i)

@@ -184,7 +184,8 @@ def grad_norm(gpu, grads, out=None):
 
 def clip_grads(gpu, grads, max_norm, norm=None):
     """Scales the tensors in place by min(1, max_norm / (norm + 1e-6)) and returns the norm (1,), taken here unless it is given.
-    Tensors must not overlap. An optimizer step that follows in :func:`adamw_segmented` can clip by itself, without this pass."""
+    Tensors must not overlap, nor have the norm among their elements. An optimizer step that follows in :func:`adamw_segmented` can
+    clip by itself, without this pass."""
     grads = list(grads)
     if norm is None:
         norm = grad_norm(gpu, grads)

@@ -180,9 +180,9 @@ int asca_adamw_segmented_cast(asca_ctx* ctx, float* p, const float* g, float* m,
                               const int64_t* seg_off, const float* lr_t, const float* eps_t, int n_seg,
                               float beta1, float beta2, float wd_eff, void* p_bf16);
 /* Same update with the gradient entering as min(1, max_norm / (norm + 1e-6)) * g: clipping by the norm that asca_grad_norm has
- * left in device memory, without a pass that rewrites the gradient. p_bf16 nullable; max_norm > 0 and finite. In all three forms
- * seg_off, lr_t and eps_t are read before the call returns and travel with the launches (128 tensors each): a captured graph keeps
- * the values that they had. */
+ * left in device memory, without a pass that rewrites the gradient. p_bf16 nullable; max_norm > 0 and finite; norm apart from p, m, v and p_bf16. In
+ * all three forms seg_off, lr_t and eps_t are read before the call returns and travel with the launches (128 tensors each): a
+ * captured graph keeps the values that they had. */
 int asca_adamw_segmented_clip(asca_ctx* ctx, float* p, const float* g, float* m, float* v,
                               const int64_t* seg_off, const float* lr_t, const float* eps_t, int n_seg,
                               float beta1, float beta2, float wd_eff, void* p_bf16, const float* norm, float max_norm);
@@ -196,7 +196,8 @@ int asca_adamw_host(asca_ctx* ctx, float* p, const float* g, float* m, float* v,
  * aligned, the caller's until the call's work has run; calls with scratch of their own may overlap, captured and replayed
  * ones included.
  * asca_clip_grads: g *= min(1, max_norm / (norm + 1e-6)) in place, norm read on the device; nothing is written where the factor
- * is 1. Tensors must not overlap. max_norm >= 0 and finite. A norm that is not finite follows the formula (factor 0, or NaN). */
+ * is 1. Tensors must not overlap, nor have the norm among their elements. max_norm >= 0 and finite. A norm that is not finite
+ * follows the formula (factor 0, or NaN). */
 int64_t asca_grad_norm_ws(asca_ctx* ctx, int count);
 int asca_grad_norm(asca_ctx* ctx, void* const* grads, const int64_t* n, const int* dtype, int count, float* norm,
                    void* ws, size_t ws_bytes);

@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+import asca_b200
 from asca_b200 import ops
 from test_gpu_train_ops import DTYPES, U, join_case, rand, within
 from test_gpu_train_ops import test_gated_residual_forward_and_gradients as check_join
@@ -91,3 +92,24 @@ def test_a_captured_adamw_keeps_its_rates(gpu, n_seg, clip):
     finally:
         gpu.use_torch_stream()
     assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
+def test_a_norm_among_what_is_written_is_refused(gpu):
+    """It would be read by blocks that begin behind the first write."""
+    flat = rand(1, 4000)
+    before = flat.clone()
+    for norm in (flat[:1], flat[3999:], flat[1000:1001]):
+        with pytest.raises(asca_b200.AscaError) as err:
+            ops.clip_grads(gpu, [flat[2000:], flat[:2000]], 1.0, norm=norm)
+        assert err.value.code == -1
+    off, lr, eps = np.array([0, 1000]), np.float32([1e-3]), np.float32([1e-8])
+    p, g, m, v = flat.view(4, 1000)
+    for t in (p, m, v):
+        with pytest.raises(asca_b200.AscaError) as err:
+            ops.adamw_segmented(gpu, p, g, m, v, off, lr, eps, 0.9, 0.95, 0.0, norm=t[500:501], max_norm=1.0)
+        assert err.value.code == -1
+    assert torch.equal(flat, before)
+    room = torch.zeros(9, device="cuda")   # right behind them is apart
+    norm = ops.grad_norm(gpu, [room[:8]], out=room[8:])
+    ops.clip_grads(gpu, [room[:8]], 1.0, norm=norm)
+    assert not room.any()
