@@ -569,9 +569,11 @@ int asca_embed_scaled_bwd(asca_ctx* ctx, const void* dx, const uint32_t* ids, in
             asca_with_width<T, T>(v, [&](auto wd) {
                 stable_sort::with_threads(N, [&](auto threads) {
                     auto kern = embed_small_kernel<wd(), threads(), T>;
-                    const size_t sums = (size_t)threads() * 4 * frag<wd(), T>::E, sorts = stable_sort::smem_bytes(threads(), j.bins);
-                    const size_t smem = 4 * (((size_t)N + 7) & ~(size_t)7) * 4 + std::max(sums, sorts);
-                    if (smem > 32 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+                    auto size = [&](size_t n, int bins) {
+                        return 16 * ((n + 7) & ~(size_t)7) + std::max((size_t)threads() * 4 * frag<wd(), T>::E, stable_sort::smem_bytes(threads(), bins));
+                    };
+                    const size_t smem = size((size_t)N, j.bins);
+                    e = asca_allow_smem(kern, smem, size(threads() * stable_sort::PER, stable_sort::MAX_BINS));
                     if (e == cudaSuccess) kern<<<grid, threads(), smem, ctx->stream>>>(a, j, lanes, (int)rows);
                 });
             });

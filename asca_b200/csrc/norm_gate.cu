@@ -598,7 +598,7 @@ struct Bwd {
         const int cta = PAIR ? (threads + 63) / 64 * 32 : threads;
         auto kern = a.gate && a.gate_rows == 1 ? join_bwd_kernel<T, FOUR, LANES, CTA, PAIR, true> : join_bwd_kernel<T, FOUR, LANES, CTA, PAIR, false>;
         const size_t smem = STAGES * stage_bytes<T>(cta);
-        const cudaError_t e = smem > 40 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+        const cudaError_t e = asca_allow_smem(kern, smem, STAGES * stage_bytes<T>(CTA));
         if (e != cudaSuccess) return e;
         if (PAIR) return asca_launch_cluster(ctx, kern, dim3(2 * grid.x), dim3(cta), smem, 2, a);
         kern<<<grid, cta, smem, ctx->stream>>>(a);

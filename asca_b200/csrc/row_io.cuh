@@ -85,6 +85,13 @@ inline void asca_with_width(int v, F f) {
 }
 
 #ifdef __CUDACC__
+// Lets a kernel have `smem` bytes of dynamic shared memory where that may be more than the 48 KiB that it has anyway, its static arrays
+// (24 KiB at most here) among them. The limit belongs to the kernel on the device, not to a context or a call: `most` is the largest
+// size that any call of the kernel has, so that no call of another context on another thread lowers it in front of this one's launch.
+template <typename K>
+inline cudaError_t asca_allow_smem(K kern, size_t smem, size_t most) {
+    return smem > 24 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) : cudaSuccess;
+}
 // Launches a kernel that begins with pdl_wait() behind the one before it on the stream without waiting for that one's end to be
 // scheduled: a second or third launch of one call then costs about a microsecond less.
 template <typename... KArgs, typename... Args>

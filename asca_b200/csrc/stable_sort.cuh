@@ -405,7 +405,7 @@ static inline int sort(asca_ctx* ctx, const Job& j, int32_t* table, const Fill& 
         with_threads(j.n, [&](auto threads) {
             auto kern = sort_small_kernel<threads()>;
             const size_t smem = smem_bytes(threads(), j.bins);
-            if (smem > 40 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            e = asca_allow_smem(kern, smem, smem_bytes(threads(), MAX_BINS));
             if (e == cudaSuccess) kern<<<(unsigned)(1 + fill.ctas), threads(), smem, ctx->stream>>>(j, fill);
         });
         ASCA_CUDA(ctx, e);
@@ -417,10 +417,7 @@ static inline int sort(asca_ctx* ctx, const Job& j, int32_t* table, const Fill& 
     const bool scanned = (int64_t)n * j.bins > OWN_SCAN;
     int q_log = 0;   // threads a bin
     while (q_log < 5 && (j.bins << (q_log + 1)) <= 512) ++q_log;
-    if (smem > 24 * 1024) {   // (16 KiB of static arrays beside it)
-        ASCA_CUDA(ctx, cudaFuncSetAttribute(place_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        ASCA_CUDA(ctx, cudaFuncSetAttribute(place_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    }
+    ASCA_CUDA(ctx, asca_allow_smem(scanned ? place_kernel<true> : place_kernel<false>, smem, smem_bytes(512, MAX_BINS)));
     auto share = [&](int launch) {
         const int64_t from = fill.n * launch / (2 * j.passes);
         return Fill{fill.p + from, fill.n * (launch + 1) / (2 * j.passes) - from, fill.ctas};

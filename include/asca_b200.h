@@ -180,9 +180,9 @@ int asca_adamw_segmented_cast(asca_ctx* ctx, float* p, const float* g, float* m,
                               const int64_t* seg_off, const float* lr_t, const float* eps_t, int n_seg,
                               float beta1, float beta2, float wd_eff, void* p_bf16);
 /* Same update with the gradient entering as min(1, max_norm / (norm + 1e-6)) * g: clipping by the norm that asca_grad_norm has
- * left in device memory, without a pass that rewrites the gradient. p_bf16 nullable; max_norm > 0 and finite; norm apart from p, m, v and p_bf16. In
- * all three forms seg_off, lr_t and eps_t are read before the call returns and travel with the launches (128 tensors each): a
- * captured graph keeps the values that they had. */
+ * left in device memory, without a pass that rewrites the gradient. p_bf16 nullable; max_norm > 0 and finite; norm
+ * apart from p, m, v and p_bf16. In all three forms seg_off, lr_t and eps_t are read before the call returns and travel with
+ * the launches (128 tensors each): a captured graph keeps the values that they had. */
 int asca_adamw_segmented_clip(asca_ctx* ctx, float* p, const float* g, float* m, float* v,
                               const int64_t* seg_off, const float* lr_t, const float* eps_t, int n_seg,
                               float beta1, float beta2, float wd_eff, void* p_bf16, const float* norm, float max_norm);

@@ -1,13 +1,15 @@
 """The operators around the blocks of a training step where their plans change: pairs of CTAs, strips and gate groups, columns one by
 one, several contexts at once, what a graph keeps, what is refused. The statements in 64 bits and their bounds are those of
 test_gpu_train_ops.py."""
+import threading
+
 import numpy as np
 import pytest
 import torch
 
 import asca_b200
 from asca_b200 import ops
-from test_gpu_train_ops import DTYPES, U, join_case, rand, within
+from test_gpu_train_ops import DTYPES, U, join_case, rand, route, text, within
 from test_gpu_train_ops import test_gated_residual_forward_and_gradients as check_join
 
 pytestmark = pytest.mark.gpu
@@ -113,3 +115,60 @@ def test_a_norm_among_what_is_written_is_refused(gpu):
     norm = ops.grad_norm(gpu, [room[:8]], out=room[8:])
     ops.clip_grads(gpu, [room[:8]], 1.0, norm=norm)
     assert not room.any()
+
+
+# Calls whose shared memory differs, of two contexts on two threads (the C boundary lets go of the interpreter's lock).
+def dispatch_call(g, e):
+    n = 5000
+    experts, ws = route(e, n, 1, e, "any"), torch.empty(g.lib.asca_moe_topk_dispatch_ws(n, 1, e), dtype=torch.uint8, device="cuda")
+    out = [torch.empty(size, dtype=torch.int32, device="cuda") for size in (n, e + 1, n)]
+    call = lambda: g._run("asca_moe_topk_dispatch", experts.data_ptr(), n, 1, e, *[t.data_ptr() for t in out], ws.data_ptr(), ws.numel())  # noqa: E731
+    return call, out, (experts, ws)
+
+
+def few_tokens_call(g, n):
+    d = 64
+    dx, ids, table = rand(1, n, d), text(2, n, 50_000, "zipf"), torch.empty(50_000, d, device="cuda")
+    call = lambda: g._run("asca_embed_scaled_bwd", dx.data_ptr(), ids.data_ptr(), n, d, 50_000, 1.0, 0, 0, table.data_ptr(), None, 0)  # noqa: E731
+    return call, [table], (dx, ids)
+
+
+def join_call(g, cols):
+    y, x, d_xn, d_x, d_y = (rand(i, 8, cols) for i in range(5))
+    ws = torch.empty(g.lib.asca_gated_residual_rmsnorm_bwd_ws(g._ctx, 8, cols), dtype=torch.uint8, device="cuda")
+    call = lambda: g._run("asca_gated_residual_rmsnorm_bwd", y.data_ptr(), x.data_ptr(), d_xn.data_ptr(), None, None, None, 0, None, 1, 1.0, 1.0, 1e-6, 8, cols,  # noqa: E731
+                          asca_b200.F32, 0, d_x.data_ptr(), d_y.data_ptr(), None, None, None, ws.data_ptr(), ws.numel())
+    return call, [d_x, d_y], (y, x, d_xn, ws)
+
+
+@pytest.mark.parametrize("make,sizes", [(dispatch_call, (2048, 1400)), (few_tokens_call, (4096, 3000)), (join_call, (2048, 1400)), (join_call, (8192, 4500))])
+def test_two_contexts_on_two_threads(gpu, make, sizes):
+    contexts = [asca_b200.Gpu(0) for _ in sizes]
+    calls = [make(g, size) for g, size in zip(contexts, sizes)]
+    torch.cuda.synchronize()
+    want = []
+    for g, (call, out, _) in zip(contexts, calls):
+        call()
+        g.sync()
+        want.append([t.clone() for t in out])
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(g, call):
+        for _ in range(1500):
+            try:
+                call()
+            except asca_b200.AscaError as e:
+                errors.append(str(e))
+        g.sync()
+
+    threads = [threading.Thread(target=work, args=(g, c[0])) for g, c in zip(contexts, calls)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, f"{len(errors)} calls, the first: {errors[0]}"
+    for (_, out, _), w in zip(calls, want):
+        assert all(torch.equal(a, b) for a, b in zip(out, w))
+    for g in contexts:
+        g.close()
