@@ -501,7 +501,7 @@ int asca_embed_scaled_fwd(asca_ctx* ctx, const void* table, const uint32_t* ids,
 }
 
 int64_t asca_embed_scaled_bwd_ws(int64_t N, int64_t d, int64_t vocab) {
-    if (N < 0 || d <= 0 || vocab <= 0) return ASCA_ERR_ARG;
+    if (N < 0 || N >= ((int64_t)1 << 31) || d <= 0 || d >= (1 << 30) || vocab <= 0 || vocab >= ((int64_t)1 << 31)) return ASCA_ERR_ARG;   // (as the call)
     return (int64_t)Plan(N, d, vocab).bytes();
 }
 

@@ -189,7 +189,7 @@ int check_rows(asca_ctx* ctx, const char* who, int64_t N, int64_t K, int64_t d, 
 extern "C" {
 
 int64_t asca_moe_topk_dispatch_ws(int64_t N, int64_t K, int64_t E) {
-    if (N < 0 || K <= 0 || K >= (1 << 16) || N >= ((int64_t)1 << 31) / K || E <= 0 || E + 1 > stable_sort::MAX_BINS) return ASCA_ERR_ARG;
+    if (N < 0 || K <= 0 || K >= (1 << 16) || N >= ((int64_t)1 << 31) / K || E <= 0 || E >= stable_sort::MAX_BINS) return ASCA_ERR_ARG;
     return (int64_t)stable_sort::scratch_bytes(N * K, (int)E + 1);   // (few assignments: none)
 }
 
@@ -197,7 +197,7 @@ int asca_moe_topk_dispatch(asca_ctx* ctx, const int32_t* experts, int64_t N, int
                            void* ws, size_t ws_bytes) {
     if (!ctx) return ASCA_ERR_ARG;
     ASCA_TRY(check_rows(ctx, "moe_topk_dispatch", N, K, 1, ASCA_F32, ASCA_F32));
-    ASCA_REQUIRE(ctx, E >= 1 && E + 1 <= stable_sort::MAX_BINS, "moe_topk_dispatch: 1 to %d experts", stable_sort::MAX_BINS - 1);
+    ASCA_REQUIRE(ctx, E >= 1 && E < stable_sort::MAX_BINS, "moe_topk_dispatch: 1 to %d experts", stable_sort::MAX_BINS - 1);
     ASCA_REQUIRE(ctx, offsets, "moe_topk_dispatch: null pointer");
     asca_device_scope on(ctx);
     if (N == 0) {

@@ -637,7 +637,7 @@ int asca_gated_residual_rmsnorm_fwd(asca_ctx* ctx, const void* y, const float* x
 }
 
 int64_t asca_gated_residual_rmsnorm_bwd_ws(asca_ctx* ctx, int64_t rows, int64_t cols) {
-    if (!ctx || rows < 0 || cols <= 0 || cols > MAX_COLS) return ASCA_ERR_ARG;
+    if (!ctx || rows < 0 || rows >= ((int64_t)1 << 31) || cols <= 0 || cols > MAX_COLS) return ASCA_ERR_ARG;
     const Strips s(ctx, rows, cols, 0);
     return (int64_t)(s.part_w(cols) + s.part_g(cols) + 256);
 }

@@ -225,11 +225,12 @@ PyObject* embed_bwd(Call& c) {   // dx, ids, vocab, scale, d_table, accumulate
     const int64_t vocab = c.integer(), d = dx.size(-1), n = ids.numel();
     const float scale = c.number();
     if (vocab <= 0 || d <= 0) raise(PyExc_ValueError, "embed_bwd: the table has no rows or no columns");
+    const int64_t bytes = asca_embed_scaled_bwd_ws(n, d, vocab);
+    if (bytes < 0) c.ok(asca_embed_scaled_bwd(c.ctx, dx.data_ptr(), id, n, d, vocab, scale, type, 0, nullptr, nullptr, 0));   // refused before a table is made
     const bool fresh = c.arg[c.i] == Py_None;
     const T d_table = output(c, "d_table", F32, {vocab, d});
     const bool accumulate = c.truth();
     if (accumulate && fresh) raise(PyExc_ValueError, "embed_bwd: accumulate needs the d_table to add to");
-    const int64_t bytes = asca_embed_scaled_bwd_ws(n, d, vocab);
     const auto ws = c.scratch(bytes);
     c.ok(asca_embed_scaled_bwd(c.ctx, dx.data_ptr(), id, n, d, vocab, scale, type, accumulate, ptr<float>(&d_table), ws.p(), ws.n()));
     return wrap(d_table);
@@ -337,13 +338,15 @@ PyObject* moe_dispatch(Call& c) {   // experts, E
     shaped(experts, "experts", {-1, -1});
     contiguous(experts, "experts");
     const int64_t e = c.integer(), n = experts.size(0), k = experts.size(1);
-    const int64_t bins = e >= 0 ? e + 1 : 1, list = (n * k + 63) / 64 * 64;
+    const int64_t bytes = asca_moe_topk_dispatch_ws(n, k, e);
+    if (bytes < 0) c.ok(asca_moe_topk_dispatch(c.ctx, ptr<int32_t>(&experts), n, k, e, nullptr, nullptr, nullptr, nullptr, 0));   // refused before an output is made
+    const int64_t bins = e + 1, list = (n * k + 63) / 64 * 64;
     T perm, offsets, slot;
     if (2 * list + bins <= SHARED) {
         const T all = c.make({2 * list + bins}, I32);
         perm = part(all, 0, {n * k}), slot = part(all, list, {n, k}), offsets = part(all, 2 * list, {bins});
     } else perm = c.make({n * k}, I32), offsets = c.make({bins}, I32), slot = c.make({n, k}, I32);
-    const auto ws = c.scratch(asca_moe_topk_dispatch_ws(n, k, e));
+    const auto ws = c.scratch(bytes);
     c.ok(asca_moe_topk_dispatch(c.ctx, ptr<int32_t>(&experts), n, k, e, ptr<int32_t>(&perm), ptr<int32_t>(&offsets), ptr<int32_t>(&slot), ws.p(), ws.n()));
     return tuple({wrap(perm), wrap(offsets), wrap(slot)});
 }

@@ -172,3 +172,23 @@ def test_two_contexts_on_two_threads(gpu, make, sizes):
         assert all(torch.equal(a, b) for a, b in zip(out, w))
     for g in contexts:
         g.close()
+
+
+def test_sizes_are_refused_before_memory_is_taken(gpu):
+    experts, ids = torch.zeros(4, 2, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    for bad in (1 << 28, 1 << 31, 1 << 40, (1 << 63) - 1):
+        with pytest.raises(asca_b200.AscaError) as err:
+            ops.moe_topk_dispatch(gpu, experts, bad)
+        assert err.value.code == -1 and "experts" in str(err.value)
+    dx = torch.zeros(4, 1, device="cuda")
+    for bad in (1 << 31, 1 << 40, (1 << 63) - 1):
+        with pytest.raises(asca_b200.AscaError) as err:
+            ops.embed_bwd(gpu, dx, ids, bad)
+        assert err.value.code == -1 and "shape" in str(err.value)
+    assert torch.cuda.max_memory_allocated() - held < 1 << 20
+    # the C boundary's own scratch size: a call of that many rows is refused
+    for bad in (1 << 31, (1 << 63) - 1):
+        assert gpu.lib.asca_gated_residual_rmsnorm_bwd_ws(gpu._ctx, bad, 8) < 0

@@ -42,3 +42,11 @@ def test_norm_and_largest_norm_belong_together():
     for kw in (dict(norm=t), dict(max_norm=1.0)):
         with pytest.raises((ValueError, AssertionError)):
             ops.adamw_segmented(Closed(), t, t, t, t, [0, 8], [1e-3], [1e-8], 0.9, 0.95, 0.0, **kw)
+
+
+def test_scratch_of_sizes_that_the_calls_refuse():
+    lib = asca_b200.load()
+    for bad in (1 << 31, 1 << 40, 1 << 62, (1 << 63) - 1):
+        assert lib.asca_embed_scaled_bwd_ws(4, 8, bad) < 0 and lib.asca_embed_scaled_bwd_ws(bad, 8, 4) < 0 and lib.asca_embed_scaled_bwd_ws(4, bad, 4) < 0
+        assert lib.asca_moe_topk_dispatch_ws(4, 1, bad) < 0 and lib.asca_moe_topk_dispatch_ws(bad, 1, 4) < 0 and lib.asca_moe_topk_dispatch_ws(4, bad, 4) < 0
+    assert lib.asca_embed_scaled_bwd_ws(4, 8, (1 << 31) - 1) == 0 and lib.asca_embed_scaled_bwd_ws((1 << 31) - 1, 8, 4) > 0
