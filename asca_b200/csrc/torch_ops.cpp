@@ -16,6 +16,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <string>
 #include <vector>
@@ -251,6 +252,7 @@ struct JoinArgs {
         gate = c.tensor("gate", true);
         gate_rows = c.none() ? (rows > 0 ? rows : 1) : c.integer();
         if (gate_rows <= 0) raise(PyExc_ValueError, "gate_rows: expected a positive number of rows");
+        gate_rows = std::min(gate_rows, std::max<int64_t>(rows, 1));   // (one gate for all of them)
         if (gate) {
             typed(*gate, "gate", F32);
             shaped(*gate, "gate", {(rows + gate_rows - 1) / gate_rows, cols});

@@ -192,3 +192,19 @@ def test_sizes_are_refused_before_memory_is_taken(gpu):
     # the C boundary's own scratch size: a call of that many rows is refused
     for bad in (1 << 31, (1 << 63) - 1):
         assert gpu.lib.asca_gated_residual_rmsnorm_bwd_ws(gpu._ctx, bad, 8) < 0
+
+
+@pytest.mark.parametrize("rows", [0, 1, 300])
+def test_gate_rows_beyond_the_rows(gpu, rows):
+    """One gate for all rows, however many more rows it would serve."""
+    t, kw = join_case(max(rows, 1), 96, None, True, True, torch.float32)
+    t.update(y=t["y"][:rows], x=t["x"][:rows], gate=t["gate"][:min(rows, 1)])
+    d_xn = rand(7, rows, 96)
+    want = None
+    for per in (max(rows, 1), 1000, 1 << 31, 1 << 40, (1 << 63) - 1):
+        kw["gate_rows"] = per
+        x_out, xn = ops.gated_residual_rmsnorm_fwd(gpu, **t, **kw)
+        got = ops.gated_residual_rmsnorm_bwd(gpu, t["y"], x_out, d_xn, None, gate=t["gate"], w_post=t["w_post"], w_pre=t["w_pre"], **kw)
+        got = [x_out, xn, *got.values()]
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
