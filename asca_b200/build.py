@@ -84,18 +84,27 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return SO
 
 
-def build_torch_ops(force: bool = False) -> Path:
-    """The binding of asca_b200.ops (the library itself has been built). Torch's own libraries are in the process when it is
-    loaded; libasca_b200.so is found beside it."""
+def build_torch_ops(force: bool = False) -> Path | None:
+    """The binding of asca_b200.ops (the library itself has been built), or None where torch is not installed, which nothing else
+    needs. Torch's own libraries are in the process when it is loaded; libasca_b200.so is found beside it. It names the torch and the
+    interpreter that it was built for, and is built again for others."""
     import importlib.util
     import sysconfig
 
     src = CSRC / "torch_ops.cpp"
-    torch = Path(importlib.util.find_spec("torch").origin).parent
-    if not force and not _stale(TORCH_OPS, [src, *sorted(INCLUDE.glob("*.h")), torch / "version.py"]):
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        sys.stderr.write("torch is not installed: asca_b200/_torch_ops.so is not built\n")
+        return None
+    import torch as installed
+
+    torch = Path(spec.origin).parent
+    built_for = f"torch {installed.__version__}, {sysconfig.get_config_var('SOABI')}"
+    if not force and not _stale(TORCH_OPS, [src, *sorted(INCLUDE.glob("*.h"))]) and built_for.encode() in TORCH_OPS.read_bytes():
         return TORCH_OPS
     cuda = Path(nvcc()).resolve().parent.parent
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(installed.compiled_with_cxx11_abi())}", f'-DASCA_BUILT_FOR="{built_for}"',
            "-I", sysconfig.get_paths()["include"], "-I", str(torch / "include"), "-I", str(torch / "include/torch/csrc/api/include"),
            "-I", str(cuda / "include"), str(src), "-o", str(TORCH_OPS), "-L", str(PKG), f"-l:{SO.name}", "-L", str(torch / "lib"),
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]

@@ -503,4 +503,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", "Tensor checks, outpu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__torch_ops(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__torch_ops(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_for", ASCA_BUILT_FOR) != 0) {   // (the torch and the interpreter: asca_b200/build.py)
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

@@ -13,10 +13,25 @@ import torch
 
 from . import BF16, F32, NN, NT, TN, Gpu, _f, _i64, _p  # noqa: F401
 
+
+class _Missing:
+    """In the place of _torch_ops.so where it cannot be loaded: the functions that go through it refuse (there is no slower way in its
+    place), those that need the library alone work."""
+
+    def __init__(self, why):
+        self._why = why
+
+    def __getattr__(self, name):
+        raise ImportError("asca_b200/_torch_ops.so is missing or was built for another torch: build it with `python -m asca_b200.build`") from self._why
+
+
 try:
     from . import _torch_ops as _t
-except ImportError as e:   # no slower way in its place
-    raise ImportError("asca_b200/_torch_ops.so is missing or was built for another torch: build it with `python -m asca_b200.build`") from e
+
+    if not _t.built_for.startswith(f"torch {torch.__version__},"):   # (another torch's tensors may be laid out in another way)
+        raise ImportError(f"built for {_t.built_for}; this is torch {torch.__version__}")
+except ImportError as e:
+    _t = _Missing(e)
 
 
 def _dt(t: torch.Tensor) -> int:

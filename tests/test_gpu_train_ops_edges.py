@@ -1,7 +1,10 @@
 """The operators around the blocks of a training step where their plans change: pairs of CTAs, strips and gate groups, columns one by
 one, several contexts at once, what a graph keeps, what is refused. The statements in 64 bits and their bounds are those of
 test_gpu_train_ops.py."""
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -208,3 +211,20 @@ def test_gate_rows_beyond_the_rows(gpu, rows):
         got = [x_out, xn, *got.values()]
         want = want or got
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+WITHOUT = """
+import sys
+sys.modules["asca_b200._torch_ops"] = None   # not there
+import torch, asca_b200
+from asca_b200 import ops
+gpu = asca_b200.Gpu(0)
+gpu.use_torch_stream()
+a, b = torch.ones(64, 96, device="cuda"), torch.full((96, 32), 2.0, device="cuda")
+assert (ops.gemm(gpu, a, b) == 192).all()
+"""
+
+
+def test_products_without_the_torch_binding():
+    r = subprocess.run([sys.executable, "-c", WITHOUT], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr

@@ -1,4 +1,8 @@
 """What the operators around the blocks of a training step refuse or compute without a GPU."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -50,3 +54,47 @@ def test_scratch_of_sizes_that_the_calls_refuse():
         assert lib.asca_embed_scaled_bwd_ws(4, 8, bad) < 0 and lib.asca_embed_scaled_bwd_ws(bad, 8, 4) < 0 and lib.asca_embed_scaled_bwd_ws(4, bad, 4) < 0
         assert lib.asca_moe_topk_dispatch_ws(4, 1, bad) < 0 and lib.asca_moe_topk_dispatch_ws(bad, 1, 4) < 0 and lib.asca_moe_topk_dispatch_ws(4, bad, 4) < 0
     assert lib.asca_embed_scaled_bwd_ws(4, 8, (1 << 31) - 1) == 0 and lib.asca_embed_scaled_bwd_ws((1 << 31) - 1, 8, 4) > 0
+
+
+WITHOUT = """
+import sys, torch
+{how}
+from asca_b200 import ops
+class Closed:
+    handle, device, bound_stream = 0, 0, 1
+assert all(callable(getattr(ops, f)) for f in ("gemm", "adamw", "rmsnorm_fwd", "moe_fwd", "DeltaHostPipeline"))
+for call in (lambda: ops.embed_fwd(Closed(), None, None), lambda: ops.grad_norm(Closed(), []), lambda: ops.moe_sort_rows(Closed(), None, None)):
+    try:
+        call()
+    except ImportError as e:
+        assert "python -m asca_b200.build" in str(e)
+    else:
+        raise SystemExit("not refused")
+"""
+
+
+@pytest.mark.parametrize("how", ["sys.modules['asca_b200._torch_ops'] = None", "torch.__version__ = '9.9.9'"])   # not there, of another torch
+def test_what_needs_the_library_alone_works_without_the_torch_binding(how):
+    r = subprocess.run([sys.executable, "-c", WITHOUT.replace("{how}", how)], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+
+
+def test_the_torch_binding_is_built_for_the_torch_at_hand(monkeypatch, tmp_path):
+    from asca_b200 import _torch_ops, build
+
+    assert torch.__version__ in _torch_ops.built_for
+    commands = []
+
+    def run(cmd, **_):
+        commands.append(cmd)
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    assert build.build_torch_ops() == build.TORCH_OPS and not commands   # as it is
+    monkeypatch.setattr(torch, "__version__", "9.9.9")
+    for abi in (True, False):
+        monkeypatch.setattr(torch, "compiled_with_cxx11_abi", lambda: abi)
+        build.build_torch_ops()
+        assert f"-D_GLIBCXX_USE_CXX11_ABI={int(abi)}" in commands[-1] and any("9.9.9" in word for word in commands[-1])
+    monkeypatch.setattr("importlib.util.find_spec", lambda name: None)
+    assert build.build_torch_ops() is None and len(commands) == 2
