@@ -228,3 +228,37 @@ assert (ops.gemm(gpu, a, b) == 192).all()
 def test_products_without_the_torch_binding():
     r = subprocess.run([sys.executable, "-c", WITHOUT], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+@pytest.mark.parametrize("K", [1, 2, 3, 4, 5, 8])
+@pytest.mark.parametrize("d", [4, 40, 77, 1028])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_assignments_go_anywhere(gpu, K, d, dtype):
+    """Tokens with no assignment, one or all of them, side by side: where an assignment goes nowhere, nothing of its row is used."""
+    N, E = 160, 7
+    experts = route(K, N, K, E, "any")
+    at = torch.arange(N * K, device="cuda").view(N, K)
+    keep = torch.where((torch.arange(N, device="cuda") // 20 % 2 == 0).unsqueeze(1), at % 7 == 3, at % 3 != 0)   # thin and thick stretches
+    keep[32:48] = False   # whole batches of none
+    experts[~keep] = -1
+    _, offsets, slot = ops.moe_topk_dispatch(gpu, experts, E)
+    n = int(keep.sum())
+    assert int(offsets[-1]) == n
+    ys, weights, d_out = rand(1, N * K, d, dtype=dtype), rand(2, N, K), rand(3, N, d)
+    ys[n:] = float("nan")
+    weights[~keep] = float("nan")
+    token, k = keep.nonzero(as_tuple=True)
+    rows, w = ys.double()[slot[token, k].long()], weights.double()[token, k].unsqueeze(1)
+    z = lambda: torch.zeros(N, d, dtype=torch.float64, device="cuda")  # noqa: E731
+    mass = z().index_add_(0, token, (w * rows).abs())
+    within(ops.moe_unsort_rows(gpu, ys, slot, weights), z().index_add_(0, token, w * rows), (K + 2) * U * mass, "out")
+    d_ys, d_w = ops.moe_unsort_rows_bwd(gpu, d_out, ys, slot, weights, d_ys=torch.full_like(ys, 7.0))
+    want = w * d_out.double()[token]
+    within(d_ys[slot[token, k].long()], want, want.abs() * (torch.finfo(dtype).eps / 2 + 2 * U), "d_ys")
+    assert (d_ys[n:] == 7).all() and not d_w[~keep].any()
+    prod = rows * d_out.double()[token]
+    within(d_w[keep], prod.sum(1), (d + 2) * U * prod.abs().sum(1), "d_w")
+    for _ in range(5):
+        alias = ys.clone()
+        got = ops.moe_unsort_rows_bwd(gpu, d_out, alias, slot, weights, d_ys=alias)
+        assert torch.equal(alias[:n], d_ys[:n]) and torch.equal(got[1], d_w) and alias[n:].isnan().all()
