@@ -201,13 +201,13 @@ __global__ void __launch_bounds__(MOST, 2048 / MOST) join_fwd_kernel(const Join 
     constexpr int TEAMS = LANES ? 256 / (LANES ? LANES : 1) : 1;   // a CTA's
     const int team = LANES ? LANES : blockDim.x, tid = LANES ? threadIdx.x % (LANES ? LANES : 1) : threadIdx.x;
     const int64_t r0 = LANES ? (int64_t)blockIdx.x * TEAMS + threadIdx.x / (LANES ? LANES : 1) : blockIdx.x;
-    const bool live = r0 < a.rows;
-    const int64_t r = live ? r0 : a.rows - 1;   // (a warp's shuffles stay whole)
+    const bool live = LANES == 0 || r0 < a.rows;
+    const int64_t r = live ? r0 : 0;
     int turn = 0;
-    const int cols = a.cols;
+    const int cols = a.cols, there = live ? cols : 0;   // (a team without a row reads none, which may be written over, and shuffles with its warp)
     float y[EPT], x[EPT], w[EPT];
-    ld_cols<FOUR>(static_cast<const T*>(a.y) + r * cols, team, tid, cols, y);
-    ld_cols<FOUR>(a.x + r * cols, team, tid, cols, x);
+    ld_cols<FOUR>(static_cast<const T*>(a.y) + r * cols, team, tid, there, y);
+    ld_cols<FOUR>(a.x + r * cols, team, tid, there, x);
     const float over = 1.0f / (float)cols;
     float s = 0.0f;
     if (a.post) {
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
     const int tid = LANES ? threadIdx.x % L : threadIdx.x + (PAIR ? (blockIdx.x & 1) * blockDim.x : 0);
     const int64_t s = (int64_t)(PAIR ? blockIdx.x >> 1 : blockIdx.x) * TEAMS + (LANES ? threadIdx.x / L : 0);   // the strip
     const int64_t r0 = min(s * a.strip, a.rows), r1 = min(r0 + a.strip, a.rows);
-    const int n = (int)(r1 - r0), left = cols - tid * V;   // columns from this thread's first one on
+    const int n = (int)(r1 - r0), left = n > 0 ? cols - tid * V : 0;   // columns from this thread's first one on
     int turn = 0;
     const float over = 1.0f / (float)cols;
     // rows ahead: the next row to ask for, and this thread's places, [x_out, d_out in f32; y, d_xn][columns][thread] a stage
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(con
     // (teams that share a warp take the same number of turns)
     for (int i = 0; i < (LANES ? (int)a.strip : n); ++i) {
         const bool live = LANES == 0 || i < n;
-        const int64_t r = r0 + i, at = (live ? r : 0) * cols, mine_at = at + tid * V;
+        const int64_t r = r0 + i, at = (live ? r : r1 - 1) * cols, mine_at = at + tid * V;   // (behind its strip a team goes on at its last row)
         float next_g[EPT];
         if (EACH) ld_gain<FOUR>(a.gate && r + 1 < r1 ? a.gate + (r + 1) * cols : nullptr, team, tid, cols, next_g);
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");

@@ -262,3 +262,21 @@ def test_few_assignments_go_anywhere(gpu, K, d, dtype):
         alias = ys.clone()
         got = ops.moe_unsort_rows_bwd(gpu, d_out, alias, slot, weights, d_ys=alias)
         assert torch.equal(alias[:n], d_ys[:n]) and torch.equal(got[1], d_w) and alias[n:].isnan().all()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 5), (37, 64), (150, 100), (9500, 33), (4800, 193), (33, 256), (7, 300), (4, 5000)])   # teams without a row, and strips that end early
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_residual_over_its_inputs(gpu, rows, cols, dtype):
+    code = asca_b200.BF16 if dtype == torch.bfloat16 else asca_b200.F32
+    y, x, d_xn, d_out = rand(1, rows, cols, dtype=dtype), rand(2, rows, cols), rand(3, rows, cols, dtype=dtype), rand(4, rows, cols)
+    x_out, xn = ops.gated_residual_rmsnorm_fwd(gpu, y, x)
+    want = ops.gated_residual_rmsnorm_bwd(gpu, y, x_out, d_xn, d_out)
+    ws = torch.empty(gpu.lib.asca_gated_residual_rmsnorm_bwd_ws(gpu._ctx, rows, cols), dtype=torch.uint8, device="cuda")
+    for _ in range(5):
+        a, b = y.clone(), x.clone()
+        gpu._run("asca_gated_residual_rmsnorm_fwd", a.data_ptr(), b.data_ptr(), None, None, 0, None, 1, 1.0, 1.0, 1e-6, rows, cols, code, b.data_ptr(), a.data_ptr())
+        assert torch.equal(b, x_out) and torch.equal(a, xn)   # x_out over x, xn over y
+        a, b = y.clone(), d_out.clone()
+        gpu._run("asca_gated_residual_rmsnorm_bwd", a.data_ptr(), x_out.data_ptr(), d_xn.data_ptr(), b.data_ptr(), None, None, 0, None, 1, 1.0, 1.0, 1e-6, rows, cols,
+                 code, 0, b.data_ptr(), a.data_ptr(), None, None, None, ws.data_ptr(), ws.numel())
+        assert torch.equal(b, want["d_x"]) and torch.equal(a, want["d_y"])   # d_x over d_out, d_y over y
