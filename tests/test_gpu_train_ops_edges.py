@@ -13,7 +13,9 @@ import torch
 import asca_b200
 from asca_b200 import ops
 from test_gpu_train_ops import DTYPES, U, join_case, rand, route, text, within
+from test_gpu_train_ops import test_embedding_forward_and_gradient as check_embedding
 from test_gpu_train_ops import test_gated_residual_forward_and_gradients as check_join
+from test_gpu_train_ops import unaligned
 
 pytestmark = pytest.mark.gpu
 
@@ -280,3 +282,62 @@ def test_gated_residual_over_its_inputs(gpu, rows, cols, dtype):
         gpu._run("asca_gated_residual_rmsnorm_bwd", a.data_ptr(), x_out.data_ptr(), d_xn.data_ptr(), b.data_ptr(), None, None, 0, None, 1, 1.0, 1.0, 1e-6, rows, cols,
                  code, 0, b.data_ptr(), a.data_ptr(), None, None, None, ws.data_ptr(), ws.numel())
         assert torch.equal(b, want["d_x"]) and torch.equal(a, want["d_y"])   # d_x over d_out, d_y over y
+
+
+# Strips of many rows: several shared gates in one (20,000 x 260 has strips of 17 rows on 148 SMs, rounded up to whole groups), groups
+# over two strips and more, and the narrowest and widest teams alike.
+@pytest.mark.parametrize("rows,cols,per", [(20_000, 260, 3), (20_000, 260, 7), (20_000, 260, 20), (20_000, 260, 33), (20_000, 260, 35), (20_000, 260, 90), (40_001, 64, 3),
+                                           (40_001, 50, 11), (30_000, 100, 2), (30_000, 193, 5), (30_000, 193, 26), (603, 8192, 3), (603, 8192, 7), (603, 8191, 19)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_several_gates_in_a_strip(gpu, rows, cols, per, dtype):
+    check_join(gpu, rows, cols, per, True, True, dtype)
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 64), (300, 260), (2500, 33), (9, 5000)])
+@pytest.mark.parametrize("per", [1, 3, None])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_of_a_gate_and_gains_that_are_ones(gpu, rows, cols, per, dtype):
+    """A null gate or gain is ones; its gradient may be asked for all the same."""
+    per = per or rows
+    groups = -(-rows // per)
+    y, x, d_xn, d_out = rand(1, rows, cols, dtype=dtype), rand(2, rows, cols), rand(3, rows, cols, dtype=dtype), rand(4, rows, cols)
+    ones, gates = torch.ones(cols, device="cuda"), torch.ones(groups, cols, device="cuda")
+    x_out, xn = ops.gated_residual_rmsnorm_fwd(gpu, y, x, gate=gates, gate_rows=per, w_post=ones, w_pre=ones, branch_scale=0.5)
+    plain = ops.gated_residual_rmsnorm_fwd(gpu, y, x, branch_scale=0.5)
+    assert torch.equal(plain[0], x_out) and torch.equal(plain[1], xn)
+    want = ops.gated_residual_rmsnorm_bwd(gpu, y, x_out, d_xn, d_out, gate=gates, gate_rows=per, w_post=ones, w_pre=ones, branch_scale=0.5)
+    d_x, d_y = torch.empty_like(x), torch.empty_like(y)
+    sums = {"d_w_post": torch.full((cols,), 7.0, device="cuda"), "d_gate": torch.full((groups, cols), 7.0, device="cuda"), "d_w_pre": torch.full((cols,), 7.0, device="cuda")}
+    ws = torch.empty(gpu.lib.asca_gated_residual_rmsnorm_bwd_ws(gpu._ctx, rows, cols), dtype=torch.uint8, device="cuda")
+    gpu._run("asca_gated_residual_rmsnorm_bwd", y.data_ptr(), x_out.data_ptr(), d_xn.data_ptr(), d_out.data_ptr(), None, None, per, None, 1, 1.0, 0.5, 1e-6, rows, cols,
+             asca_b200.BF16 if dtype == torch.bfloat16 else asca_b200.F32, 0, d_x.data_ptr(), d_y.data_ptr(), *[t.data_ptr() for t in sums.values()], ws.data_ptr(), ws.numel())
+    assert torch.equal(d_x, want["d_x"]) and torch.equal(d_y, want["d_y"])
+    # the same terms, d being d_x here; a gate a row takes another form of the kernel, which may order them otherwise
+    yd, xd = y.double(), x_out.double()
+    branch = (0.5 * d_x.double() * yd / torch.sqrt((yd * yd).mean(1, keepdim=True) + 1e-6)).abs()
+    pre = (d_xn.double() * xd / torch.sqrt((xd * xd).mean(1, keepdim=True) + 1e-6)).abs()
+    index = torch.arange(rows, device="cuda") // per
+    mass = {"d_w_post": branch.sum(0), "d_gate": torch.zeros(groups, cols, dtype=torch.float64, device="cuda").index_add_(0, index, branch), "d_w_pre": pre.sum(0)}
+    for name, got in sums.items():
+        within(got, want[name].double(), 2.1 * ((min(per, rows) if name == "d_gate" else rows) + 40) * U * mass[name], name)
+
+
+# The embedding's gradient in several launches, columns one by one: short runs, runs over many pieces joined by one and by several
+# lanes beside each other, rows without a token, ids and rows that begin anywhere.
+@pytest.mark.parametrize("N,V,d,kind", [(6000, 300, 193, "zipf"), (5000, 40, 777, "zipf"), (9000, 3, 1031, "zipf"), (4500, 1, 131, "one"), (20_000, 2, 67, "past"),
+                                        (4097, 5000, 65, "distinct"), (300, 20_000, 1001, "zipf"), (6000, 900, 130, "padding"), (30_000, 7, 5, "zipf"), (5000, 70_001, 33, "zipf")])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_embedding_gradient_by_single_columns(gpu, N, V, d, kind, dtype):
+    check_embedding(gpu, N, V, d, kind, dtype)
+
+
+@pytest.mark.parametrize("N,V,d", [(6000, 300, 192), (9000, 4, 1024), (5000, 3000, 64)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_embedding_gradient_off_the_16_byte_grid(gpu, N, V, d, dtype):
+    ids, dx = text(N, N, V, "zipf"), rand(2, N, d, dtype=dtype)
+    want = ops.embed_bwd(gpu, dx, ids, V)
+    live = ids[(ids >= 0) & (ids < V)].long()
+    mass = torch.zeros(V, d, dtype=torch.float64, device="cuda").index_add_(0, live, dx[(ids >= 0) & (ids < V)].double().abs())
+    count = torch.zeros(V, 1, dtype=torch.float64, device="cuda").index_add_(0, live, torch.ones(len(live), 1, dtype=torch.float64, device="cuda"))
+    for got in (ops.embed_bwd(gpu, unaligned(dx), ids, V), ops.embed_bwd(gpu, dx, ids, V, d_table=unaligned(want)), ops.embed_bwd(gpu, unaligned(dx), unaligned(ids), V)):
+        within(got, want.double(), 2 * (count + 2) * U * mass, "d_table")   # both sides off by as much from the sum
