@@ -14,6 +14,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
+#include <utility>
 
 namespace {
 
@@ -245,11 +248,14 @@ int asca_clip_grads(asca_ctx* ctx, void* const* grads, const int64_t* n, const i
     for (int i = 0; i < count; ++i)   // (every CTA reads the norm when it begins, some behind others' writes)
         ASCA_REQUIRE(ctx, asca_apart({norm, 1, 4}, {grads[i], n[i], asca_dtype_size(dtype[i])}), "clip_grads: the norm lies in tensor %d", i);
     // an element that two tensors share would be scaled by both
-    std::vector<std::pair<uintptr_t, uintptr_t>> span;
+    using Span = std::pair<uintptr_t, uintptr_t>;
+    const std::unique_ptr<Span[]> span(new (std::nothrow) Span[(size_t)count + 1]);
+    if (!span) return asca_fail(ctx, ASCA_ERR_OOM, "clip_grads: no host memory for the places of %d tensors", count);
+    int spans = 0;
     for (int i = 0; i < count; ++i)
-        if (n[i] > 0) span.push_back({(uintptr_t)grads[i], (uintptr_t)grads[i] + (size_t)n[i] * asca_dtype_size(dtype[i])});
-    std::sort(span.begin(), span.end());
-    for (size_t i = 1; i < span.size(); ++i) ASCA_REQUIRE(ctx, span[i].first >= span[i - 1].second, "clip_grads: two tensors overlap");
+        if (n[i] > 0) span[spans++] = {(uintptr_t)grads[i], (uintptr_t)grads[i] + (size_t)n[i] * asca_dtype_size(dtype[i])};
+    std::sort(span.get(), span.get() + spans);
+    for (int i = 1; i < spans; ++i) ASCA_REQUIRE(ctx, span[i].first >= span[i - 1].second, "clip_grads: two tensors overlap");
     asca_device_scope on(ctx);
     for (int at = 0; at < count; ) {
         const Tensors t = take(grads, n, dtype, count, at);

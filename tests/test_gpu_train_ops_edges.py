@@ -341,3 +341,32 @@ def test_embedding_gradient_off_the_16_byte_grid(gpu, N, V, d, dtype):
     count = torch.zeros(V, 1, dtype=torch.float64, device="cuda").index_add_(0, live, torch.ones(len(live), 1, dtype=torch.float64, device="cuda"))
     for got in (ops.embed_bwd(gpu, unaligned(dx), ids, V), ops.embed_bwd(gpu, dx, ids, V, d_table=unaligned(want)), ops.embed_bwd(gpu, unaligned(dx), unaligned(ids), V)):
         within(got, want.double(), 2 * (count + 2) * U * mass, "d_table")   # both sides off by as much from the sum
+
+
+LITTLE_MEMORY = """
+import resource
+import numpy as np, torch, asca_b200
+gpu = asca_b200.Gpu(0)
+gpu.use_torch_stream()
+count = 20_000_000
+flat, norm = torch.ones(count, device="cuda"), torch.ones(1, device="cuda")
+at, n, dtype = flat.data_ptr() + 4 * np.arange(count, dtype=np.uint64), np.ones(count, np.int64), np.zeros(count, np.int32)
+torch.cuda.synchronize()
+held = int(next(line for line in open("/proc/self/status") if line.startswith("VmSize")).split()[1]) * 1024
+resource.setrlimit(resource.RLIMIT_AS, (held + (100 << 20), resource.RLIM_INFINITY))
+try:
+    gpu._run("asca_clip_grads", at.ctypes.data, n.ctypes.data, dtype.ctypes.data, count, norm.data_ptr(), 1.0)   # 320 MB of places
+except asca_b200.AscaError as e:
+    assert e.code == -3, e
+else:
+    raise SystemExit("not refused")
+resource.setrlimit(resource.RLIMIT_AS, (resource.RLIM_INFINITY, resource.RLIM_INFINITY))
+torch.cuda.synchronize()
+assert (flat == 1).all()   # the context is usable
+"""
+
+
+def test_clipping_more_tensors_than_the_host_has_memory_for():
+    """An error, not an exception through the C boundary, which would end the process."""
+    r = subprocess.run([sys.executable, "-c", LITTLE_MEMORY], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
