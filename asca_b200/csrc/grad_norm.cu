@@ -6,8 +6,8 @@
 // 64 bits, in which neither the square of a large f32 overflows nor that of a small one vanishes, and a long sum loses nothing. A
 // second launch adds the CTAs' sums in a fixed order. (One cluster for small gradients, in one launch, takes longer: 331,000 f32
 // 5.5 us by 16 CTAs, 4.0 by two launches.) The tensors' addresses travel with the launch (no copy in front of it, and a captured graph
-// keeps them), 128 a launch. Bound by reading the gradients: 1.09 G f32 612 us = 7.1 TB/s, 0.5 G bf16 156 us = 6.4; clipping 0.5 G
-// bf16 in place 345 us = 5.8 TB/s behind its norm.
+// keeps them), 128 a launch. Bound by reading the gradients: 1.09 G f32 613 us = 7.1 TB/s, 0.5 G bf16 162 us = 6.2; clipping 0.5 G
+// bf16 in place 323 us = 6.2 TB/s.
 //
 // A norm that is not finite follows the formula: c is 0 for an infinite norm (an infinite gradient then gives NaN), NaN for NaN.
 #include "row_io.cuh"
@@ -193,8 +193,8 @@ Tensors take(void* const* p, const int64_t* n, const int* dtype, int count, int&
     t.count = k;
     return t;
 }
-// Two CTAs an SM where that leaves each of them a share worth a CTA (8 MB: 5.1 us, 7.1 by shares of 128 KiB; 1.3 MB: 3.7 and 6.0); more
-// CTAs only in shares of 128 KiB (51 MB: 9.5 us, 10.1 by 64). Few small tensors: one CTA,
+// Two CTAs an SM where that leaves each of them a share worth a CTA (8 MB: 4.6 us, 7.1 by shares of 128 KiB; 1.3 MB: 4.0 and 6.0); more
+// CTAs only in shares of 128 KiB (51 MB: 9.0 us, 10.1 by 64). Few small tensors: one CTA,
 // and no second launch.
 int ctas_of(const asca_ctx* ctx, const Tensors& t) {
     const int64_t all = t.off[t.count], share = std::min(MOST, std::max(LEAST, all / (2 * ctx->sm_count)));

@@ -16,16 +16,18 @@
 //
 // A row belongs to a team: lanes of a warp up to 256 columns, else a CTA with eight columns a thread (backward, above 4096 columns, the
 // two CTAs of a cluster, because the column sums take 128 registers a thread); the row stays in registers between its two reductions,
-// so every matrix passes HBM once, which is what bounds both directions: 32,768 x 2048 with bf16 y 121 us forward (6.7 TB/s), 195
-// backward (6.2 TB/s), 160 and 291 with a gate a row. Rows of 64 columns take the backward pass 63 us for 200,000 (3.6 TB/s: a
-// reduction for every 64 columns), rows of 8192 180 us for 4096 (2.9 TB/s: the cluster's barrier waits for the row's stores; a CTA of
-// 1024 threads, with half of the registers, takes 212). The statistics are taken again in the backward pass, whose rows are in
+// so every matrix passes HBM once, which is what bounds both directions: 32,768 x 2048 with bf16 y 120 us forward (6.7 TB/s), 196
+// backward (6.2 TB/s), 157 and 285 with a gate a row. Rows of 64 columns take the backward pass 64 us for 200,000 (3.6 TB/s: a
+// reduction for every 64 columns), rows of 8192 180 us for 4096 (3.4 TB/s; 188 with f32 y, 4.3 TB/s: the cluster's barrier waits for the
+// row's stores; a CTA of 1024 threads, with half of the registers, takes 212 with bf16 y). The statistics are taken again in the backward pass, whose rows are in
 // registers anyway: nothing is kept for it.
 //
 // Backward, a team owns a strip of consecutive rows and the same columns in all of them, so that the column sums stay in its
 // registers; a strip's sums of the gains go out once, a gate's once for every group of rows in the strip, and a second launch adds
 // the strips in a fixed order. A group of rows up to two strips long gets strips that end where groups end: its gate's gradient is
-// then written at once.
+// then written at once. That pays where the strips become little longer by it and costs where they leave CTAs without one: 32,768 x 2048
+// bf16, strips of 111 rows, one gate for all 194 us; groups of 112 rows 194 (210 with the strips as they are), of 128 219 (207), of 200
+// 334 (203), of 222 277 (200), of 300, beyond the rule, 200.
 #include "row_io.cuh"
 
 #include <algorithm>
@@ -288,7 +290,7 @@ template <typename T>
 constexpr size_t stage_bytes(int threads) { return (size_t)threads * EPT * (8 + 2 * sizeof(T)); }
 
 // EACH: every row has a gate of its own, which is asked for a row ahead. (In the other form that costs a shared gate 9 % of the pass;
-// without it a gate a row waits for its gate in every row: 351 us for 32,768 x 2048 where this form takes 297.)
+// without it a gate a row waits for its gate in every row: 351 us for 32,768 x 2048 where this form took 297 beside it.)
 template <typename T, bool FOUR, int LANES, int MOST, bool PAIR, bool EACH>
 __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) join_bwd_kernel(const Join a) {
     extern __shared__ __align__(16) char smem[];
