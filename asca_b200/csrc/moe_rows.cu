@@ -9,7 +9,7 @@
 //   unsort   out[t] = sum_k w[a] ys[slot[a]]             d_ys[slot[a]] = w[a] d_out[t],  d_w[a] = <d_out[t], ys[slot[a]]>
 //
 // All four go by token: a token's row is read (or written) once whatever K is, and the sums over k run in the order of k. Rows at and
-// behind offsets[E] are neither read nor written. Bound by HBM.
+// behind offsets[E] are not written, and no value of theirs is used. Bound by HBM.
 #include "row_io.cuh"
 #include "stable_sort.cuh"
 
@@ -50,9 +50,10 @@ __global__ void __launch_bounds__(256) sort_rows_kernel(const TX* __restrict__ x
 }
 
 // unsort and its gradient: some lanes own PAIRS / KS tokens, KS assignments of each at a time: PAIRS rows of the sorted side in flight.
-// There is no branch around a single load: an assignment that goes nowhere asks for another one's row of the same lanes (`live`), whose
-// value it does not use, and where all of them go nowhere nothing is asked for. (Row 0 in its place would be read although it may lie
-// behind the last expert's, and while another CTA writes d_ys over ys there.)
+// There is no branch around a load. Forward an assignment that goes nowhere asks for row 0 and does not use it (with another
+// assignment's row of the same lanes in its place all loads wait for all slots: 65,536 x 2 x 1024 f32 131 us, 127 here; 16,000 x 4 x 1024
+// 58, 56; rows of single columns gain by it, 40,000 x 3 x 777 99, 123 here). In the gradient, where d_ys may be ys and row 0 another
+// CTA's to write, it asks for a row of the same lanes (`live`), and where all of them go nowhere nothing is asked for: same times.
 constexpr int PAIRS = 4;
 
 // weights null: every weight is one. K = 1: up to 256 lanes a token, so that a block goes over four rows from end to end, which HBM
@@ -72,22 +73,14 @@ __global__ void __launch_bounds__(256) unsort_rows_kernel(const TS* __restrict__
         for (int k0 = 0; k0 < K; k0 += KS) {
             F r[T][KS];
             float w[T][KS];
-            uint32_t s[T][KS], live = ~0u;
+            uint32_t s[T][KS];
 #pragma unroll
             for (int i = 0; i < T; ++i) {
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
                     s[i][j] = t0 + i < N && k0 + j < K ? (uint32_t)slot[(t0 + i) * K + k0 + j] : ~0u;
-                    live = s[i][j] < rows ? s[i][j] : live;
-                }
-            }
-            if (live >= rows) continue;
-#pragma unroll
-            for (int i = 0; i < T; ++i) {
-#pragma unroll
-                for (int j = 0; j < KS; ++j) {   // (weights asked for with the slots: 100,000 x 1024 f32 158 us, 137 here)
                     w[i][j] = s[i][j] < rows && weights ? weights[(t0 + i) * K + k0 + j] : 1.0f;
-                    r[i][j].load(ys + (int64_t)(s[i][j] < rows ? s[i][j] : live) * d, c, lanes, d);
+                    r[i][j].load(ys + (int64_t)(s[i][j] < rows ? s[i][j] : 0) * d, c, lanes, d);
                 }
             }
 #pragma unroll

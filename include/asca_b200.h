@@ -358,7 +358,8 @@ int64_t asca_moe_topk_dispatch_ws(int64_t N, int64_t K, int64_t E);
 int asca_moe_topk_dispatch(asca_ctx* ctx, const int32_t* experts, int64_t N, int64_t K, int64_t E, int32_t* perm,
                            int32_t* offsets, int32_t* slot, void* ws, size_t ws_bytes);
 /* The rows moved there and back, and their gradients. Rows of the sorted side (xs, ys, d_xs, d_ys: N*K x d) at and behind
- * offsets[E] are neither read nor written. Each side has a dtype of its own; sums are f32 in the order of k.
+ * offsets[E] are not written, and no value of theirs is used (asca_moe_unsort_rows and asca_moe_sort_rows_bwd may ask for row 0 where
+ * an assignment goes nowhere). Each side has a dtype of its own; sums are f32 in the order of k.
  *   asca_moe_sort_rows        xs[slot[t,k]] = x[t]
  *   asca_moe_sort_rows_bwd    d_x[t] = sum_k d_xs[slot[t,k]]
  *   asca_moe_unsort_rows      out[t] = sum_k weights[t,k] ys[slot[t,k]]      (weights nullable: ones)
