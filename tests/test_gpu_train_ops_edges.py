@@ -370,3 +370,75 @@ def test_clipping_more_tensors_than_the_host_has_memory_for():
     """An error, not an exception through the C boundary, which would end the process."""
     r = subprocess.run([sys.executable, "-c", LITTLE_MEMORY], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def test_ids_of_either_type_and_any_shape(gpu):
+    table, dx = rand(1, 50, 24), rand(2, 60, 24)
+    ids = text(3, 60, 50, "zipf")
+    x, g = ops.embed_fwd(gpu, table, ids, scale=2.0), ops.embed_bwd(gpu, dx, ids, 50, scale=2.0)
+    unsigned = ids.view(torch.uint32)   # -1 is 2^32 - 1 there
+    for shape in ((60,), (3, 20), (1, 5, 12), (60, 1)):
+        for t in (ids, unsigned):
+            assert torch.equal(ops.embed_fwd(gpu, table, t.view(shape), scale=2.0), x.view(*shape, 24))
+            assert torch.equal(ops.embed_bwd(gpu, dx.view(*shape, 24), t.view(shape), 50, scale=2.0), g)
+    one = ids[ids >= 0][0].view(())   # a single id
+    assert torch.equal(ops.embed_fwd(gpu, table, one), table[int(one)]) and torch.equal(ops.embed_bwd(gpu, dx[0], one, 50)[int(one)], dx[0])
+
+
+def test_parameters_and_inference_mode(gpu):
+    """Tensors that autograd knows are data here; outputs know nothing of it."""
+    t, kw = join_case(40, 96, 10, True, True, torch.float32)
+    d_xn = rand(7, 40, 96)
+
+    def step(t):
+        x_out, xn = ops.gated_residual_rmsnorm_fwd(gpu, **t, **kw)
+        got = ops.gated_residual_rmsnorm_bwd(gpu, t["y"], x_out, d_xn, None, gate=t["gate"], w_post=t["w_post"], w_pre=t["w_pre"], **kw)
+        return [x_out, xn, *got.values(), *ops.moe_topk_dispatch(gpu, route(1, 40, 2, 5, "any"), 5), ops.grad_norm(gpu, list(got.values()))]
+
+    want = step(t)
+    for got in (step({k: torch.nn.Parameter(v) for k, v in t.items()}),):
+        assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(got, want))
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(step(t), want))
+    part = want[4]   # a gradient that shares an allocation is a tensor like any other
+    part.mul_(2.0).requires_grad_()
+    (part * part).sum().backward()
+    assert torch.equal(part.grad, 2 * part.detach())
+
+
+def test_accumulated_and_clipped_in_a_graph(gpu):
+    """Each replay adds once more, and clips what is there."""
+    n, v, d = 5000, 90, 40
+    ids, dx = text(1, n, v, "zipf"), rand(2, n, d)
+    t, kw = join_case(n, d, 300, True, True, torch.float32)
+    d_xn = rand(3, n, d)
+    stream = torch.cuda.Stream()
+    table, loose = torch.zeros(v, d, device="cuda"), rand(4, 1000)
+    sums = {"d_gate": torch.zeros_like(t["gate"]), "d_w_post": torch.zeros(d, device="cuda"), "d_w_pre": torch.zeros(d, device="cuda")}
+
+    def step():
+        ops.embed_bwd(gpu, dx, ids, v, d_table=table, accumulate=True)
+        ops.gated_residual_rmsnorm_bwd(gpu, t["y"], t["x"], d_xn, None, gate=t["gate"], w_post=t["w_post"], w_pre=t["w_pre"], grads=sums, **kw)
+        ops.clip_grads(gpu, [table, *sums.values(), loose], 1.0)
+
+    held = [table, loose, *sums.values()]
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(stream):
+            gpu.use_torch_stream()
+            start = [h.clone() for h in held]
+            for _ in range(3):
+                step()
+            want = [h.clone() for h in held]
+            for h, s in zip(held, start):
+                h.copy_(s)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                step()
+            for _ in range(3):
+                graph.replay()
+            stream.synchronize()
+    finally:
+        gpu.use_torch_stream()
+    assert all(torch.equal(a, b) for a, b in zip(held, want)) and not torch.equal(want[0], start[0])
