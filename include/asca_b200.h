@@ -525,8 +525,9 @@ int asca_model_adamw_step(asca_ctx* ctx, asca_model* m, float lr, float beta1, f
                           float wd);
 /* The gradient norm of the whole buffer (asca_grad_norm), and the optimizer step that clips by it: the gradient enters as
  * min(1, max_norm / (norm + 1e-6)) * grads, the buffer itself is left as it is. norm: host float; nullable in the second, which then
- * does not wait for the device. ASCA_ERR_UNSUPPORTED while a communicator is attached (asca_model_dp_attach). No counterpart in
- * the reference, whose trainer does not clip. */
+ * does not wait for the device. A model's first call allocates the norm and its scratch: not while the stream is captured.
+ * ASCA_ERR_UNSUPPORTED while a communicator is attached (asca_model_dp_attach). No counterpart in the reference, whose trainer
+ * does not clip. */
 int asca_model_grad_norm(asca_ctx* ctx, asca_model* m, float* norm);
 int asca_model_adamw_step_clip(asca_ctx* ctx, asca_model* m, float lr, float beta1, float beta2, float eps, float wd,
                                float max_norm, float* norm);
