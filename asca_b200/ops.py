@@ -28,8 +28,9 @@ class _Missing:
 try:
     from . import _torch_ops as _t
 
-    if not _t.built_for.startswith(f"torch {torch.__version__},"):   # (another torch's tensors may be laid out in another way)
-        raise ImportError(f"built for {_t.built_for}; this is torch {torch.__version__}")
+    _for = getattr(_t, "built_for", "a torch that it does not name")
+    if not _for.startswith(f"torch {torch.__version__},"):   # (another torch's tensors may be laid out in another way)
+        raise ImportError(f"built for {_for}; this is torch {torch.__version__}")
 except ImportError as e:
     _t = _Missing(e)
 

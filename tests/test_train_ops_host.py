@@ -73,7 +73,8 @@ for call in (lambda: ops.embed_fwd(Closed(), None, None), lambda: ops.grad_norm(
 """
 
 
-@pytest.mark.parametrize("how", ["sys.modules['asca_b200._torch_ops'] = None", "torch.__version__ = '9.9.9'"])   # not there, of another torch
+# not there, of another torch, one that does not say of which
+@pytest.mark.parametrize("how", ["sys.modules['asca_b200._torch_ops'] = None", "torch.__version__ = '9.9.9'", "sys.modules['asca_b200._torch_ops'] = type(sys)('old')"])
 def test_what_needs_the_library_alone_works_without_the_torch_binding(how):
     r = subprocess.run([sys.executable, "-c", WITHOUT.replace("{how}", how)], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
