@@ -194,8 +194,7 @@ Tensors take(void* const* p, const int64_t* n, const int* dtype, int count, int&
     return t;
 }
 // Two CTAs an SM where that leaves each of them a share worth a CTA (8 MB: 4.6 us, 7.1 by shares of 128 KiB; 1.3 MB: 4.0 and 6.0); more
-// CTAs only in shares of 128 KiB (51 MB: 9.0 us, 10.1 by 64). Few small tensors: one CTA,
-// and no second launch.
+// CTAs only in shares of 128 KiB (51 MB: 9.0 us, 10.1 by 64). Few small tensors: one CTA, and no second launch.
 int ctas_of(const asca_ctx* ctx, const Tensors& t) {
     const int64_t all = t.off[t.count], share = std::min(MOST, std::max(LEAST, all / (2 * ctx->sm_count)));
     if (all <= ONE_CTA && t.count <= 16) return all > 0;

@@ -19,8 +19,8 @@
 // so every matrix passes HBM once, which is what bounds both directions: 32,768 x 2048 with bf16 y 120 us forward (6.7 TB/s), 196
 // backward (6.2 TB/s), 157 and 285 with a gate a row. Rows of 64 columns take the backward pass 64 us for 200,000 (3.6 TB/s: a
 // reduction for every 64 columns), rows of 8192 180 us for 4096 (3.4 TB/s; 188 with f32 y, 4.3 TB/s: the cluster's barrier waits for the
-// row's stores; a CTA of 1024 threads, with half of the registers, takes 212 with bf16 y). The statistics are taken again in the backward pass, whose rows are in
-// registers anyway: nothing is kept for it.
+// row's stores; a CTA of 1024 threads, with half of the registers, takes 212 with bf16 y). The statistics are taken again in the
+// backward pass, whose rows are in registers anyway: nothing is kept for it.
 //
 // Backward, a team owns a strip of consecutive rows and the same columns in all of them, so that the column sums stay in its
 // registers; a strip's sums of the gains go out once, a gate's once for every group of rows in the strip, and a second launch adds
